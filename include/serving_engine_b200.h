@@ -63,6 +63,7 @@ enum seb_status {
 #define SEB_ERRBIT_TIMEOUT 4u  /* a bounded wait on an mbarrier gave up */
 #define SEB_ERRBIT_KLEN 8u     /* k_len larger than the block table row can hold */
 #define SEB_ERRBIT_META 16u    /* a row / query index outside the metadata arrays */
+#define SEB_ERRBIT_NOBLOCK 32u /* the free list holds fewer blocks than a step needs */
 
 SEB_API const char* seb_version(void);
 SEB_API const char* seb_status_string(int status);
@@ -319,6 +320,91 @@ SEB_API int seb_allreduce_add_rmsnorm(void* const* partial, void* const* x, void
                                       const void* weight, int64_t n_tokens, int32_t hidden, float eps,
                                       int32_t dtype, int32_t rank, int32_t world, int32_t all_ranks,
                                       uint32_t polls, int32_t* err, void* stream);
+
+/* ------------------------------------------------------------------------
+ * The 4-bit KV pool. New: the reference's pool holds the model's element type.
+ *
+ * One layer is two planes k_cache, v_cache of bytes [num_blocks, num_kv_heads,
+ * 9 * head_dim], 16-byte aligned: a row is one kv head of one 16-token block, and
+ * every 64 values of a token's head are a group x ~ scale * n + low with n in 0..15
+ * and scale, low in fp16 (4.5 bits a value; a group of equal values is exact to
+ * fp16). csrc/q4_format.cuh gives the order of the bytes. seb_copy_blocks copies such
+ * a pool too ([num_layers, 2, num_blocks, ...], block_bytes = 9 * head_dim *
+ * num_kv_heads). head_dim 64, 128 or 256.
+ * ------------------------------------------------------------------------ */
+
+/* seb_kv_append for a 4-bit pool: quantises k_new and v_new (bf16 or fp16) into the
+ * tokens' slots. Values beyond +-65504 are clamped; a group that holds an infinity or
+ * a NaN reads back as NaN. Out-of-range slots set SEB_ERRBIT_SLOT and are skipped. */
+SEB_API int seb_kv_append_q4(const void* k_new, int64_t k_stride_token, int64_t k_stride_head,
+                             const void* v_new, int64_t v_stride_token, int64_t v_stride_head,
+                             int64_t n_tokens, const int64_t* slot_mapping, void* k_cache, void* v_cache,
+                             int64_t num_blocks, int32_t num_kv_heads, int32_t head_dim, int32_t dtype,
+                             int32_t* err, void* stream);
+
+/* The values of the given slots: k_out, v_out [n_tokens, num_kv_heads, head_dim] of
+ * any element type, contiguous and 16-byte aligned. An out-of-range slot sets
+ * SEB_ERRBIT_SLOT and gives zeros. */
+SEB_API int seb_kv_gather_q4(const void* k_cache, const void* v_cache, int64_t num_blocks,
+                             int32_t num_kv_heads, int32_t head_dim, const int64_t* slots, int64_t n_tokens,
+                             void* k_out, void* v_out, int32_t dtype, int32_t* err, void* stream);
+
+/* seb_rope_kv_append with an RMSNorm of every query and key head in front of the
+ * rotation: y = x * rsqrt(mean(x^2) + eps) * weight over the head's head_dim values,
+ * then y * cos + rotate_half(y) * sin, all in fp32 and rounded once to the element
+ * type. q_weight, k_weight: [head_dim], either may be NULL (that kind of head is not
+ * normed). cache_bits: 16 (a pool of the element type, as seb_kv_append) or 4 (a 4-bit
+ * pool; keys are rounded to the element type, then quantised). */
+SEB_API int seb_qk_norm_rope_append(const void* qkv, int64_t qkv_stride_token, int64_t n_tokens,
+                                    int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, const void* cos,
+                                    const void* sin, int64_t cos_sin_stride_token, const void* q_weight,
+                                    const void* k_weight, float eps, const int64_t* slot_mapping, void* q_out,
+                                    int64_t q_out_stride_token, void* k_cache, void* v_cache, int64_t num_blocks,
+                                    int32_t cache_bits, int32_t dtype, int32_t* err, void* stream);
+
+/* Paged attention over a 4-bit pool, for rows of any q_len: row r's tokens are
+ * q_starts[r] .. + q_lens[r], at positions q_pos_offsets[r] and on, and see the keys
+ * j < k_lens[r] (causal: j <= position). q, out: bf16 or fp16; the sums are fp32. A
+ * query that sees no key gets O = 0 and LSE = -inf; tokens of no row are left as they
+ * are. Rows' token ranges must not overlap. A block id out of range sets
+ * SEB_ERRBIT_BLOCK_ID and its keys count as masked; a k_len beyond the table sets
+ * SEB_ERRBIT_KLEN and ends there; a row outside total_query sets SEB_ERRBIT_META and
+ * is skipped. workspace: seb_paged_attention_q4_workspace_size(...) bytes. */
+SEB_API int64_t seb_paged_attention_q4_workspace_size(int32_t num_rows, int32_t total_query, int32_t num_q_heads,
+                                                      int32_t num_kv_heads, int32_t head_dim);
+
+SEB_API int seb_paged_attention_q4(const void* q, int64_t q_stride_token, int64_t q_stride_head,
+                                   const void* k_cache, const void* v_cache, int64_t num_blocks,
+                                   const int32_t* block_table, int64_t block_table_stride, int64_t max_blocks,
+                                   const int32_t* q_starts, const int32_t* q_lens, const int32_t* k_lens,
+                                   const int32_t* q_pos_offsets, int32_t num_rows, int32_t total_query,
+                                   int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int32_t dtype,
+                                   float scale, int32_t is_causal, void* out, int64_t out_stride_token,
+                                   int64_t out_stride_head, float* lse, int64_t lse_stride_token, void* workspace,
+                                   int64_t workspace_bytes, int32_t* err, void* stream);
+
+/* A step's metadata from request lengths that are on the GPU (what the engine's host
+ * code computes at serving_engine/block_manager.py:87-111, model_runner.py:127-170 and
+ * paged_attention_kernel.py:163-200). Row r holds context_lens[r] tokens and adds
+ * q_lens[r]: q_starts, k_lens and q_pos_offsets as in build_paged_batch_metadata, and
+ * for each token its row, its position and its slot. A row's new blocks, those past
+ * ceil(context / 16), come from the free list in row order and are written to its row
+ * of block_table [num_rows, max_blocks]; the other entries are read.
+ * free_ids is a ring of free_capacity block ids of which free_state = {head, count}
+ * are free; free_next receives the state after the step (a separate array, so a call
+ * can be repeated). total_query is the length of the token arrays; places past the
+ * rows' tokens get row -1, position 0 and slot -1.
+ * Where the list is too short the block and its tokens' slots are -1 and
+ * SEB_ERRBIT_NOBLOCK is set; a k_len beyond the table sets SEB_ERRBIT_KLEN (slots -1,
+ * no block taken); negative lengths (taken as 0), more tokens than total_query and a
+ * free_state outside the ring (taken as empty) set SEB_ERRBIT_META.
+ * num_rows <= 16384. */
+SEB_API int seb_step_tables(const int32_t* q_lens, const int32_t* context_lens, int32_t num_rows,
+                            int32_t total_query, int32_t* block_table, int64_t block_table_stride,
+                            int64_t max_blocks, const int32_t* free_ids, int32_t free_capacity,
+                            const int32_t* free_state, int32_t* q_starts, int32_t* k_lens,
+                            int32_t* q_pos_offsets, int32_t* item_row, int64_t* positions, int64_t* slot_mapping,
+                            int32_t* free_next, int32_t* err, void* stream);
 
 /* Self-test of the bounded waits every kernel uses (no counterpart in the
  * reference, which has no device-side waits): one launch waits `polls` times

@@ -14,13 +14,14 @@ from .build import LIB_PATH
 
 SEB_F32, SEB_F16, SEB_BF16 = 0, 1, 2
 SEB_OK, SEB_EINVAL, SEB_EUNSUPPORTED, SEB_ECUDA, SEB_EWORKSPACE = 0, 1, 2, 3, 4
-ERRBIT_BLOCK_ID, ERRBIT_SLOT, ERRBIT_TIMEOUT, ERRBIT_KLEN, ERRBIT_META = 1, 2, 4, 8, 16
+ERRBIT_BLOCK_ID, ERRBIT_SLOT, ERRBIT_TIMEOUT, ERRBIT_KLEN, ERRBIT_META, ERRBIT_NOBLOCK = 1, 2, 4, 8, 16, 32
 ERRBIT_NAMES = {
     ERRBIT_BLOCK_ID: "block id out of range",
     ERRBIT_SLOT: "slot out of range",
     ERRBIT_TIMEOUT: "bounded wait timed out",
     ERRBIT_KLEN: "k_len exceeds block table row",
     ERRBIT_META: "row/query index out of range",
+    ERRBIT_NOBLOCK: "free list holds too few blocks",
 }
 
 # name -> (restype, argtypes); must match include/serving_engine_b200.h
@@ -104,6 +105,47 @@ SIGNATURES = {
          c_void_p],
     ),
     "seb_swiglu": (c_int32, [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int32, c_int32, c_void_p]),
+    "seb_kv_append_q4": (
+        c_int32,
+        [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p,
+         c_void_p, c_int64, c_int32, c_int32, c_int32, c_void_p, c_void_p],
+    ),
+    "seb_kv_gather_q4": (
+        c_int32,
+        [c_void_p, c_void_p, c_int64, c_int32, c_int32, c_void_p, c_int64, c_void_p, c_void_p, c_int32, c_void_p,
+         c_void_p],
+    ),
+    "seb_qk_norm_rope_append": (
+        c_int32,
+        [c_void_p, c_int64, c_int64, c_int32, c_int32, c_int32,  # qkv, stride, n_tokens, hq, hkv, head_dim
+         c_void_p, c_void_p, c_int64,                            # cos, sin, stride
+         c_void_p, c_void_p, c_float,                            # q_weight, k_weight, eps
+         c_void_p, c_void_p, c_int64,                            # slot_mapping, q_out, stride
+         c_void_p, c_void_p, c_int64, c_int32, c_int32, c_void_p, c_void_p],  # caches, num_blocks, bits, dtype, err, stream
+    ),
+    "seb_paged_attention_q4_workspace_size": (c_int64, [c_int32, c_int32, c_int32, c_int32, c_int32]),
+    "seb_paged_attention_q4": (
+        c_int32,
+        [c_void_p, c_int64, c_int64,            # q, strides
+         c_void_p, c_void_p, c_int64,           # k_cache, v_cache, num_blocks
+         c_void_p, c_int64, c_int64,            # block_table, stride, max_blocks
+         c_void_p, c_void_p, c_void_p, c_void_p,  # q_starts, q_lens, k_lens, q_pos_offsets
+         c_int32, c_int32,                      # num_rows, total_query
+         c_int32, c_int32, c_int32, c_int32,    # hq, hkv, head_dim, dtype
+         c_float, c_int32,                      # scale, is_causal
+         c_void_p, c_int64, c_int64,            # out, strides
+         c_void_p, c_int64,                     # lse, stride
+         c_void_p, c_int64, c_void_p, c_void_p],  # workspace, bytes, err, stream
+    ),
+    "seb_step_tables": (
+        c_int32,
+        [c_void_p, c_void_p, c_int32, c_int32,  # q_lens, context_lens, num_rows, total_query
+         c_void_p, c_int64, c_int64,            # block_table, stride, max_blocks
+         c_void_p, c_int32, c_void_p,           # free_ids, capacity, free_state
+         c_void_p, c_void_p, c_void_p,          # q_starts, k_lens, q_pos_offsets
+         c_void_p, c_void_p, c_void_p,          # item_row, positions, slot_mapping
+         c_void_p, c_void_p, c_void_p],         # free_next, err, stream
+    ),
     "seb_selftest_bounded_wait": (c_int32, [c_uint32, c_void_p, c_void_p]),
     "seb_peer_alloc": (c_int32, [c_size_t, POINTER(c_void_p)]),
     "seb_peer_free": (c_int32, [c_void_p]),

@@ -24,6 +24,7 @@ import numpy as np
 import torch
 
 from . import ops
+from .q4 import paged_attention_q4
 
 PAGED_K_TILE_SIZE = ops.BLOCK_SIZE  # one physical block per key tile (paged_attention_kernel.py:12)
 PAGED_Q_TILE_SIZE = 16
@@ -251,7 +252,8 @@ def paged_flash_attention(q, k_cache, v_cache, metadata, num_q_heads, num_kv_hea
     the reference builder's keys, and head_dim-64 batches with prefill rows, are
     split into decode items and prefill units on the device (one small routing
     kernel, no readback). Other dtypes and shapes run every token through the
-    decode kernel, which computes any row exactly.
+    decode kernel, which computes any row exactly. A 4-bit pool (uint8 planes
+    [num_blocks, num_kv_heads, 9 * head_dim]) goes to paged_attention_q4.
     """
     rows = metadata["q_lens"].shape[0]
     width = int(metadata["block_table_row_stride"])
@@ -261,6 +263,10 @@ def paged_flash_attention(q, k_cache, v_cache, metadata, num_q_heads, num_kv_hea
     mk = metadata.get("max_k_len")
     if mk is not None and mk > width * ops.BLOCK_SIZE:
         raise ValueError(f"paged_flash_attention: k_len {mk} exceeds the block table width {width} x {ops.BLOCK_SIZE}")
+    if k_cache.dtype == torch.uint8:
+        return paged_attention_q4(q, k_cache, v_cache, metadata["block_table"], metadata["q_starts"],
+                                  metadata["q_lens"], metadata["k_lens"], metadata["q_pos_offsets"], num_q_heads,
+                                  num_kv_heads, scale, is_causal)
     o = torch.empty_like(q)
     lse = torch.empty((q.shape[0], num_q_heads), dtype=torch.float32, device=q.device)
     if rows == 0 or q.shape[0] == 0:

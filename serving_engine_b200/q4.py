@@ -1,0 +1,228 @@
+"""The 4-bit KV pool: its tensors, and the ops that write it, read it and attend over it.
+
+One layer of the pool is two uint8 planes (K and V) of shape [num_blocks, kv heads,
+9 * head_dim]; ``new_q4_pool`` makes the pool of a model, [layers, 2, num_blocks, kv
+heads, 9 * head_dim]. Every 64 values of a token's head share a scale and a lowest
+value in fp16 and take 4 bits each, 4.5 bits in all: 3.6 times the tokens of a 16-bit
+pool, and as much less to read in a decode step. include/serving_engine_b200.h states
+what each call computes and csrc/q4_format.cuh the order of the bytes.
+
+The ops follow ``ops``: shapes, dtypes and devices are checked on the host without a
+sync, work goes to the current stream, out-of-range indices met at run time are
+reported by ``check_device_errors``. bf16 and fp16, head_dim 64, 128 and 256.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import ops
+from ._lib import check, lib
+from .ops import BLOCK_SIZE, LAUNCHES, _after, _half_dtype, _nvtx, _require_cuda, _stream, dtype_code, err_word
+
+HEAD_DIMS = (64, 128, 256)
+
+
+def row_bytes(head_dim: int) -> int:
+    """Bytes of one kv head of one block in one plane: 8 * head_dim of codes, head_dim of (scale, low) pairs."""
+    if head_dim not in HEAD_DIMS:
+        raise ValueError(f"4-bit KV pool: head_dim {head_dim} not supported {HEAD_DIMS}")
+    return 9 * head_dim
+
+
+def new_q4_pool(num_layers: int, num_blocks: int, num_kv_heads: int, head_dim: int, device="cuda") -> torch.Tensor:
+    """A zeroed 4-bit pool for a model: uint8 [layers, 2, num_blocks, kv heads, 9 * head_dim]."""
+    return torch.zeros(num_layers, 2, num_blocks, num_kv_heads, row_bytes(head_dim), dtype=torch.uint8, device=device)
+
+
+def _check_planes(name: str, k_cache: torch.Tensor, v_cache: torch.Tensor, num_kv_heads: int, head_dim: int) -> None:
+    want = row_bytes(head_dim)
+    if k_cache.dtype != torch.uint8 or v_cache.dtype != torch.uint8:
+        raise ValueError(f"{name}: a 4-bit pool is uint8, got {k_cache.dtype} and {v_cache.dtype}")
+    if k_cache.dim() != 3 or k_cache.shape[1] != num_kv_heads or k_cache.shape[2] != want:
+        raise ValueError(f"{name}: k_cache must be [num_blocks, {num_kv_heads}, {want}], got {tuple(k_cache.shape)}")
+    if v_cache.shape != k_cache.shape or not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+        raise ValueError(f"{name}: k_cache and v_cache must be contiguous and of equal shape")
+
+
+def _check_slots(name: str, slots: torch.Tensor, n: int) -> torch.Tensor:
+    if slots.dtype != torch.int64 or slots.dim() != 1 or slots.numel() != n:
+        raise ValueError(f"{name}: slot_mapping must be int64 [{n}]")
+    return slots if slots.is_contiguous() else slots.contiguous()
+
+
+@_nvtx
+def kv_append_q4(k_new: torch.Tensor, v_new: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                 slot_mapping: torch.Tensor) -> None:
+    """``kv_append`` into a 4-bit pool: quantises k_new, v_new [n_tokens, H, D] (unit
+    stride on D, any token and head strides) into the slots slot_mapping, int64
+    [n_tokens], of the planes k_cache, v_cache [num_blocks, H, 9 * D]. One launch."""
+    dev = _require_cuda("kv_append_q4", k_new, v_new, k_cache, v_cache, slot_mapping)
+    dt = _half_dtype("kv_append_q4", k_new, v_new)
+    if k_new.dim() != 3 or v_new.shape != k_new.shape:
+        raise ValueError(f"kv_append_q4: k_new/v_new must both be [n_tokens, H, D], got {tuple(k_new.shape)} "
+                         f"and {tuple(v_new.shape)}")
+    n, h, d = k_new.shape
+    _check_planes("kv_append_q4", k_cache, v_cache, h, d)
+    if k_new.stride(2) != 1 or v_new.stride(2) != 1:
+        raise ValueError("kv_append_q4: new K/V must have unit stride on head_dim")
+    slot_mapping = _check_slots("kv_append_q4", slot_mapping, n)
+    if n == 0:
+        return
+    st = lib().seb_kv_append_q4(
+        k_new.data_ptr(), k_new.stride(0), k_new.stride(1), v_new.data_ptr(), v_new.stride(0), v_new.stride(1), n,
+        slot_mapping.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0], h, d, dt,
+        err_word(dev).data_ptr(), _stream(dev))
+    check("seb_kv_append_q4", st)
+    LAUNCHES[0] += 1
+    _after(dev)
+
+
+@_nvtx
+def kv_gather_q4(k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor, head_dim: int,
+                 dtype: torch.dtype = torch.bfloat16) -> tuple[torch.Tensor, torch.Tensor]:
+    """The K and V values that the pool's slots (int64 [n]) stand for, each [n, kv heads,
+    head_dim] of ``dtype`` (fp32, fp16 or bf16; computed in fp32, rounded once). One launch."""
+    dev = _require_cuda("kv_gather_q4", k_cache, v_cache, slots)
+    if k_cache.dim() != 3:
+        raise ValueError(f"kv_gather_q4: k_cache must be [num_blocks, kv heads, 9 * head_dim], got {tuple(k_cache.shape)}")
+    h, n = k_cache.shape[1], slots.numel()
+    _check_planes("kv_gather_q4", k_cache, v_cache, h, head_dim)
+    slots = _check_slots("kv_gather_q4", slots, n)
+    k = torch.empty(n, h, head_dim, dtype=dtype, device=dev)
+    v = torch.empty_like(k)
+    dt = dtype_code(k)
+    if n == 0:
+        return k, v
+    st = lib().seb_kv_gather_q4(k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0], h, head_dim, slots.data_ptr(),
+                                n, k.data_ptr(), v.data_ptr(), dt, err_word(dev).data_ptr(), _stream(dev))
+    check("seb_kv_gather_q4", st)
+    LAUNCHES[0] += 1
+    _after(dev)
+    return k, v
+
+
+@_nvtx
+def qk_norm_rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, slot_mapping: torch.Tensor,
+                        k_cache: torch.Tensor, v_cache: torch.Tensor, num_q_heads: int, num_kv_heads: int,
+                        q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None, eps: float = 1e-6,
+                        out: torch.Tensor | None = None) -> torch.Tensor:
+    """RMSNorm of every query and key head, the rotary embedding and the KV write in one
+    launch: returns q [n_tokens, num_q_heads, head_dim] and writes K and V of token t to
+    slot slot_mapping[t] of a 16-bit pool ([num_blocks, 16, kv heads, head_dim] of qkv's
+    dtype) or of a 4-bit one (uint8 [num_blocks, kv heads, 9 * head_dim]).
+
+    qkv: [n_tokens, (num_q_heads + 2 * num_kv_heads) * head_dim], q heads, then k, then v;
+    cos/sin: [n_tokens, head_dim] (any leading views that flatten to that); q_weight,
+    k_weight: [head_dim] norm weights, None where the model has no such norm. Computed in
+    fp32 and rounded once (rope_kv_append rounds every product as the eager ops do).
+    """
+    ts = [qkv, cos, sin, slot_mapping, k_cache, v_cache] + [w for w in (q_weight, k_weight) if w is not None]
+    dev = _require_cuda("qk_norm_rope_append", *ts)
+    q4_pool = k_cache.dtype == torch.uint8
+    if v_cache.dtype != k_cache.dtype:
+        raise ValueError(f"qk_norm_rope_append: k_cache must be of v_cache's dtype, got {k_cache.dtype} and {v_cache.dtype}")
+    dt = _half_dtype("qk_norm_rope_append", qkv, cos, sin, *ts[6:], *(() if q4_pool else (k_cache, v_cache)))
+    if qkv.dim() != 2 or qkv.stride(1) != 1:
+        raise ValueError("qk_norm_rope_append: qkv must be [n_tokens, width] with unit column stride")
+    n, d = qkv.shape[0], cos.shape[-1]
+    if d not in HEAD_DIMS:
+        raise ValueError(f"qk_norm_rope_append: head_dim {d} not supported {HEAD_DIMS}")
+    if num_q_heads <= 0 or num_kv_heads <= 0 or qkv.shape[1] != (num_q_heads + 2 * num_kv_heads) * d:
+        raise ValueError(f"qk_norm_rope_append: qkv width {qkv.shape[1]} != ({num_q_heads} + 2 x {num_kv_heads}) x {d}")
+    if q4_pool:
+        _check_planes("qk_norm_rope_append", k_cache, v_cache, num_kv_heads, d)
+    else:
+        if k_cache.dim() != 4 or tuple(k_cache.shape[1:]) != (BLOCK_SIZE, num_kv_heads, d):
+            raise ValueError(f"qk_norm_rope_append: k_cache must be [num_blocks, {BLOCK_SIZE}, {num_kv_heads}, {d}], "
+                             f"got {tuple(k_cache.shape)}")
+        if v_cache.shape != k_cache.shape or not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+            raise ValueError("qk_norm_rope_append: k_cache and v_cache must be contiguous and of equal shape")
+    if cos.dim() != 2:
+        cos = cos.reshape(-1, d)
+    if sin.dim() != 2:
+        sin = sin.reshape(-1, sin.shape[-1])
+    if cos.shape != (n, d) or sin.shape != (n, d) or cos.stride() != sin.stride() or cos.stride(1) != 1:
+        raise ValueError(f"qk_norm_rope_append: cos and sin must be [n_tokens={n}, head_dim={d}] with equal strides")
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is not None and (w.shape != (d,) or not w.is_contiguous()):
+            raise ValueError(f"qk_norm_rope_append: {name} must be [{d}] and contiguous")
+    slot_mapping = _check_slots("qk_norm_rope_append", slot_mapping, n)
+    if out is None:
+        out = torch.empty((n, num_q_heads, d), dtype=qkv.dtype, device=dev)
+    elif (out.shape != (n, num_q_heads, d) or out.stride(2) != 1 or out.stride(1) != d or out.dtype != qkv.dtype
+          or out.device != dev):
+        raise ValueError("qk_norm_rope_append: out must be [n_tokens, num_q_heads, head_dim] of qkv's dtype and device "
+                         "with contiguous heads")
+    if n == 0:
+        return out
+    st = lib().seb_qk_norm_rope_append(
+        qkv.data_ptr(), qkv.stride(0), n, num_q_heads, num_kv_heads, d, cos.data_ptr(), sin.data_ptr(), cos.stride(0),
+        None if q_weight is None else q_weight.data_ptr(), None if k_weight is None else k_weight.data_ptr(), eps,
+        slot_mapping.data_ptr(), out.data_ptr(), out.stride(0), k_cache.data_ptr(), v_cache.data_ptr(),
+        k_cache.shape[0], 4 if q4_pool else 16, dt, err_word(dev).data_ptr(), _stream(dev))
+    check("seb_qk_norm_rope_append", st)
+    LAUNCHES[0] += 1
+    _after(dev)
+    return out
+
+
+@_nvtx
+def paged_attention_q4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+                       q_starts: torch.Tensor, q_lens: torch.Tensor, k_lens: torch.Tensor,
+                       q_pos_offsets: torch.Tensor, num_q_heads: int, num_kv_heads: int, scale: float,
+                       is_causal: bool = True, out: torch.Tensor | None = None,
+                       lse: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Paged attention over a 4-bit pool for rows of any length (decode rows, drafted
+    tokens, prefill chunks, mixed): (out like q, lse fp32 [total_query, num_q_heads]).
+
+    q: [total_query, num_q_heads, D] with unit stride on D; the planes as in
+    ``kv_append_q4``; block_table int32 [rows, max_blocks]; the other arrays int32 [rows].
+    A query that sees no key gets 0 and -inf; tokens of no row keep what out held.
+    """
+    dev = _require_cuda("paged_attention_q4", q, k_cache, v_cache, block_table, q_starts, q_lens, k_lens, q_pos_offsets)
+    dt = _half_dtype("paged_attention_q4", q)
+    if q.dim() != 3 or q.stride(2) != 1 or q.shape[1] != num_q_heads:
+        raise ValueError(f"paged_attention_q4: q must be [total_query, {num_q_heads}, head_dim] with unit inner stride, "
+                         f"got {tuple(q.shape)}")
+    total_q, _, d = q.shape
+    if num_kv_heads <= 0 or num_q_heads % num_kv_heads:
+        raise ValueError(f"paged_attention_q4: num_q_heads {num_q_heads} not a multiple of num_kv_heads {num_kv_heads}")
+    _check_planes("paged_attention_q4", k_cache, v_cache, num_kv_heads, d)
+    rows = q_starts.numel()
+    for name, t in (("q_starts", q_starts), ("q_lens", q_lens), ("k_lens", k_lens), ("q_pos_offsets", q_pos_offsets)):
+        if t.dtype != torch.int32 or t.dim() != 1 or t.numel() != rows:
+            raise ValueError(f"paged_attention_q4: {name} must be int32 [{rows}]")
+        if not t.is_contiguous():
+            raise ValueError(f"paged_attention_q4: {name} must be contiguous")
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != rows:
+        raise ValueError(f"paged_attention_q4: block_table must be int32 [{rows}, max_blocks], "
+                         f"got {tuple(block_table.shape)}")
+    if block_table.stride(1) != 1:
+        block_table = block_table.contiguous()
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    elif out.shape != q.shape or out.stride(2) != 1 or out.dtype != q.dtype or out.device != dev:
+        raise ValueError("paged_attention_q4: out must match q, with unit stride on head_dim")
+    if lse is None:
+        lse = torch.empty((total_q, num_q_heads), dtype=torch.float32, device=dev)
+    elif lse.shape != (total_q, num_q_heads) or lse.dtype != torch.float32 or lse.stride(1) != 1 or lse.device != dev:
+        raise ValueError(f"paged_attention_q4: lse must be fp32 [{total_q}, {num_q_heads}] with unit column stride")
+    max_blocks = block_table.shape[1]
+    if rows == 0 or total_q == 0:
+        return out, lse
+    if max_blocks == 0:  # no row has a key
+        out.zero_()
+        lse.fill_(float("-inf"))
+        return out, lse
+    nbytes = lib().seb_paged_attention_q4_workspace_size(rows, total_q, num_q_heads, num_kv_heads, d)
+    ws = ops.workspace(dev, nbytes)
+    st = lib().seb_paged_attention_q4(
+        q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0],
+        block_table.data_ptr(), block_table.stride(0), max_blocks, q_starts.data_ptr(), q_lens.data_ptr(),
+        k_lens.data_ptr(), q_pos_offsets.data_ptr(), rows, total_q, num_q_heads, num_kv_heads, d, dt, scale,
+        1 if is_causal else 0, out.data_ptr(), out.stride(0), out.stride(1), lse.data_ptr(), lse.stride(0),
+        ws.data_ptr(), ws.numel(), err_word(dev).data_ptr(), _stream(dev))
+    check("seb_paged_attention_q4", st)
+    LAUNCHES[0] += 1
+    _after(dev)
+    return out, lse
