@@ -369,7 +369,11 @@ SEB_API int seb_qk_norm_rope_append(const void* qkv, int64_t qkv_stride_token, i
  * are. Rows' token ranges must not overlap. A block id out of range sets
  * SEB_ERRBIT_BLOCK_ID and its keys count as masked; a k_len beyond the table sets
  * SEB_ERRBIT_KLEN and ends there; a row outside total_query sets SEB_ERRBIT_META and
- * is skipped. workspace: seb_paged_attention_q4_workspace_size(...) bytes. */
+ * is skipped.
+ * workspace: seb_paged_attention_q4_workspace_size(...) bytes, 16-byte aligned, of any
+ * content. counter_slot: 0 .. SEB_Q4_COUNTER_SLOTS - 1, a set of the library's own
+ * arrival counters. Calls that may overlap on the GPU need a workspace and a slot each. */
+#define SEB_Q4_COUNTER_SLOTS 128
 SEB_API int64_t seb_paged_attention_q4_workspace_size(int32_t num_rows, int32_t total_query, int32_t num_q_heads,
                                                       int32_t num_kv_heads, int32_t head_dim);
 
@@ -381,7 +385,7 @@ SEB_API int seb_paged_attention_q4(const void* q, int64_t q_stride_token, int64_
                                    int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, int32_t dtype,
                                    float scale, int32_t is_causal, void* out, int64_t out_stride_token,
                                    int64_t out_stride_head, float* lse, int64_t lse_stride_token, void* workspace,
-                                   int64_t workspace_bytes, int32_t* err, void* stream);
+                                   int64_t workspace_bytes, int32_t counter_slot, int32_t* err, void* stream);
 
 /* A step's metadata from request lengths that are on the GPU (what the engine's host
  * code computes at serving_engine/block_manager.py:87-111, model_runner.py:127-170 and

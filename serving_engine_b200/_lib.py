@@ -135,7 +135,7 @@ SIGNATURES = {
          c_float, c_int32,                      # scale, is_causal
          c_void_p, c_int64, c_int64,            # out, strides
          c_void_p, c_int64,                     # lse, stride
-         c_void_p, c_int64, c_void_p, c_void_p],  # workspace, bytes, err, stream
+         c_void_p, c_int64, c_int32, c_void_p, c_void_p],  # workspace, bytes, counter_slot, err, stream
     ),
     "seb_step_tables": (
         c_int32,
@@ -163,6 +163,7 @@ SIGNATURES = {
 SEB_MAX_PEERS = 8
 SEB_PEER_HANDLE_BYTES = 64
 SEB_PEER_FLAG_BYTES = 1024
+Q4_COUNTER_SLOTS = 128  # SEB_Q4_COUNTER_SLOTS
 NOALLOC_SCRATCH_BYTES = 32 << 20  # SEB_NOALLOC_SCRATCH_BYTES
 
 _LIB: ctypes.CDLL | None = None

@@ -15,8 +15,7 @@ from __future__ import annotations
 
 import torch
 
-from . import ops
-from ._lib import check, lib
+from ._lib import Q4_COUNTER_SLOTS, check, lib
 from .ops import BLOCK_SIZE, LAUNCHES, _after, _half_dtype, _nvtx, _require_cuda, _stream, dtype_code, err_word
 
 HEAD_DIMS = (64, 128, 256)
@@ -32,6 +31,25 @@ def row_bytes(head_dim: int) -> int:
 def new_q4_pool(num_layers: int, num_blocks: int, num_kv_heads: int, head_dim: int, device="cuda") -> torch.Tensor:
     """A zeroed 4-bit pool for a model: uint8 [layers, 2, num_blocks, kv heads, 9 * head_dim]."""
     return torch.zeros(num_layers, 2, num_blocks, num_kv_heads, row_bytes(head_dim), dtype=torch.uint8, device=device)
+
+
+# (device, stream) -> (workspace, counter slot). A workspace that a larger call outgrew
+# stays allocated: a captured CUDA graph may hold its address.
+_workspaces: dict[tuple[int, int], tuple[torch.Tensor, int]] = {}
+_retired: list[torch.Tensor] = []
+
+
+def _workspace(dev: torch.device, stream: int, nbytes: int) -> tuple[torch.Tensor, int]:
+    """The stream's own workspace and counters, so calls on different streams may overlap."""
+    held = _workspaces.get((dev.index, stream))
+    if held is None or held[0].numel() < nbytes:
+        slot = len(_workspaces) % Q4_COUNTER_SLOTS if held is None else held[1]
+        if held is not None:
+            _retired.append(held[0])
+        with torch.inference_mode(False):
+            held = (torch.empty(nbytes, dtype=torch.uint8, device=dev), slot)
+        _workspaces[dev.index, stream] = held
+    return held
 
 
 def _check_planes(name: str, k_cache: torch.Tensor, v_cache: torch.Tensor, num_kv_heads: int, head_dim: int) -> None:
@@ -178,6 +196,10 @@ def paged_attention_q4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
     q: [total_query, num_q_heads, D] with unit stride on D; the planes as in
     ``kv_append_q4``; block_table int32 [rows, max_blocks]; the other arrays int32 [rows].
     A query that sees no key gets 0 and -inf; tokens of no row keep what out held.
+
+    Every stream has its own workspace: calls on different streams may overlap. A CUDA
+    graph holds the workspace of the stream it was captured on; graphs captured on one
+    stream must not be replayed at the same time.
     """
     dev = _require_cuda("paged_attention_q4", q, k_cache, v_cache, block_table, q_starts, q_lens, k_lens, q_pos_offsets)
     dt = _half_dtype("paged_attention_q4", q)
@@ -215,13 +237,14 @@ def paged_attention_q4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
         lse.fill_(float("-inf"))
         return out, lse
     nbytes = lib().seb_paged_attention_q4_workspace_size(rows, total_q, num_q_heads, num_kv_heads, d)
-    ws = ops.workspace(dev, nbytes)
+    stream = _stream(dev)
+    ws, slot = _workspace(dev, stream, nbytes)
     st = lib().seb_paged_attention_q4(
         q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0],
         block_table.data_ptr(), block_table.stride(0), max_blocks, q_starts.data_ptr(), q_lens.data_ptr(),
         k_lens.data_ptr(), q_pos_offsets.data_ptr(), rows, total_q, num_q_heads, num_kv_heads, d, dt, scale,
         1 if is_causal else 0, out.data_ptr(), out.stride(0), out.stride(1), lse.data_ptr(), lse.stride(0),
-        ws.data_ptr(), ws.numel(), err_word(dev).data_ptr(), _stream(dev))
+        ws.data_ptr(), ws.numel(), slot, err_word(dev).data_ptr(), stream)
     check("seb_paged_attention_q4", st)
     LAUNCHES[0] += 1
     _after(dev)
