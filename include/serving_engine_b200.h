@@ -369,7 +369,7 @@ SEB_API int seb_qk_norm_rope_append(const void* qkv, int64_t qkv_stride_token, i
  * are. Rows' token ranges must not overlap. A block id out of range sets
  * SEB_ERRBIT_BLOCK_ID and its keys count as masked; a k_len beyond the table sets
  * SEB_ERRBIT_KLEN and ends there; a row outside total_query sets SEB_ERRBIT_META and
- * is skipped.
+ * is skipped. Rows of q and out are 16-byte aligned.
  * workspace: seb_paged_attention_q4_workspace_size(...) bytes, 16-byte aligned, of any
  * content. counter_slot: 0 .. SEB_Q4_COUNTER_SLOTS - 1, a set of the library's own
  * arrival counters. Calls that may overlap on the GPU need a workspace and a slot each. */

@@ -20,9 +20,9 @@
 // p_j sV_jG becomes fp16 (unit 2^-11) after a power of two that keeps it below 2^15.
 // Scores, maxima, sums and O are fp32.
 //
-// Work: a unit is (row, tile of tokens, kv head) and its blocks; the units of all rows
-// laid end to end are cut in equal runs of blocks, one per resident warp, whatever
-// the rows' lengths. A warp keeps all query heads of the group (and several tokens of
+// Work: a unit is (row, tile of tokens, kv head) and its blocks, taken in pairs; the units
+// of all rows laid end to end are cut in equal runs of pairs, one per resident warp,
+// whatever the rows' lengths. A warp keeps all query heads of the group (and several tokens of
 // a row, up to 8 * NT columns) on one tile, so each KV byte is read once per tile.
 // Parts of a unit are joined in shared memory, and over CTAs in the workspace by the
 // last to arrive, in order of their place, so results do not depend on timing.
@@ -37,6 +37,7 @@ namespace {
 constexpr unsigned kFull = 0xffffffffu;
 constexpr float kLn2 = 0.69314718055994530942f;
 constexpr float kLog2e = 1.44269504088896340736f;
+constexpr uint32_t kMinRun = 2;          // pairs of blocks of the shortest run worth a warp
 constexpr float kNoMax = -FLT_MAX;       // no score yet: any score is above it by more than the threshold
 constexpr float kThreshold = 8.f;        // scores may exceed the reference by 2^8 before it is moved
 constexpr float kScaleThreshold = 64.f;  // p * V scale stays below 2^8 * 2^6
@@ -57,10 +58,10 @@ struct Q4Params {
   int32_t num_rows;
   int32_t total_query;
   int32_t hq, hkv, group;
-  int32_t tile;  // tokens of a tile
+  int32_t tile;       // tokens of a tile
+  uint32_t by_group;  // col / group == col * by_group >> 16 for the columns of a tile
   float scale_log2;
   int32_t causal;
-  int32_t vec;   // q and out rows are 16-byte aligned
   char* out;
   int64_t o_st, o_sh;  // elements
   float* lse;
@@ -79,8 +80,8 @@ __device__ int32_t g_q4_counters[SEB_Q4_COUNTER_SLOTS][kMaxCtas * 32];
 
 struct Row {
   int q_len, q_start, q_pos, k_len;
-  int nblk;   // blocks of each of its units; at least 1 where it has tokens
-  int tiles;
+  uint32_t pairs;  // pairs of blocks of each of its units; at least 1
+  uint32_t tiles;
 };
 
 __device__ __forceinline__ Row row_of(const Q4Params& p, int r, uint32_t* bad) {
@@ -99,89 +100,425 @@ __device__ __forceinline__ Row row_of(const Q4Params& p, int r, uint32_t* bad) {
   }
   int64_t seen = w.k_len;
   if (p.causal) seen = min(seen, (int64_t)w.q_pos + w.q_len);
-  w.nblk = max((int)((seen + 15) >> 4), 1);
+  w.pairs = (uint32_t)max((int)((seen + 31) >> 5), 1);
   w.tiles = (w.q_len + p.tile - 1) / p.tile;
   return w;
 }
 
-__device__ __forceinline__ int64_t blocks_of(const Q4Params& p, const Row& w) {
-  return (int64_t)w.tiles * p.hkv * w.nblk;
-}
+__device__ __forceinline__ uint32_t pairs_of(const Q4Params& p, const Row& w) { return w.tiles * p.hkv * w.pairs; }
 
 // What a warp leaves of a unit that it did not do alone.
 struct Part {
-  int64_t unit;  // the unit's first block in the run of all units; -1: no part
-  int64_t end;   // and past its last
-  int row, tile, kvh, cols;
+  uint32_t unit;  // the unit's first pair in the run of all units
+  uint32_t end;   // and past its last; 0: no part
+  int64_t token;  // the tile's first
+  int kvh, cols;
 };
 
+// Shared memory: parts, prefix sums and barriers, then for each warp its ring of pairs
+// of blocks and room for the first of its two parts (the last one goes where the ring was).
 template <int D, int NT, int NW, int STAGES>
 struct Smem {
   static constexpr int kCols = 8 * NT;
-  static constexpr int kStage = 2 * q4::Layout<D>::kRow;
+  static constexpr int kStage = 4 * q4::Layout<D>::kRow;  // K and V rows of two blocks
   static constexpr int kPartBytes = kCols * (D + 2) * 4;
   static constexpr int kRing = STAGES * kStage > kPartBytes ? STAGES * kStage : kPartBytes;
   static constexpr int kWarp = (kRing + kPartBytes + 127) / 128 * 128;
-  static constexpr int kParts = 0;                                  // Part[NW][2]
-  static constexpr int kPrefix = kParts + NW * 2 * (int)sizeof(Part);  // int64 [NW * 32 + 1]
-  static constexpr int kBars = kPrefix + (NW * 32 + 2) * 8;
+  static constexpr int kParts = 0;                                     // Part[NW][2]
+  static constexpr int kPrefix = kParts + NW * 2 * (int)sizeof(Part);  // uint32 [NW * 32 + 1]
+  static constexpr int kBars = kPrefix + (NW * 32 + 2) * 4;
   static constexpr int kWarps = (kBars + NW * STAGES * 8 + 127) / 128 * 128;
   static constexpr int kBytes = kWarps + NW * kWarp;
 };
 
-// Weighted sum of `n` parts of one column; lane l holds dims l * D / 32 and on, so that
-// O = o / l with scores against m. part(i) gives part i's O row and its (m, l).
-template <int D, bool GLOBAL, typename F>
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// 2^e as a float, e in [-126, 127]; and the exponent of a float that is not subnormal
+__device__ __forceinline__ float power2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+__device__ __forceinline__ int exponent(float x) { return (int)((__float_as_uint(x) >> 23) & 255) - 127; }
+
+// The token, of its tile, of a column.
+__device__ __forceinline__ int token_of(const Q4Params& p, int col) { return (int)(col * p.by_group >> 16); }
+
+// Lane l's dims l * D / 32 and on of a row of floats.
+template <int D, bool GLOBAL>
+__device__ __forceinline__ void load_dims(const float* row, int lane, float (&v)[D / 32]) {
+  constexpr int DL = D / 32;
+  if constexpr (DL == 2) {
+    const float2* at = reinterpret_cast<const float2*>(row) + lane;
+    const float2 x = GLOBAL ? __ldcg(at) : *at;
+    v[0] = x.x, v[1] = x.y;
+  } else {
+#pragma unroll
+    for (int c = 0; c < DL / 4; ++c) {
+      const float4* at = reinterpret_cast<const float4*>(row) + lane * (DL / 4) + c;
+      const float4 x = GLOBAL ? __ldcg(at) : *at;
+      v[4 * c] = x.x, v[4 * c + 1] = x.y, v[4 * c + 2] = x.z, v[4 * c + 3] = x.w;
+    }
+  }
+}
+
+// Joins `n` parts of one column: lane l gets its dims of the sum of O, against the largest
+// reference m, and the sum l. part(i, row, ml) finds part i's O and its (m, l). LANES: the
+// parts taken at a time.
+template <int D, int LANES, bool GLOBAL, typename F>
 __device__ __forceinline__ void join(int n, int lane, F part, float (&o)[D / 32], float& m, float& l) {
   constexpr int DL = D / 32;
   m = -INFINITY;
-  for (int i = lane; i < n; i += 32) {
-    const float2* ml;
-    const float* row;
-    part(i, row, ml);
-    m = fmaxf(m, GLOBAL ? __ldcg(ml).x : ml->x);
-  }
-#pragma unroll
-  for (int off = 16; off >= 1; off >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, off));
-  const float ref = m == -INFINITY ? 0.f : m;
   l = 0.f;
 #pragma unroll
   for (int e = 0; e < DL; ++e) o[e] = 0.f;
-  for (int i0 = 0; i0 < n; i0 += 32) {
-    float w = 0.f, li = 0.f;
-    if (i0 + lane < n) {
-      const float2* ml;
-      const float* row;
-      part(i0 + lane, row, ml);
-      const float2 v = GLOBAL ? __ldcg(ml) : *ml;
-      w = exp2f(v.x - ref);
-      li = v.y * w;
+#pragma unroll 1
+  for (int i0 = 0; i0 < n; i0 += LANES) {
+    const float* row;
+    const float2* ml;
+    float2 mine = make_float2(-INFINITY, 0.f);
+    const int i = i0 + lane % LANES;
+    if (i < n) {
+      part(i, row, ml);
+      mine = GLOBAL ? __ldcg(ml) : *ml;
     }
+    float top = mine.x;
 #pragma unroll
-    for (int off = 16; off >= 1; off >>= 1) li += __shfl_xor_sync(kFull, li, off);
-    l += li;
-    const int cnt = min(32, n - i0);
-#pragma unroll 8
+    for (int off = LANES / 2; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, off));
+    top = fmaxf(top, m);
+    const float ref = top == -INFINITY ? 0.f : top;
+    const float keep = exp2_fast(m - ref);
+    const float w = exp2_fast(mine.x - ref);
+    float sum = mine.y * w;
+#pragma unroll
+    for (int off = LANES / 2; off >= 1; off >>= 1) sum += __shfl_xor_sync(kFull, sum, off);
+    l = fmaf(l, keep, sum);
+    m = top;
+#pragma unroll
+    for (int e = 0; e < DL; ++e) o[e] *= keep;
+    const int cnt = min(LANES, n - i0);
+#pragma unroll(GLOBAL ? 4 : 2)
     for (int k = 0; k < cnt; ++k) {
-      const float2* ml;
-      const float* row;
       part(i0 + k, row, ml);
-      const float wk = __shfl_sync(kFull, w, k);
       float v[DL];
-      if constexpr (DL == 2) {
-        const float2 x = GLOBAL ? __ldcg(reinterpret_cast<const float2*>(row) + lane)
-                                : reinterpret_cast<const float2*>(row)[lane];
-        v[0] = x.x, v[1] = x.y;
-      } else {
-#pragma unroll
-        for (int c = 0; c < DL / 4; ++c) {
-          const float4* at = reinterpret_cast<const float4*>(row) + lane * (DL / 4) + c;
-          const float4 x = GLOBAL ? __ldcg(at) : *at;
-          v[4 * c] = x.x, v[4 * c + 1] = x.y, v[4 * c + 2] = x.z, v[4 * c + 3] = x.w;
-        }
-      }
+      load_dims<D, GLOBAL>(row, lane, v);
+      const float wk = __shfl_sync(kFull, w, k);
 #pragma unroll
       for (int e = 0; e < DL; ++e) o[e] = fmaf(wk, v[e], o[e]);
+    }
+  }
+}
+
+// One column's result: O / l and LSE, by a warp.
+template <typename T, int D>
+__device__ __forceinline__ void write_column(const Q4Params& p, int64_t token, int kvh, int col, int lane,
+                                             const float (&o)[D / 32], float m, float l) {
+  constexpr int DL = D / 32;
+  const int tk = token_of(p, col);
+  const int64_t tok = token + tk;
+  const int head = kvh * p.group + col - tk * p.group;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  T* dst = reinterpret_cast<T*>(p.out) + tok * p.o_st + (int64_t)head * p.o_sh + lane * DL;
+  T r[DL];
+#pragma unroll
+  for (int e = 0; e < DL; ++e) r[e] = Elem<T>::from_float(o[e] * inv);
+  if constexpr (DL == 2) *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<const uint32_t*>(r);
+  else if constexpr (DL == 4) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(r);
+  else *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(r);
+  if (lane == 0) p.lse[tok * p.lse_st + head] = l == 0.f ? -INFINITY : fmaf(m, kLn2, logf(l));
+}
+
+// What a warp keeps of the unit it is on.
+template <int D, int NT>
+struct Tile {
+  static constexpr int GR = D / q4::kGroup;
+  uint32_t qf[GR][NT][4][2];  // Q as the B operand: column 8 nt + g, dims 16 t .. 16 t + 15 of every group
+  float qs[GR][NT][2];        // sum of q over a group, columns 8 nt + 2 t and the next
+  float ch[NT][2];            // what brings a score to log2 units
+  float m[NT][2], l[NT][2];   // reference, and this lane's share of the sum
+  float low[GR][NT][2];       // this lane's share of sum p (low + 8 scale)
+  float one[(GR + 1) / 2][NT][4];  // sum of the rounded p * scale, two groups to a tile
+  float o[GR][4][NT][4];      // sum of those and the codes
+  float v_down;               // power of two that V's scales are taken by
+};
+
+template <typename T> struct Two;
+template <> struct Two<__half> {
+  using type = __half2;
+  static __device__ __forceinline__ type zero() { return __half2half2(__ushort_as_half(0)); }
+};
+template <> struct Two<__nv_bfloat16> {
+  using type = __nv_bfloat162;
+  static __device__ __forceinline__ type zero() { return __bfloat162bfloat162(__ushort_as_bfloat16(0)); }
+};
+__device__ __forceinline__ __half low_of(__half2 x) { return __low2half(x); }
+__device__ __forceinline__ __half high_of(__half2 x) { return __high2half(x); }
+__device__ __forceinline__ __nv_bfloat16 low_of(__nv_bfloat162 x) { return __low2bfloat16(x); }
+__device__ __forceinline__ __nv_bfloat16 high_of(__nv_bfloat162 x) { return __high2bfloat16(x); }
+
+// A lane's share of the columns' queries, as they are.
+template <typename T, int D, int NT>
+struct Queries {
+  typename Two<T>::type raw[NT][D / q4::kGroup][8];
+};
+
+template <typename T, int D, int NT>
+__device__ __forceinline__ void fetch_queries(const Q4Params& p, Queries<T, D, NT>& q, int64_t token, int kvh, int cols,
+                                              int lane) {
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int col = nt * 8 + (lane >> 2);
+    const bool live = col < cols;
+    const int tk = live ? token_of(p, col) : 0, hd = live ? col - tk * p.group : 0;
+    const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.q) + (token + tk) * p.q_st +
+                                                      (int64_t)(kvh * p.group + hd) * p.q_sh + 16 * (lane & 3));
+#pragma unroll
+    for (int gr = 0; gr < D / q4::kGroup; ++gr)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        *reinterpret_cast<uint4*>(&q.raw[nt][gr][4 * h]) = live ? __ldg(src + gr * 8 + h) : make_uint4(0u, 0u, 0u, 0u);
+  }
+}
+
+// Scaled by a power of two for each column, so that fp16 holds them, as the B operand.
+template <typename T, int D, int NT>
+__device__ __forceinline__ void convert_queries(const Q4Params& p, Tile<D, NT>& u, const Queries<T, D, NT>& q, int lane) {
+  constexpr int GR = D / q4::kGroup;
+  const int t = lane & 3;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const auto& raw = q.raw[nt];
+    auto most = Two<T>::zero();
+#pragma unroll
+    for (int gr = 0; gr < GR; ++gr)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) most = __hmax2_nan(most, __habs2(raw[gr][e]));
+    float top = q4::max_nan(Elem<T>::to_float(low_of(most)), Elem<T>::to_float(high_of(most)));
+    top = q4::max_nan(top, __shfl_xor_sync(kFull, top, 1));
+    top = q4::max_nan(top, __shfl_xor_sync(kFull, top, 2));
+    const int ex = top > 0.f ? min(max(exponent(top) - 14, -100), 112) : 0;  // the largest goes to [2^14, 2^15)
+    const float down = power2(-ex);
+#pragma unroll
+    for (int gr = 0; gr < GR; ++gr) {
+      float sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) {  // pairs that meet lower codes and pairs that meet upper ones, in turn
+        const float a = Elem<T>::to_float(low_of(raw[gr][w])) * down;
+        const float b = Elem<T>::to_float(high_of(raw[gr][w])) * down;
+        sum += a + b;
+        u.qf[gr][nt][w >> 1][w & 1] = w & 1 ? Mma<__half>::pack(a * 0.0625f, b * 0.0625f) : Mma<__half>::pack(a, b);
+      }
+      sum += __shfl_xor_sync(kFull, sum, 1);
+      sum += __shfl_xor_sync(kFull, sum, 2);
+      sum *= power2(-24);  // as the codes carry it
+      u.qs[gr][nt][0] = __shfl_sync(kFull, sum, 8 * t);
+      u.qs[gr][nt][1] = __shfl_sync(kFull, sum, 8 * t + 4);
+    }
+    const float up = fminf(fminf(fabsf(p.scale_log2) * power2(24), FLT_MAX) * power2(ex), FLT_MAX);
+    const float c = copysignf(up, p.scale_log2);
+    u.ch[nt][0] = __shfl_sync(kFull, c, 8 * t);
+    u.ch[nt][1] = __shfl_sync(kFull, c, 8 * t + 4);
+  }
+}
+
+// A lane's words of a panel, and its tokens' (scale, low) pairs.
+template <int G>
+__device__ __forceinline__ void load_words(const char* at, uint32_t (&w)[2 * G]) {
+  if constexpr (G == 2) *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(at);
+  else *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(at);
+}
+template <int G>
+__device__ __forceinline__ void load_pairs(const char* at, __half2 (&a)[G]) {
+  if constexpr (G == 2) *reinterpret_cast<uint2*>(a) = *reinterpret_cast<const uint2*>(at);
+  else *reinterpret_cast<uint32_t*>(a) = *reinterpret_cast<const uint32_t*>(at);
+}
+
+// KB blocks of 16 keys. `place` holds their rows, K and V of one after the other. MASK: some
+// key is not for every column; of keys key0 and on a column then sees those below its
+// `end`, and none of block i where bit i of `unread` says that it has no data.
+template <int D, int NT, int KB, bool MASK>
+__device__ __forceinline__ void take_blocks(Tile<D, NT>& u, const char* place, int lane, int key0, unsigned unread,
+                                            const int (&end)[NT][2]) {
+  using L = q4::Layout<D>;
+  constexpr int P = L::kPanels, G = L::kGroups, GR = P * G;
+  const int g = lane >> 2, t = lane & 3;
+  auto hidden = [&](int b, int nt, int c) {
+    return MASK && (((unread >> b) & 1) || key0 + 16 * b + g + 8 * (c >> 1) >= end[nt][c & 1]);
+  };
+
+  // S^T = K Q^T in log2 units: for each block 16 keys x 8 NT columns, one sum for each group
+  float x[KB][NT][4];
+#pragma unroll
+  for (int b = 0; b < KB; ++b) {
+#pragma unroll
+    for (int pn = 0; pn < P; ++pn) {
+      const char* kb = place + b * 2 * L::kRow;
+      uint32_t w[2][2 * G];  // of keys g and g + 8
+      __half2 pr[2][G];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        load_words<G>(kb + pn * 8 * L::kWidth + (g + 8 * h) * (L::kWidth / 2) + t * (8 * G), w[h]);
+        load_pairs<G>(kb + L::kCodes + pn * 64 * G + (g + 8 * h) * 4 * G, pr[h]);
+      }
+#pragma unroll
+      for (int gi = 0; gi < G; ++gi) {
+        const int gr = pn * G + gi;
+        float acc[NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) acc[nt][c] = 0.f;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          uint32_t k0 = w[0][gi * 2 + i], k1 = w[1][gi * 2 + i];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+              Mma<__half>::run(acc[nt], k0 & 0x000f000fu, k1 & 0x000f000fu, k0 & 0x00f000f0u, k1 & 0x00f000f0u,
+                               u.qf[gr][nt][2 * i + h][0], u.qf[gr][nt][2 * i + h][1]);
+            k0 >>= 8, k1 >>= 8;
+          }
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float scale = __low2float(pr[h][gi]), low = __high2float(pr[h][gi]);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int c = 2 * h; c < 2 * h + 2; ++c) {
+              const float q = u.qs[gr][nt][c & 1];
+              x[b][nt][c] = fmaf(scale, acc[nt][c], gr == 0 ? low * q : fmaf(low, q, x[b][nt][c]));
+            }
+        }
+      }
+    }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        x[b][nt][c] *= u.ch[nt][c & 1];
+        if (hidden(b, nt, c)) x[b][nt][c] = -INFINITY;
+      }
+  }
+
+  // this lane's largest score of each column, and the largest V scale
+  float top[NT][2];
+  bool move = false;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      top[nt][h] = fmaxf(x[0][nt][h], x[0][nt][h + 2]);
+#pragma unroll
+      for (int b = 1; b < KB; ++b) top[nt][h] = fmaxf(top[nt][h], fmaxf(x[b][nt][h], x[b][nt][h + 2]));
+      move |= top[nt][h] > u.m[nt][h] + kThreshold;
+    }
+  __half2 vp[KB][P][2][G];  // of keys g and g + 8
+  __half2 most = __half2half2(__ushort_as_half(0));
+#pragma unroll
+  for (int b = 0; b < KB; ++b)
+#pragma unroll
+    for (int pn = 0; pn < P; ++pn)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        load_pairs<G>(place + (b * 2 + 1) * L::kRow + L::kCodes + pn * 64 * G + (g + 8 * h) * 4 * G, vp[b][pn][h]);
+#pragma unroll
+        for (int gi = 0; gi < G; ++gi) most = __hmax2(most, vp[b][pn][h][gi]);
+      }
+  float vmax = __low2float(most);
+  if (__any_sync(kFull, move || vmax * u.v_down > kScaleThreshold)) {
+    // move the references: the power of two of V's scales, and the scores' maxima
+#pragma unroll
+    for (int k = 16; k >= 1; k >>= 1) vmax = fmaxf(vmax, __shfl_xor_sync(kFull, vmax, k));
+    float v_fix = 1.f;
+    if (vmax * u.v_down > kScaleThreshold) {
+      const float now = power2(-min(max(exponent(vmax), -24), 16));
+      v_fix = now / u.v_down;
+      u.v_down = now;
+    }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float mx = top[nt][h];
+        mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 4));
+        mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 8));
+        mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 16));
+        const float now = fmaxf(mx, u.m[nt][h]);
+        const float fix = exp2_fast(u.m[nt][h] - now);  // from kNoMax: 0
+        u.m[nt][h] = now;
+        u.l[nt][h] *= fix;
+#pragma unroll
+        for (int gr = 0; gr < GR; ++gr) {
+          u.low[gr][nt][h] *= fix;
+          u.one[gr / 2][nt][(gr & 1) * 2 + h] *= fix * v_fix;
+#pragma unroll
+          for (int mt = 0; mt < 4; ++mt) {
+            u.o[gr][mt][nt][h] *= fix * v_fix;
+            u.o[gr][mt][nt][h + 2] *= fix * v_fix;
+          }
+        }
+      }
+  }
+
+  // O^T += V^T (P scale)^T, and the lows' share. The codes count from 8 here: sum p scale n +
+  // sum p low = sum p' (n - 8) + sum p (low + 8 scale) with p' = p scale rounded to fp16, so
+  // that its rounding meets n - 8 and no more; sum p' is one more row of the product.
+  // Keys that a column does not see have p = 0, and none of their parameters is used.
+#pragma unroll
+  for (int b = 0; b < KB; ++b) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) x[b][nt][c] = exp2_fast(x[b][nt][c] - u.m[nt][c & 1]);
+      u.l[nt][0] += x[b][nt][0] + x[b][nt][2];
+      u.l[nt][1] += x[b][nt][1] + x[b][nt][3];
+    }
+#pragma unroll
+    for (int pn = 0; pn < P; ++pn) {
+      const char* vb = place + (b * 2 + 1) * L::kRow + pn * 8 * L::kWidth + (g ^ L::turn(t)) * (8 * G);
+      uint32_t w[2][2 * G];  // of key pairs t and t + 4
+      load_words<G>(vb + t * L::kWidth, w[0]);
+      load_words<G>(vb + (t + 4) * L::kWidth, w[1]);
+#pragma unroll
+      for (int gi = 0; gi < G; ++gi) {
+        const int gr = pn * G + gi;
+        uint32_t b0[NT], b1[NT];
+        float z[NT][4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float scale = __low2float(vp[b][pn][h][gi]), low = __high2float(vp[b][pn][h][gi]);
+          const float sv = scale * u.v_down, mid = fmaf(8.f, scale, low);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int c = 2 * h; c < 2 * h + 2; ++c) {
+              const bool hide = hidden(b, nt, c);
+              z[nt][c] = hide ? 0.f : x[b][nt][c] * sv;
+              u.low[gr][nt][c & 1] = fmaf(x[b][nt][c], hide ? 0.f : mid, u.low[gr][nt][c & 1]);
+            }
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          b0[nt] = movmatrix_trans(Mma<__half>::pack(z[nt][0], z[nt][1]));
+          b1[nt] = movmatrix_trans(Mma<__half>::pack(z[nt][2], z[nt][3]));
+          constexpr uint32_t kOnes = 0x3c003c00u;
+          Mma<__half>::run(u.one[gr / 2][nt], gr & 1 ? 0u : kOnes, gr & 1 ? kOnes : 0u, gr & 1 ? 0u : kOnes,
+                           gr & 1 ? kOnes : 0u, b0[nt], b1[nt]);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          uint32_t v0 = w[0][gi * 2 + i], v1 = w[1][gi * 2 + i];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+              Mma<__half>::run(u.o[gr][2 * i + h][nt], v0 & 0x000f000fu, v0 & 0x00f000f0u, v1 & 0x000f000fu,
+                               v1 & 0x00f000f0u, b0[nt], b1[nt]);
+            v0 >>= 8, v1 >>= 8;
+          }
+        }
+      }
     }
   }
 }
@@ -190,32 +527,32 @@ template <typename T, int D, int NT, int NW, int STAGES, int CTAS>
 __global__ void __launch_bounds__(NW * 32, CTAS) q4_attention_kernel(const Q4Params p) {
   using L = q4::Layout<D>;
   using S = Smem<D, NT, NW, STAGES>;
-  constexpr int P = L::kPanels, G = L::kGroups;  // panels, groups of a panel
+  constexpr int GR = D / q4::kGroup;
   constexpr int kCols = S::kCols;
   extern __shared__ __align__(128) char smem[];
   Part* parts = reinterpret_cast<Part*>(smem + S::kParts);
-  int64_t* prefix = reinterpret_cast<int64_t*>(smem + S::kPrefix);
+  uint32_t* prefix = reinterpret_cast<uint32_t*>(smem + S::kPrefix);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t = lane & 3;
 
   // ---- the units of all rows, and this warp's run of blocks
   const int chunk = (p.num_rows + NW * 32 - 1) / (NW * 32);  // rows that a thread sums up
   {
-    int64_t sum = 0;
-    uint32_t bad = 0;
-    for (int r = tid * chunk; r < min((tid + 1) * chunk, p.num_rows); ++r) sum += blocks_of(p, row_of(p, r, &bad));
+    uint32_t sum = 0, bad = 0;
+#pragma unroll 1
+    for (int r = tid * chunk; r < min((tid + 1) * chunk, p.num_rows); ++r) sum += pairs_of(p, row_of(p, r, &bad));
     if (bad && blockIdx.x == 0) atomic_or_err(p.err, bad);
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
-      const int64_t o = __shfl_up_sync(kFull, sum, off);
+      const uint32_t o = __shfl_up_sync(kFull, sum, off);
       if (lane >= off) sum += o;
     }
     prefix[tid + 1] = sum;
     if (tid == 0) prefix[0] = 0;
-    if (lane < 2) parts[warp * 2 + lane].unit = -1;
+    if (lane < 2) parts[warp * 2 + lane].end = 0;
   }
   __syncthreads();
-  int64_t total = 0, before = 0;
+  uint32_t total = 0, before = 0;
 #pragma unroll
   for (int w = 0; w < NW; ++w) {
     if (w == warp) before = total;
@@ -224,12 +561,12 @@ __global__ void __launch_bounds__(NW * 32, CTAS) q4_attention_kernel(const Q4Par
   __syncthreads();
   prefix[tid + 1] += before;
   __syncthreads();
-  const int64_t warps = (int64_t)gridDim.x * NW;
-  const int64_t per = max((total + warps - 1) / warps, (int64_t)4);
-  const int64_t cta0 = (int64_t)blockIdx.x * NW * per, cta1 = min(cta0 + NW * per, total);
+  const uint32_t warps = gridDim.x * NW;
+  const uint32_t per = max((total + warps - 1) / warps, kMinRun), span = NW * per;
+  const uint32_t cta0 = blockIdx.x * span, cta1 = min(cta0 + span, total);
   if (cta0 >= total) return;
-  int64_t pos = cta0 + warp * per;
-  const int64_t stop = min(pos + per, total);
+  uint32_t pos = cta0 + warp * per;
+  const uint32_t stop = min(pos + per, total);
 
   const uint32_t bars = smem_u32(smem + S::kBars) + warp * STAGES * 8;
   char* ring = smem + S::kWarps + warp * S::kWarp;
@@ -250,35 +587,34 @@ __global__ void __launch_bounds__(NW * 32, CTAS) q4_attention_kernel(const Q4Par
       else hi = mid - 1;
     }
     int r = lo * chunk;
-    int64_t off = pos - prefix[lo];
-    uint32_t bad = 0;
+    uint32_t off = pos - prefix[lo], bad = 0;
     Row row = row_of(p, r, &bad);
-    uint32_t it = 0;  // blocks taken through the ring so far
+    uint32_t it = 0;  // pairs taken through the ring so far
     bool dead = false;
 
     while (pos < stop) {
-      int64_t len = blocks_of(p, row);
-      while (off >= len) {
+      uint32_t len = pairs_of(p, row);
+#pragma unroll 1
+      while (off >= len && r + 1 < p.num_rows) {
         off -= len;
         row = row_of(p, ++r, &bad);
-        len = blocks_of(p, row);
+        len = pairs_of(p, row);
       }
-      const int64_t unit = off / row.nblk;
-      const int blk0 = (int)(off - unit * row.nblk);
-      const int kvh = (int)(unit % p.hkv), tile = (int)(unit / p.hkv);
-      const int n = (int)min((int64_t)(row.nblk - blk0), stop - pos);
-      const int tok0 = tile * p.tile;                    // first token of the tile in the row
+      if (off >= len) break;  // rows that overlap, beyond what can be counted
+      const uint32_t unit = off / row.pairs;  // tiles of one kv head are neighbours: they read the same blocks
+      const uint32_t pair0 = off - unit * row.pairs, n = min(row.pairs - pair0, stop - pos);
+      const int kvh = (int)(unit / row.tiles), tile = (int)(unit - kvh * row.tiles);
+      const int blk0 = 2 * (int)pair0;
+      const int tok0 = tile * p.tile;  // first token of the tile in the row
       const int toks = min(p.tile, row.q_len - tok0);
       const int cols = toks * p.group;
-      // keys that the tile's first and last token see
-      int64_t seen0 = row.k_len, seen1 = row.k_len;
-      if (p.causal) {
-        seen0 = min(seen0, max((int64_t)row.q_pos + tok0 + 1, (int64_t)0));
-        seen1 = min(seen1, max((int64_t)row.q_pos + tok0 + toks, (int64_t)0));
-      }
-      const int see_all = (int)seen0, see_any = (int)seen1;
-      const int first_sees = (int)min((int64_t)row.q_pos + tok0 + 1, (int64_t)(1 << 30));  // and one more per token
-      const int blk1 = min(blk0 + n, (see_any + 15) >> 4);  // blocks from here on hold nothing for this tile
+      const int64_t token = (int64_t)row.q_start + tok0;
+      // keys that the tile's first and last token see; each token sees one more than the one before it
+      const int first_sees =
+          p.causal ? (int)min((int64_t)row.q_pos + tok0 + 1, (int64_t)(1 << 30)) : row.k_len;
+      const int see_all = min(row.k_len, max(first_sees, 0));
+      const int see_any = p.causal ? min(row.k_len, max(first_sees + toks - 1, 0)) : row.k_len;
+      const int blk1 = min(blk0 + 2 * (int)n, (see_any + 15) >> 4);  // blocks from here on hold nothing for this tile
 
       // ---- block ids, 32 at a time; ring prologue
       const int32_t* table = p.block_table + (int64_t)r * p.bt_stride;
@@ -291,439 +627,197 @@ __global__ void __launch_bounds__(NW * 32, CTAS) q4_attention_kernel(const Q4Par
         }
         return id;
       };
-      int ids = load_id(blk0 + lane), ids_next = load_id(blk0 + 32 + lane);
+      int ids = load_id(blk0 + lane);
+      Queries<T, D, NT> queries;
+      fetch_queries(p, queries, token, kvh, cols, lane);
+      unsigned unread = 0;  // bits 2 s, 2 s + 1: that block of ring place s has no data
       uint32_t issued = it;
-      auto issue = [&](int b) {  // stage block b (of the row); called for blk0, blk0 + 1, ... in turn
+      // Stage blocks b and b + 1; called for blk0, blk0 + 2, ... in turn. Lanes 0..3 copy a row each.
+      auto stage = [&](int b) {
         const int j = b - blk0;
-        if (j > 0 && (j & 31) == 0) {
-          ids = ids_next;
-          ids_next = load_id(b + 32 + lane);
-        }
-        const int id = __shfl_sync(kFull, ids, j & 31);
-        if (lane == 0) {
-          const uint32_t s = issued % STAGES;
-          const uint32_t bar = bars + 8 * s, dst = ring_a + s * S::kStage;
-          if (id >= 0) {
-            const int64_t at = ((int64_t)id * p.hkv + kvh) * L::kRow;
-            mbar_arrive_expect_tx(bar, S::kStage);
-            bulk_g2s(dst, p.k_cache + at, L::kRow, bar);
-            bulk_g2s(dst + L::kRow, p.v_cache + at, L::kRow, bar);
-          } else {
-            mbar_arrive_expect_tx(bar, 0);
-          }
+        if (j > 0 && (j & 31) == 0) ids = load_id(b + lane);
+        const int id = __shfl_sync(kFull, ids, (j + ((lane >> 1) & 1)) & 31);
+        const unsigned read = __ballot_sync(kFull, id >= 0) & 5u;  // lanes 0 and 2
+        const uint32_t s = issued % STAGES;
+        const uint32_t bar = bars + 8 * s;
+        unread = (unread & ~(3u << (2 * s))) | ((read & 1 ? 0u : 1u) | (read & 4 ? 0u : 2u)) << (2 * s);
+        if (lane == 0) mbar_arrive_expect_tx(bar, __popc(read) * 2 * L::kRow);
+        __syncwarp();
+        if (lane < 4 && id >= 0) {
+          const int64_t at = ((int64_t)id * p.hkv + kvh) * L::kRow;
+          bulk_g2s(ring_a + s * S::kStage + lane * L::kRow, (lane & 1 ? p.v_cache : p.k_cache) + at, L::kRow, bar);
         }
         ++issued;
-        return id;
       };
-      uint32_t unread = 0;  // bit s: the block in ring place s could not be read
-      auto stage = [&](int b) {
-        const uint32_t s = issued % STAGES;
-        unread = (unread & ~(1u << s)) | (issue(b) < 0 ? 1u << s : 0u);
-      };
-      for (int b = blk0; b < min(blk0 + STAGES, blk1); ++b) stage(b);
+      for (int b = blk0; b < min(blk0 + 2 * STAGES, blk1); b += 2) stage(b);
 
-      // ---- Q as the B operand: column 8 nt + g, dims 16 t .. 16 t + 15 of every group
-      uint32_t qf[P * G][NT][4][2];
-      float qs[P * G][NT][2], ch[NT][2];
+      Tile<D, NT> u;
+      convert_queries(p, u, queries, lane);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const int col = nt * 8 + g;
-        const bool live = col < cols;
-        const int tk = live ? col / p.group : 0, hd = live ? col - tk * p.group : 0;
-        const T* src = reinterpret_cast<const T*>(p.q) + ((int64_t)row.q_start + tok0 + tk) * p.q_st +
-                       (int64_t)(kvh * p.group + hd) * p.q_sh + 16 * t;
-        float top = 0.f;
-        uint4 raw[P * G][2];
 #pragma unroll
-        for (int gr = 0; gr < P * G; ++gr)
+        for (int h = 0; h < 2; ++h) {
+          u.m[nt][h] = kNoMax;
+          u.l[nt][h] = 0.f;
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            raw[gr][h] = make_uint4(0u, 0u, 0u, 0u);
-            if (live) {
-              const T* at = src + gr * 64 + 8 * h;
-              if (p.vec) {
-                raw[gr][h] = *reinterpret_cast<const uint4*>(at);
-              } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) reinterpret_cast<T*>(&raw[gr][h])[e] = at[e];
-              }
-            }
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              top = q4::max_nan(top, fabsf(Elem<T>::to_float(reinterpret_cast<const T*>(&raw[gr][h])[e])));
-          }
-        top = q4::max_nan(top, __shfl_xor_sync(kFull, top, 1));
-        top = q4::max_nan(top, __shfl_xor_sync(kFull, top, 2));
-        // 2^-e with the largest element in [2^14, 2^15) after it
-        const int ex = top > 0.f ? min(max((int)((__float_as_uint(top) >> 23) & 255) - 127 - 14, -100), 112) : 0;
-        const float down = __uint_as_float((uint32_t)(127 - ex) << 23);
-#pragma unroll
-        for (int gr = 0; gr < P * G; ++gr) {
-          float sum = 0.f;
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {  // 4 elements: two that meet lower codes, two that meet upper ones
-            const T* e = reinterpret_cast<const T*>(&raw[gr][w >> 1]) + (w & 1) * 4;
-            const __half2 a = __floats2half2_rn(Elem<T>::to_float(e[0]) * down, Elem<T>::to_float(e[1]) * down);
-            const __half2 b = __floats2half2_rn(Elem<T>::to_float(e[2]) * (down * 0.0625f),
-                                                Elem<T>::to_float(e[3]) * (down * 0.0625f));
-            qf[gr][nt][w][0] = *reinterpret_cast<const uint32_t*>(&a);
-            qf[gr][nt][w][1] = *reinterpret_cast<const uint32_t*>(&b);
-            sum += __low2float(a) + __high2float(a) + 16.f * (__low2float(b) + __high2float(b));
-          }
-          sum += __shfl_xor_sync(kFull, sum, 1);
-          sum += __shfl_xor_sync(kFull, sum, 2);
-          sum *= 5.9604644775390625e-8f;  // 2^-24, as the codes carry it
-          qs[gr][nt][0] = __shfl_sync(kFull, sum, 8 * t);
-          qs[gr][nt][1] = __shfl_sync(kFull, sum, 8 * t + 4);
+          for (int gr = 0; gr < GR; ++gr) u.low[gr][nt][h] = 0.f;
         }
-        // back: 2^(ex + 24), in two steps where one would leave the range
-        const float up = fminf(fabsf(p.scale_log2) * 16777216.f, FLT_MAX) * __uint_as_float((uint32_t)(127 + ex) << 23);
-        const float c = copysignf(fminf(up, FLT_MAX), p.scale_log2);
-        ch[nt][0] = __shfl_sync(kFull, c, 8 * t);
-        ch[nt][1] = __shfl_sync(kFull, c, 8 * t + 4);
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int gr = 0; gr < GR; ++gr) {
+            u.one[gr / 2][nt][c] = 0.f;
+#pragma unroll
+            for (int mt = 0; mt < 4; ++mt) u.o[gr][mt][nt][c] = 0.f;
+          }
       }
-
-      // ---- the blocks
-      float m[NT][2], l[NT][2], low[P * G][NT][2], o[P * G][4][NT][4];
+      int end[NT][2];  // keys that the lane's columns see
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          m[nt][h] = kNoMax;
-          l[nt][h] = 0.f;
-#pragma unroll
-          for (int gr = 0; gr < P * G; ++gr) low[gr][nt][h] = 0.f;
-        }
-#pragma unroll
-      for (int gr = 0; gr < P * G; ++gr)
-#pragma unroll
-        for (int mt = 0; mt < 4; ++mt)
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) o[gr][mt][nt][c] = 0.f;
-      float v_down = 0.f;  // power of two that V's scales are taken by; 0 until a block sets it
+        for (int h = 0; h < 2; ++h)
+          end[nt][h] = p.causal ? min(row.k_len, first_sees + token_of(p, nt * 8 + 2 * t + h)) : row.k_len;
+      u.v_down = power2(60);  // the first scale moves it
 
-      for (int b = blk0; b < blk1; ++b, ++it) {
+      for (int b = blk0; b < blk1; b += 2, ++it) {
         const uint32_t s = it % STAGES;
         if (dead || !mbar_wait_bounded(bars + 8 * s, (it / STAGES) & 1)) {
           if (!dead && lane == 0) atomic_or_err(p.err, SEB_ERRBIT_TIMEOUT);
           dead = true;
           break;
         }
-        const char* kb = ring + s * S::kStage;
-        const char* vb = kb + L::kRow;
-        uint32_t kw[P][2][2 * G], vw[P][2][2 * G];  // words of keys g, g + 8; of key pairs t, t + 4
-        float2 kp[P * G][2], vp[P * G][2];          // (scale, low) of keys g, g + 8
+        const unsigned none = (unread >> (2 * s)) & 3;
+        const char* place = ring + s * S::kStage;
+        // two blocks at once where the tile leaves registers for it
+        constexpr int KB = GR * NT <= 2 ? 2 : 1;
+        if (none == 0 && (b + 2) * 16 <= see_all) {
 #pragma unroll
-        for (int pn = 0; pn < P; ++pn)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const char* ka = kb + pn * 8 * L::kWidth + (g + 8 * h) * (L::kWidth / 2) + t * (8 * G);
-            const char* va = vb + pn * 8 * L::kWidth + (t + 4 * h) * L::kWidth + (g ^ L::turn(t)) * (8 * G);
-            const char* kq = kb + L::kCodes + pn * 64 * G + (g + 8 * h) * 4 * G;
-            const char* vq = vb + L::kCodes + pn * 64 * G + (g + 8 * h) * 4 * G;
-            __half2 a[G], c[G];
-            if constexpr (G == 2) {
-              *reinterpret_cast<uint4*>(kw[pn][h]) = *reinterpret_cast<const uint4*>(ka);
-              *reinterpret_cast<uint4*>(vw[pn][h]) = *reinterpret_cast<const uint4*>(va);
-              *reinterpret_cast<uint2*>(a) = *reinterpret_cast<const uint2*>(kq);
-              *reinterpret_cast<uint2*>(c) = *reinterpret_cast<const uint2*>(vq);
-            } else {
-              *reinterpret_cast<uint2*>(kw[pn][h]) = *reinterpret_cast<const uint2*>(ka);
-              *reinterpret_cast<uint2*>(vw[pn][h]) = *reinterpret_cast<const uint2*>(va);
-              *reinterpret_cast<uint32_t*>(a) = *reinterpret_cast<const uint32_t*>(kq);
-              *reinterpret_cast<uint32_t*>(c) = *reinterpret_cast<const uint32_t*>(vq);
-            }
-#pragma unroll
-            for (int gr = 0; gr < G; ++gr) {
-              kp[pn * G + gr][h] = __half22float2(a[gr]);
-              vp[pn * G + gr][h] = __half22float2(c[gr]);
-            }
-          }
-        const bool bad_block = (unread >> s) & 1;
-        __syncwarp();  // every lane has its words: the place may be filled again
-        if (b + STAGES < blk1) stage(b + STAGES);
-
-        // S^T = K Q^T: 16 keys x 8 NT columns, one sum for each group
-        float x[NT][4];
-#pragma unroll
-        for (int gr = 0; gr < P * G; ++gr) {
-          float acc[NT][4];
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) acc[nt][c] = 0.f;
-#pragma unroll
-          for (int w = 0; w < 2; ++w) {
-            uint32_t k0 = kw[gr / G][0][gr % G * 2 + w], k1 = kw[gr / G][1][gr % G * 2 + w];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt)
-                Mma<__half>::run(acc[nt], k0 & 0x000f000fu, k1 & 0x000f000fu, k0 & 0x00f000f0u, k1 & 0x00f000f0u,
-                                 qf[gr][nt][2 * w + h][0], qf[gr][nt][2 * w + h][1]);
-              k0 >>= 8, k1 >>= 8;
-            }
-          }
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              const float2 pr = kp[gr][c >> 1];
-              const float base = gr == 0 ? pr.y * qs[gr][nt][c & 1] : fmaf(pr.y, qs[gr][nt][c & 1], x[nt][c]);
-              x[nt][c] = fmaf(pr.x, acc[nt][c], base);
-            }
+          for (int i = 0; i < 2; i += KB)
+            take_blocks<D, NT, KB, false>(u, place + i * 2 * L::kRow, lane, (b + i) * 16, 0, end);
+        } else {
+#pragma unroll 1
+          for (int i = 0; i < 2; ++i)
+            take_blocks<D, NT, 1, true>(u, place + i * 2 * L::kRow, lane, (b + i) * 16, (none >> i) & 1, end);
         }
-        // masked keys: score -inf, and no parameter of theirs (it may be NaN) meets a zero weight
-        const int key = b * 16 + g;
-        const bool masked = bad_block || (b + 1) * 16 > see_all;
-        bool hide[NT][4];
-        if (masked) {
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              const int tk = (nt * 8 + 2 * t + (c & 1)) / p.group;
-              const int last = p.causal ? min(row.k_len, first_sees + tk) : row.k_len;
-              hide[nt][c] = bad_block || key + 8 * (c >> 1) >= last;
-            }
-        }
-        float d[NT][4], far = -INFINITY;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            d[nt][c] = fmaf(x[nt][c], ch[nt][c & 1], -m[nt][c & 1]);
-            if (masked && hide[nt][c]) d[nt][c] = -INFINITY;
-            far = fmaxf(far, d[nt][c]);
-          }
-        float sv[P * G][2], big = 0.f;
-#pragma unroll
-        for (int gr = 0; gr < P * G; ++gr)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            sv[gr][h] = vp[gr][h].x * v_down;
-            big = fmaxf(big, sv[gr][h]);
-          }
-        if (__any_sync(kFull, far > kThreshold || big > kScaleThreshold || v_down == 0.f)) {
-          // move the references: scores' maxima, and the power of two of V's scales
-          float vmax = 0.f;
-#pragma unroll
-          for (int gr = 0; gr < P * G; ++gr)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) vmax = fmaxf(vmax, key + 8 * h < see_any && !bad_block ? vp[gr][h].x : 0.f);
-#pragma unroll
-          for (int k = 16; k >= 1; k >>= 1) vmax = fmaxf(vmax, __shfl_xor_sync(kFull, vmax, k));
-          float v_fix = 1.f;
-          if (v_down == 0.f || vmax * v_down > kScaleThreshold) {
-            const int ex = min(max((int)((__float_as_uint(vmax) >> 23) & 255) - 127, -24), 16);
-            const float now = __uint_as_float((uint32_t)(127 - ex) << 23);
-            v_fix = v_down == 0.f ? 1.f : now / v_down;
-            v_down = now;
-#pragma unroll
-            for (int gr = 0; gr < P * G; ++gr)
-#pragma unroll
-              for (int h = 0; h < 2; ++h) sv[gr][h] = vp[gr][h].x * v_down;
-          }
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              float mx = -INFINITY;
-#pragma unroll
-              for (int c = h; c < 4; c += 2)
-                if (!(masked && hide[nt][c])) mx = fmaxf(mx, __fmul_rn(x[nt][c], ch[nt][h]));
-              mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 4));
-              mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 8));
-              mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 16));
-              const float now = fmaxf(mx, m[nt][h]);
-              const float fix = m[nt][h] == kNoMax ? 0.f : exp2f(m[nt][h] - now);
-              m[nt][h] = now;
-              l[nt][h] *= fix;
-#pragma unroll
-              for (int gr = 0; gr < P * G; ++gr) {
-                low[gr][nt][h] *= fix;
-#pragma unroll
-                for (int mt = 0; mt < 4; ++mt) {
-                  o[gr][mt][nt][h] *= fix * v_fix;
-                  o[gr][mt][nt][h + 2] *= fix * v_fix;
-                }
-              }
-#pragma unroll
-              for (int c = h; c < 4; c += 2)  // the product rounded as in `now`: the largest score gets 0, however large
-                d[nt][c] = masked && hide[nt][c] ? -INFINITY : __fsub_rn(__fmul_rn(x[nt][c], ch[nt][h]), now);
-            }
-        }
-        float pr[NT][4];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c) pr[nt][c] = exp2f(d[nt][c]);
-          l[nt][0] += pr[nt][0] + pr[nt][2];
-          l[nt][1] += pr[nt][1] + pr[nt][3];
-        }
-
-        // O^T += V^T (P sV)^T, and the lows' share
-#pragma unroll
-        for (int gr = 0; gr < P * G; ++gr) {
-          uint32_t b0[NT], b1[NT];
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            float w[4], z[4];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              w[c] = pr[nt][c] * sv[gr][c >> 1];
-              z[c] = pr[nt][c] * vp[gr][c >> 1].y;
-              if (masked && hide[nt][c]) w[c] = z[c] = 0.f;
-            }
-            low[gr][nt][0] += z[0] + z[2];
-            low[gr][nt][1] += z[1] + z[3];
-            b0[nt] = movmatrix_trans(Mma<__half>::pack(w[0], w[1]));
-            b1[nt] = movmatrix_trans(Mma<__half>::pack(w[2], w[3]));
-          }
-#pragma unroll
-          for (int w = 0; w < 2; ++w) {
-            uint32_t v0 = vw[gr / G][0][gr % G * 2 + w], v1 = vw[gr / G][1][gr % G * 2 + w];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt)
-                Mma<__half>::run(o[gr][2 * w + h][nt], v0 & 0x000f000fu, v0 & 0x00f000f0u, v1 & 0x000f000fu,
-                                 v1 & 0x00f000f0u, b0[nt], b1[nt]);
-              v0 >>= 8, v1 >>= 8;
-            }
-          }
-        }
+        __syncwarp();  // every lane has read the place: it may be filled again
+        if (b + 2 * STAGES < blk1) stage(b + 2 * STAGES);
       }
       if (dead)  // leave no copy in flight behind
         for (; it != issued; ++it) mbar_wait_bounded(bars + 8 * (it % STAGES), (it / STAGES) & 1, 1u << 16);
 
-      // ---- the unit's result, or this warp's part of it
-      const float v_up = v_down == 0.f ? 0.f : 16777216.f / v_down;
-      const bool whole = blk0 == 0 && n == row.nblk;
+      // ---- the result, or this warp's part of it, by way of shared memory. Nothing is in flight to the ring now.
+      const bool whole = n == row.pairs;
       const bool last_run = pos + n == stop;
-      float* po = reinterpret_cast<float*>(last_run ? ring : ring + S::kRing);
+      float* po = reinterpret_cast<float*>(whole || last_run ? ring : ring + S::kRing);
+      const float v_up = power2(24) / u.v_down;
       __syncwarp();
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          float lt = l[nt][h];
+          const int col = nt * 8 + 2 * t + h;
+          float lt = u.l[nt][h];
 #pragma unroll
           for (int k = 4; k <= 16; k <<= 1) lt += __shfl_xor_sync(kFull, lt, k);
-          const int col = nt * 8 + 2 * t + h;
-          const float mm = m[nt][h] == kNoMax ? -INFINITY : m[nt][h];
-          const float inv = whole ? (lt == 0.f ? 0.f : 1.f / lt) : 1.f;
-          const int tk = col / p.group, hd = col - tk * p.group;
-          const int64_t tok = (int64_t)row.q_start + tok0 + tk;
 #pragma unroll
-          for (int gr = 0; gr < P * G; ++gr) {
-            float z = low[gr][nt][h];
+          for (int gr = 0; gr < GR; ++gr) {
+            float z = u.low[gr][nt][h];
 #pragma unroll
             for (int k = 4; k <= 16; k <<= 1) z += __shfl_xor_sync(kFull, z, k);
-            if (col >= cols) continue;
+            const float one = u.one[gr / 2][nt][(gr & 1) * 2 + h] * (8.f * power2(-24));
             float v[8];
 #pragma unroll
             for (int mt = 0; mt < 4; ++mt) {
-              v[2 * mt] = fmaf(o[gr][mt][nt][h], v_up, z) * inv;
-              v[2 * mt + 1] = fmaf(o[gr][mt][nt][h + 2], v_up * 0.0625f, z) * inv;
+              v[2 * mt] = fmaf(u.o[gr][mt][nt][h] - one, v_up, z);
+              v[2 * mt + 1] = fmaf(fmaf(u.o[gr][mt][nt][h + 2], 0.0625f, -one), v_up, z);
             }
-            const int dim = gr * 64 + g * 8;
-            if (!whole) {
-              float4* dst = reinterpret_cast<float4*>(po + col * D + dim);
+            if (col < cols) {
+              float4* dst = reinterpret_cast<float4*>(po + col * D + gr * 64 + g * 8);
               dst[0] = make_float4(v[0], v[1], v[2], v[3]);
               dst[1] = make_float4(v[4], v[5], v[6], v[7]);
-            } else {
-              T* dst = reinterpret_cast<T*>(p.out) + tok * p.o_st + (int64_t)(kvh * p.group + hd) * p.o_sh + dim;
-              T r8[8];
-#pragma unroll
-              for (int e = 0; e < 8; ++e) r8[e] = Elem<T>::from_float(v[e]);
-              if (p.vec) {
-                *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(r8);
-              } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) dst[e] = r8[e];
-              }
             }
           }
-          if (g == 0 && col < cols) {
-            if (!whole) {
-              po[kCols * D + 2 * col] = mm;
-              po[kCols * D + 2 * col + 1] = lt;
-            } else {
-              p.lse[tok * p.lse_st + kvh * p.group + hd] = lt == 0.f ? -INFINITY : fmaf(mm, kLn2, logf(lt));
-            }
-          }
+          if (g == 0 && col < cols)
+            reinterpret_cast<float2*>(po + kCols * D)[col] =
+                make_float2(u.m[nt][h] == kNoMax ? -INFINITY : u.m[nt][h], lt);
         }
-      if (!whole && lane == 0) {
-        const int64_t first = pos - blk0;
-        parts[warp * 2 + (last_run ? 1 : 0)] = Part{first, first + row.nblk, r, tile, kvh, cols};
+      __syncwarp();
+      if (whole) {
+#pragma unroll 1
+        for (int col = 0; col < cols; ++col) {
+          float o[D / 32];
+          load_dims<D, false>(po + col * D, lane, o);
+          const float2 ml = reinterpret_cast<const float2*>(po + kCols * D)[col];
+          write_column<T, D>(p, token, kvh, col, lane, o, ml.x, ml.y);
+        }
+      } else if (lane == 0) {
+        parts[warp * 2 + (last_run ? 1 : 0)] = Part{pos - pair0, pos - pair0 + row.pairs, token, kvh, cols};
       }
+      fence_proxy_async_smem();  // the ring is written by copies next
+      __syncwarp();
       pos += n;
       off += n;
     }
   }
 
-  // ---- join the parts. Neighbours of one unit are neighbours in the list; a warp takes a column.
+  // ---- join the parts. A unit's parts are one of each of neighbouring warps, so in the list of
+  // 2 NW places neighbours but for empty places; a bit of a mask stands for each place. A warp
+  // takes a column; of units that go on in other CTAs first, so that their arrival is early.
   __syncthreads();
   const float* base = reinterpret_cast<const float*>(smem + S::kWarps);
-  auto part_at = [&](int i) { return base + ((i >> 1) * S::kWarp + ((i & 1) ? 0 : S::kRing)) / 4; };
-  int job = 0;
-  for (int i = 0; i < 2 * NW;) {
-    const Part pt = parts[i];
-    if (pt.unit < 0) {
-      ++i;
-      continue;
-    }
-    int n = 0, j = i;
-    unsigned list = 0;  // bit k: entry k is a part of this unit
-    for (; j < 2 * NW; ++j) {
-      if (parts[j].unit < 0) continue;
-      if (parts[j].unit != pt.unit) break;
-      list |= 1u << j;
-      ++n;
-    }
-    i = j;
-    for (int col = 0; col < pt.cols; ++col, ++job) {
-      if (job % NW != warp) continue;
-      float o[D / 32], m, l;
-      join<D, false>(n, lane, [&](int k, const float*& row, const float2*& ml) {
-        const float* at = part_at(__fns(list, 0, k + 1));
-        row = at + col * D;
-        ml = reinterpret_cast<const float2*>(at + kCols * D) + col;
-      }, o, m, l);
-      if (pt.unit < cta0 || pt.end > cta1) {  // the unit goes on in other CTAs
-        const int64_t span = NW * per;
-        const int first = (int)(pt.unit / span), last = (int)((pt.end - 1) / span);
-        const int64_t slot = ((int64_t)blockIdx.x * 2 + (pt.unit >= cta0 ? 1 : 0)) * kCols + col;
-        float* dst = p.ws_o + slot * D + lane * (D / 32);
-#pragma unroll
-        for (int e = 0; e < D / 32; ++e) dst[e] = o[e];
-        if (lane == 0) reinterpret_cast<float2*>(p.ws_ml)[slot] = make_float2(m, l);
-        __threadfence();
-        __syncwarp();
-        int32_t* ctr = g_q4_counters[p.counter_slot] + first * kCols + col;
-        int arrived = 0;
-        if (lane == 0) arrived = atomicAdd(ctr, 1);
-        arrived = __shfl_sync(kFull, arrived, 0);
-        if (arrived != last - first) continue;
-        if (lane == 0) *ctr = 0;
-        __threadfence();
-        join<D, true>(last - first + 1, lane, [&](int k, const float*& row, const float2*& ml) {
-          const int64_t at = ((int64_t)(first + k) * 2 + (k == 0 ? 1 : 0)) * kCols + col;
-          row = p.ws_o + at * D;
-          ml = reinterpret_cast<const float2*>(p.ws_ml) + at;
+  uint32_t unit = 0, end = 0;
+  if (lane < 2 * NW) {
+    unit = parts[lane].unit;
+    end = parts[lane].end;
+  }
+  const unsigned used = __ballot_sync(kFull, end != 0);
+  const unsigned below = used & ((1u << lane) - 1);
+  const uint32_t before_me = __shfl_sync(kFull, unit, below ? 31 - __clz(below) : 0);
+  const unsigned starts = __ballot_sync(kFull, end != 0 && (below == 0 || before_me != unit));
+  const unsigned spanning = __ballot_sync(kFull, end != 0 && (unit < cta0 || end > cta1)) & starts;
+#pragma unroll 1
+  for (int pass = 0; pass < 2; ++pass) {
+    int job = 0;
+#pragma unroll 1
+    for (unsigned left = pass == 0 ? spanning : starts & ~spanning; left; left &= left - 1) {
+      const int i = __ffs(left) - 1, w0 = i >> 1;
+      const unsigned later = starts & ~((2u << i) - 1);  // the next unit's first place and on
+      const unsigned list = used & ~((1u << i) - 1) & (later ? (1u << (__ffs(later) - 1)) - 1 : ~0u);
+      const int n = __popc(list);
+      const Part pt = parts[i];
+#pragma unroll 1
+      for (int col = (warp + NW - job % NW) % NW; col < pt.cols; col += NW) {
+        float o[D / 32], m, l;
+        join<D, 8, false>(n, lane, [&](int k, const float*& row, const float2*& ml) {
+          const float* at = base + ((w0 + k) * S::kWarp + (list >> (2 * (w0 + k)) & 1 ? S::kRing : 0)) / 4;
+          row = at + col * D;
+          ml = reinterpret_cast<const float2*>(at + kCols * D) + col;
         }, o, m, l);
-      }
-      const int tk = col / p.group, hd = col - tk * p.group;
-      const int64_t tok = (int64_t)__ldg(p.q_starts + pt.row) + pt.tile * p.tile + tk;
-      const int head = pt.kvh * p.group + hd;
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-      T* dst = reinterpret_cast<T*>(p.out) + tok * p.o_st + (int64_t)head * p.o_sh + lane * (D / 32);
+        if (pass == 0) {
+          const int first = pt.unit / span, last = (pt.end - 1) / span;
+          const int64_t slot = ((int64_t)blockIdx.x * 2 + (pt.unit >= cta0 ? 1 : 0)) * kCols + col;
+          float* dst = p.ws_o + slot * D + lane * (D / 32);
 #pragma unroll
-      for (int e = 0; e < D / 32; ++e) dst[e] = Elem<T>::from_float(o[e] * inv);
-      if (lane == 0) p.lse[tok * p.lse_st + head] = l == 0.f ? -INFINITY : fmaf(m, kLn2, logf(l));
+          for (int e = 0; e < D / 32; ++e) dst[e] = o[e];
+          if (lane == 0) reinterpret_cast<float2*>(p.ws_ml)[slot] = make_float2(m, l);
+          __threadfence();
+          __syncwarp();
+          int32_t* ctr = g_q4_counters[p.counter_slot] + first * kCols + col;
+          int arrived = 0;
+          if (lane == 0) arrived = atomicAdd(ctr, 1);
+          arrived = __shfl_sync(kFull, arrived, 0);
+          if (arrived != last - first) continue;
+          if (lane == 0) *ctr = 0;
+          __threadfence();
+          join<D, 32, true>(last - first + 1, lane, [&](int k, const float*& row, const float2*& ml) {
+            const int64_t at = ((int64_t)(first + k) * 2 + (k == 0 ? 1 : 0)) * kCols + col;
+            row = p.ws_o + at * D;
+            ml = reinterpret_cast<const float2*>(p.ws_ml) + at;
+          }, o, m, l);
+        }
+        write_column<T, D>(p, pt.token, pt.kvh, col, lane, o, m, l);
+      }
+      job += pt.cols;
     }
   }
 }
@@ -731,20 +825,16 @@ __global__ void __launch_bounds__(NW * 32, CTAS) q4_attention_kernel(const Q4Par
 // Warps of a CTA and CTAs of an SM by the columns of a warp's tile, as registers allow.
 template <int D, int NT>
 struct Shape {
-  static constexpr int kRegs = D / 64 * NT;  // a measure of the tile's accumulators
-  static constexpr int kWarps = kRegs <= 2 ? 8 : kRegs <= 4 ? 4 : 6;
-  static constexpr int kCtas = kRegs <= 2 ? 2 : kRegs <= 4 ? 3 : 1;
-  static constexpr int kStages = D == 256 ? 2 : 4;
+  static constexpr int kSize = D / 64 * NT;  // a measure of the tile's accumulators
+  static constexpr int kWarps = kSize <= 2 ? 8 : kSize <= 4 ? 4 : 6;
+  static constexpr int kCtas = kSize <= 2 ? 2 : kSize <= 4 ? 3 : 1;
+  static constexpr int kStages = D == 64 ? 4 : D == 128 ? 2 : 1;
 };
 
-// Columns (in eights) of a warp's tile: enough for the group, and for the tokens of an average row.
-int tiles_of_columns(int group, int head_dim, int rows, int total_query) {
-  const int most = head_dim == 256 ? 2 : 4;
-  const int64_t tokens = (total_query + (int64_t)rows - 1) / rows;
-  const int64_t cols = group * std::max<int64_t>(tokens, 1);
-  int nt = cols <= 8 ? 1 : cols <= 16 ? 2 : 4;
-  if (group > 8 && nt < 2) nt = 2;
-  return std::min(nt, most);
+// Columns (in eights) of a warp's tile: enough for the group, and for more tokens where rows
+// have several and the registers hold them.
+int column_tiles(int group, int head_dim, int rows, int total_query) {
+  return group > 8 || (total_query > rows && head_dim <= 128) ? 2 : 1;
 }
 
 template <int D, int NT>
@@ -773,21 +863,32 @@ int launch(Q4Params& p, void* workspace, int64_t bytes, cudaStream_t s) {
   p.ws_o = static_cast<float*>(workspace);
   p.ws_ml = p.ws_o + (int64_t)ctas * 2 * 8 * NT * D;
   p.tile = std::max(1, 8 * NT / p.group);
+  p.by_group = (65536 + p.group - 1) / p.group;
   const int rc = set_smem_limit_once<kern>(smem);
   if (rc != SEB_OK) return rc;
-  kern<<<ctas, Sh::kWarps * 32, smem, s>>>(p);
+  // no more CTAs than the longest rows that the table allows would fill
+  const int64_t tiles = ((int64_t)p.total_query + (int64_t)p.num_rows * (p.tile - 1)) / p.tile;
+  const int64_t pairs = tiles * p.hkv * ((p.max_blocks + 1) / 2);
+  if (pairs > 0xffff0000ll) {
+    set_error("seb_paged_attention_q4: %lld tiles of %lld blocks are too much work for one call", (long long)tiles * p.hkv,
+              (long long)p.max_blocks);
+    return SEB_EUNSUPPORTED;
+  }
+  const int64_t most = (pairs + Sh::kWarps * kMinRun - 1) / (Sh::kWarps * kMinRun);
+  kern<<<(unsigned)std::min<int64_t>(ctas, most), Sh::kWarps * 32, smem, s>>>(p);
   return launch_status("q4_attention_kernel");
 }
 
+template <typename T, int D>
+int launch_columns(Q4Params& p, int nt, void* workspace, int64_t bytes, cudaStream_t s) {
+  return nt == 1 ? launch<T, D, 1>(p, workspace, bytes, s) : launch<T, D, 2>(p, workspace, bytes, s);
+}
+
 template <typename T>
-int launch_shape(Q4Params& p, int d, int nt, void* workspace, int64_t bytes, cudaStream_t s) {
-  if (d == 64)
-    return nt == 1 ? launch<T, 64, 1>(p, workspace, bytes, s)
-                   : nt == 2 ? launch<T, 64, 2>(p, workspace, bytes, s) : launch<T, 64, 4>(p, workspace, bytes, s);
-  if (d == 128)
-    return nt == 1 ? launch<T, 128, 1>(p, workspace, bytes, s)
-                   : nt == 2 ? launch<T, 128, 2>(p, workspace, bytes, s) : launch<T, 128, 4>(p, workspace, bytes, s);
-  return nt == 1 ? launch<T, 256, 1>(p, workspace, bytes, s) : launch<T, 256, 2>(p, workspace, bytes, s);
+int launch_dim(Q4Params& p, int d, int nt, void* workspace, int64_t bytes, cudaStream_t s) {
+  return d == 64 ? launch_columns<T, 64>(p, nt, workspace, bytes, s)
+                 : d == 128 ? launch_columns<T, 128>(p, nt, workspace, bytes, s)
+                            : launch_columns<T, 256>(p, nt, workspace, bytes, s);
 }
 
 }  // namespace
@@ -797,10 +898,9 @@ extern "C" int64_t seb_paged_attention_q4_workspace_size(int32_t num_rows, int32
                                                          int32_t num_kv_heads, int32_t head_dim) {
   using namespace seb;
   if (num_rows <= 0 || total_query <= 0 || num_q_heads <= 0 || num_kv_heads <= 0) return 0;
-  const int nt = tiles_of_columns(num_q_heads / num_kv_heads, head_dim, num_rows, total_query);
-  if (head_dim == 64) return nt == 1 ? workspace_of<64, 1>() : nt == 2 ? workspace_of<64, 2>() : workspace_of<64, 4>();
-  if (head_dim == 128)
-    return nt == 1 ? workspace_of<128, 1>() : nt == 2 ? workspace_of<128, 2>() : workspace_of<128, 4>();
+  const int nt = column_tiles(num_q_heads / num_kv_heads, head_dim, num_rows, total_query);
+  if (head_dim == 64) return nt == 1 ? workspace_of<64, 1>() : workspace_of<64, 2>();
+  if (head_dim == 128) return nt == 1 ? workspace_of<128, 1>() : workspace_of<128, 2>();
   return head_dim == 256 ? (nt == 1 ? workspace_of<256, 1>() : workspace_of<256, 2>()) : 0;
 }
 
@@ -837,6 +937,9 @@ extern "C" int seb_paged_attention_q4(const void* q, int64_t q_stride_token, int
   SEB_CHECK_ARG(aligned(k_cache, 16) && aligned(v_cache, 16), "seb_paged_attention_q4: the pool must be 16-byte aligned");
   SEB_CHECK_ARG(counter_slot >= 0 && counter_slot < SEB_Q4_COUNTER_SLOTS,
                 "seb_paged_attention_q4: counter_slot %d outside [0, %d)", counter_slot, SEB_Q4_COUNTER_SLOTS);
+  SEB_CHECK_ARG(aligned(q, 16) && aligned(out, 16) && q_stride_token % 8 == 0 && q_stride_head % 8 == 0 &&
+                    out_stride_token % 8 == 0 && out_stride_head % 8 == 0,
+                "seb_paged_attention_q4: rows of q and out must be 16-byte aligned");
   Q4Params p{};
   p.counter_slot = counter_slot;
   p.q = static_cast<const char*>(q);
@@ -859,16 +962,14 @@ extern "C" int seb_paged_attention_q4(const void* q, int64_t q_stride_token, int
   p.group = group;
   p.scale_log2 = scale * kLog2e;
   p.causal = is_causal ? 1 : 0;
-  p.vec = aligned(q, 16) && aligned(out, 16) && q_stride_token % 8 == 0 && q_stride_head % 8 == 0 &&
-          out_stride_token % 8 == 0 && out_stride_head % 8 == 0;
   p.out = static_cast<char*>(out);
   p.o_st = out_stride_token;
   p.o_sh = out_stride_head;
   p.lse = lse;
   p.lse_st = lse_stride_token;
   p.err = err;
-  const int nt = tiles_of_columns(group, head_dim, num_rows, total_query);
+  const int nt = column_tiles(group, head_dim, num_rows, total_query);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return dtype == SEB_BF16 ? launch_shape<__nv_bfloat16>(p, head_dim, nt, workspace, workspace_bytes, s)
-                           : launch_shape<__half>(p, head_dim, nt, workspace, workspace_bytes, s);
+  return dtype == SEB_BF16 ? launch_dim<__nv_bfloat16>(p, head_dim, nt, workspace, workspace_bytes, s)
+                           : launch_dim<__half>(p, head_dim, nt, workspace, workspace_bytes, s);
 }

@@ -62,6 +62,11 @@ def _check_planes(name: str, k_cache: torch.Tensor, v_cache: torch.Tensor, num_k
         raise ValueError(f"{name}: k_cache and v_cache must be contiguous and of equal shape")
 
 
+def _aligned(t: torch.Tensor) -> bool:
+    """Whether a [tokens, heads, head_dim] tensor's rows are 16-byte aligned."""
+    return t.data_ptr() % 16 == 0 and t.stride(0) % 8 == 0 and t.stride(1) % 8 == 0
+
+
 def _check_slots(name: str, slots: torch.Tensor, n: int) -> torch.Tensor:
     if slots.dtype != torch.int64 or slots.dim() != 1 or slots.numel() != n:
         raise ValueError(f"{name}: slot_mapping must be int64 [{n}]")
@@ -221,8 +226,12 @@ def paged_attention_q4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
                          f"got {tuple(block_table.shape)}")
     if block_table.stride(1) != 1:
         block_table = block_table.contiguous()
+    if not _aligned(q):
+        q = q.contiguous()
+        if not _aligned(q):
+            q = q.clone()
     if out is None:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        out = torch.empty((total_q, num_q_heads, d), dtype=q.dtype, device=dev)
     elif out.shape != q.shape or out.stride(2) != 1 or out.dtype != q.dtype or out.device != dev:
         raise ValueError("paged_attention_q4: out must match q, with unit stride on head_dim")
     if lse is None:
@@ -236,6 +245,9 @@ def paged_attention_q4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
         out.zero_()
         lse.fill_(float("-inf"))
         return out, lse
+    result = out
+    if not _aligned(out):
+        out = result.clone(memory_format=torch.contiguous_format)
     nbytes = lib().seb_paged_attention_q4_workspace_size(rows, total_q, num_q_heads, num_kv_heads, d)
     stream = _stream(dev)
     ws, slot = _workspace(dev, stream, nbytes)
@@ -248,4 +260,6 @@ def paged_attention_q4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
     check("seb_paged_attention_q4", st)
     LAUNCHES[0] += 1
     _after(dev)
-    return out, lse
+    if result is not out:
+        result.copy_(out)
+    return result, lse
