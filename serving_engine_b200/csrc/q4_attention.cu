@@ -26,7 +26,7 @@
 // a row, up to 8 * NT columns) on one tile, so each KV byte is read once per tile.
 // Parts of a unit are joined in shared memory, and over CTAs in the workspace by the
 // last to arrive, in order of their place, so results do not depend on timing.
-#include "q4_format.cuh"
+#include "q4_attention.cuh"
 
 #include <algorithm>
 #include <cfloat>
@@ -34,76 +34,16 @@
 namespace seb {
 namespace {
 
-constexpr unsigned kFull = 0xffffffffu;
-constexpr float kLn2 = 0.69314718055994530942f;
-constexpr float kLog2e = 1.44269504088896340736f;
 constexpr uint32_t kMinRun = 2;          // pairs of blocks of the shortest run worth a warp
 constexpr float kNoMax = -FLT_MAX;       // no score yet: any score is above it by more than the threshold
 constexpr float kThreshold = 8.f;        // scores may exceed the reference by 2^8 before it is moved
 constexpr float kScaleThreshold = 64.f;  // p * V scale stays below 2^8 * 2^6
-
-struct Q4Params {
-  const char* q;
-  int64_t q_st, q_sh;  // elements
-  const char* k_cache;
-  const char* v_cache;
-  int64_t num_blocks;
-  const int32_t* block_table;
-  int64_t bt_stride;
-  int64_t max_blocks;
-  const int32_t* q_starts;
-  const int32_t* q_lens;
-  const int32_t* k_lens;
-  const int32_t* q_pos;
-  int32_t num_rows;
-  int32_t total_query;
-  int32_t hq, hkv, group;
-  int32_t tile;       // tokens of a tile
-  uint32_t by_group;  // col / group == col * by_group >> 16 for the columns of a tile
-  float scale_log2;
-  int32_t causal;
-  char* out;
-  int64_t o_st, o_sh;  // elements
-  float* lse;
-  int64_t lse_st;
-  int32_t counter_slot;
-  float* ws_o;        // [CTA][2][columns][D]
-  float* ws_ml;       // [CTA][2][columns][2]
-  int32_t* err;
-};
 
 // Arrivals at the units that span CTAs, one for each column, at the CTA that a unit
 // starts in. Zero when the library is loaded, and again after every call (the last to
 // arrive clears it); calls that may overlap use different slots.
 constexpr int kMaxCtas = 512;
 __device__ int32_t g_q4_counters[SEB_Q4_COUNTER_SLOTS][kMaxCtas * 32];
-
-struct Row {
-  int q_len, q_start, q_pos, k_len;
-  uint32_t pairs;  // pairs of blocks of each of its units; at least 1
-  uint32_t tiles;
-};
-
-__device__ __forceinline__ Row row_of(const Q4Params& p, int r, uint32_t* bad) {
-  Row w;
-  w.q_len = max(__ldg(p.q_lens + r), 0);
-  w.q_start = __ldg(p.q_starts + r);
-  w.q_pos = __ldg(p.q_pos + r);
-  w.k_len = max(__ldg(p.k_lens + r), 0);
-  if (w.q_len > 0 && (w.q_start < 0 || (int64_t)w.q_start + w.q_len > p.total_query)) {
-    *bad |= SEB_ERRBIT_META;
-    w.q_len = 0;
-  }
-  if (w.k_len > p.max_blocks * kBlockSize) {
-    *bad |= SEB_ERRBIT_KLEN;
-    w.k_len = (int)(p.max_blocks * kBlockSize);
-  }
-  int64_t seen = w.k_len;
-  if (p.causal) seen = min(seen, (int64_t)w.q_pos + w.q_len);
-  w.pairs = (uint32_t)max((int)((seen + 31) >> 5), 1);
-  w.tiles = (w.q_len + p.tile - 1) / p.tile;
-  return w;
-}
 
 __device__ __forceinline__ uint32_t pairs_of(const Q4Params& p, const Row& w) { return w.tiles * p.hkv * w.pairs; }
 
@@ -136,10 +76,6 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// 2^e as a float, e in [-126, 127]; and the exponent of a float that is not subnormal
-__device__ __forceinline__ float power2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
-__device__ __forceinline__ int exponent(float x) { return (int)((__float_as_uint(x) >> 23) & 255) - 127; }
-
 // The token, of its tile, of a column.
 __device__ __forceinline__ int token_of(const Q4Params& p, int col) { return (int)(col * p.by_group >> 16); }
 
@@ -241,20 +177,6 @@ struct Tile {
   float v_down;               // power of two that V's scales are taken by
 };
 
-template <typename T> struct Two;
-template <> struct Two<__half> {
-  using type = __half2;
-  static __device__ __forceinline__ type zero() { return __half2half2(__ushort_as_half(0)); }
-};
-template <> struct Two<__nv_bfloat16> {
-  using type = __nv_bfloat162;
-  static __device__ __forceinline__ type zero() { return __bfloat162bfloat162(__ushort_as_bfloat16(0)); }
-};
-__device__ __forceinline__ __half low_of(__half2 x) { return __low2half(x); }
-__device__ __forceinline__ __half high_of(__half2 x) { return __high2half(x); }
-__device__ __forceinline__ __nv_bfloat16 low_of(__nv_bfloat162 x) { return __low2bfloat16(x); }
-__device__ __forceinline__ __nv_bfloat16 high_of(__nv_bfloat162 x) { return __high2bfloat16(x); }
-
 // A lane's share of the columns' queries, as they are.
 template <typename T, int D, int NT>
 struct Queries {
@@ -295,7 +217,7 @@ __device__ __forceinline__ void convert_queries(const Q4Params& p, Tile<D, NT>& 
     float top = q4::max_nan(Elem<T>::to_float(low_of(most)), Elem<T>::to_float(high_of(most)));
     top = q4::max_nan(top, __shfl_xor_sync(kFull, top, 1));
     top = q4::max_nan(top, __shfl_xor_sync(kFull, top, 2));
-    const int ex = top > 0.f ? min(max(exponent(top) - 14, -100), 112) : 0;  // the largest goes to [2^14, 2^15)
+    const int ex = query_exponent(top);
     const float down = power2(-ex);
 #pragma unroll
     for (int gr = 0; gr < GR; ++gr) {
@@ -540,7 +462,7 @@ __global__ void __launch_bounds__(NW * 32, CTAS) q4_attention_kernel(const Q4Par
   {
     uint32_t sum = 0, bad = 0;
 #pragma unroll 1
-    for (int r = tid * chunk; r < min((tid + 1) * chunk, p.num_rows); ++r) sum += pairs_of(p, row_of(p, r, &bad));
+    for (int r = tid * chunk; r < min((tid + 1) * chunk, p.num_rows); ++r) sum += pairs_of(p, row_of<false>(p, r, &bad));
     if (bad && blockIdx.x == 0) atomic_or_err(p.err, bad);
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
@@ -588,7 +510,7 @@ __global__ void __launch_bounds__(NW * 32, CTAS) q4_attention_kernel(const Q4Par
     }
     int r = lo * chunk;
     uint32_t off = pos - prefix[lo], bad = 0;
-    Row row = row_of(p, r, &bad);
+    Row row = row_of<false>(p, r, &bad);
     uint32_t it = 0;  // pairs taken through the ring so far
     bool dead = false;
 
@@ -597,7 +519,7 @@ __global__ void __launch_bounds__(NW * 32, CTAS) q4_attention_kernel(const Q4Par
 #pragma unroll 1
       while (off >= len && r + 1 < p.num_rows) {
         off -= len;
-        row = row_of(p, ++r, &bad);
+        row = row_of<false>(p, ++r, &bad);
         len = pairs_of(p, row);
       }
       if (off >= len) break;  // rows that overlap, beyond what can be counted
@@ -831,6 +753,9 @@ struct Shape {
   static constexpr int kStages = D == 64 ? 4 : D == 128 ? 2 : 1;
 };
 
+// (token, query head of a group) pairs from which a row is a chunk.
+constexpr int kChunkFrom = 48;
+
 // Columns (in eights) of a warp's tile: enough for the group, and for more tokens where rows
 // have several and the registers hold them.
 int column_tiles(int group, int head_dim, int rows, int total_query) {
@@ -968,8 +893,11 @@ extern "C" int seb_paged_attention_q4(const void* q, int64_t q_stride_token, int
   p.lse = lse;
   p.lse_st = lse_stride_token;
   p.err = err;
+  p.chunk_from = head_dim <= 128 && total_query > num_rows ? kChunkFrom : 0;
   const int nt = column_tiles(group, head_dim, num_rows, total_query);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return dtype == SEB_BF16 ? launch_dim<__nv_bfloat16>(p, head_dim, nt, workspace, workspace_bytes, s)
-                           : launch_dim<__half>(p, head_dim, nt, workspace, workspace_bytes, s);
+  const int rc = dtype == SEB_BF16 ? launch_dim<__nv_bfloat16>(p, head_dim, nt, workspace, workspace_bytes, s)
+                                   : launch_dim<__half>(p, head_dim, nt, workspace, workspace_bytes, s);
+  if (rc != SEB_OK || p.chunk_from == 0) return rc;
+  return launch_q4_prefill(p, head_dim, dtype, s);
 }

@@ -1,0 +1,756 @@
+// Attention of prompt chunks over the 4-bit KV pool, on the 5th-generation tensor cores.
+//
+// A unit is one row, one kv head and a pair of query tiles; the 128 MMA rows of a tile pack
+// (token, query head of the group) pairs, row m = token m / group, head m % group. One CTA
+// per SM takes units in turn:
+//   warps 0-7   a warpgroup for each query tile, a thread for each row: brings its query to
+//               shared memory, then for every 128 keys reads its scores from TMEM, softmax
+//               with a lazily moved reference, writes P over them; at the end O / l and LSE;
+//   warps 8-11  read K and V codes of 8 blocks, turn them into fp16 and store them as the
+//               MMA's operands; the next 128 keys' codes are loaded meanwhile;
+//   warp 12     owns TMEM and issues S(t) = Q(t) K^T and O(t) += P(t) V, tile t's while the
+//               other tile's softmax runs.
+// K is stored by keys, V by dims (V^T): both K-major, and both as the pool has them, so a
+// word of 8 codes becomes one 16-byte store (V: of 4 pairs of tokens, 4 such stores).
+//
+// Rounding to 16 bits: a query to fp16 after a power of two of its own that puts its largest
+// element at 2^14 (exact, see q4_attention.cu; the power is part of the row's scale); K and
+// V values once to fp16 (unit 2^-11; clamped to +-65504), which is what a 16-bit pool would
+// hold; P to fp16, below 2^8. Scores, O and all sums are fp32. One rounding of K costs a
+// score about 2e-4 at unit scores, and LSE that over the root of the keys seen; units whose
+// first token sees few keys take K as the sum of two fp16 numbers, one product for each.
+//
+// Bound: the tensor pipe (4 * 128^2 * head_dim FLOPs for each tile and 128 keys) beside the
+// exponentials, 128 for each thread; the codes are 1 / 28 of the time's bytes.
+#include "q4_attention.cuh"
+#include "seb_softmax.cuh"
+#include "seb_tcgen05.cuh"
+
+#include <algorithm>
+#include <cfloat>
+#include <type_traits>
+
+namespace seb {
+namespace {
+
+constexpr int kKeys = 128;     // keys of a K / V tile
+constexpr int kRows = 128;     // rows of a query tile
+constexpr int kTiles = 2;      // query tiles of a unit
+constexpr int kStages = 2;     // K tiles, and V tiles, in shared memory
+constexpr int kThreads = 416;  // 2 softmax warpgroups, 4 warps that decode, the MMA warp
+constexpr int kTmemCols = 512;
+constexpr int kColO = 256;     // S of tile t at 128 t (P over its first 64 columns), O at 256 + t * D
+constexpr float kLazy = 8.f;   // scores may exceed the reference by 2^8 before it is moved
+constexpr int kSplitBelow = 512;  // keys seen by a unit's first token from which on K is rounded once
+// Of 16 pairs of scores, those whose exponentials run on the FMA pipe (poly_exp2x2) beside the MUFU's.
+constexpr unsigned kPolyPairs = 0x8888u;
+
+template <int D>
+struct Smem {
+  static constexpr int kPanel = 128 * 128;      // 128 rows of 128 bytes
+  static constexpr int kTile = D / 64 * kPanel;  // of Q, K or V^T
+  static constexpr int oQ = 0;
+  static constexpr int oK = oQ + kTiles * kTile;
+  static constexpr int oV = oK + kStages * kTile;
+  static constexpr int oBar = oV + kStages * kTile;
+  static constexpr int oMiss = oBar + 256;     // uint32 [4]: blocks of a tile without data
+  static constexpr int oPrefix = oMiss + 16;   // uint32 [kThreads + 1]
+  static constexpr int kBytes = oPrefix + (kThreads + 1) * 4;
+};
+
+enum {
+  kBarQFull = 0,                      // + tile: its 128 threads stored the unit's queries
+  kBarKFull = kBarQFull + kTiles,     // + stage
+  kBarKEmpty = kBarKFull + kStages,   // + stage: S of every tile has read K
+  kBarVFull = kBarKEmpty + kStages,   // + stage
+  kBarVEmpty = kBarVFull + kStages,   // + stage
+  kBarSFull = kBarVEmpty + kStages,   // + tile: S(t, j) complete, and every MMA before it
+  kBarPFull = kBarSFull + kTiles,     // + tile: P(t, j) stored
+  kBarODone = kBarPFull + kTiles,     // + tile: the unit's last PV complete
+  kBarFinal = kBarODone + kTiles,
+  kNumBars = kBarFinal + 1
+};
+static_assert(kNumBars * 8 + 8 <= 256, "barrier region");
+
+// A unit as every role sees it.
+struct Unit {
+  int row, kvh, k_len, q_len;
+  int64_t token;       // the first of the unit's tokens
+  int tok0;            // and its place in the row
+  int sees;            // keys that it sees; each later token sees one more (causal)
+  int nblk, ntiles;    // blocks that some token sees, and tiles of 128 keys
+  int tiles;           // query tiles, 1 or 2
+  bool split;          // K in two parts: a tile of keys takes two places of the ring
+};
+
+__device__ __forceinline__ uint32_t units_of(const Q4Params& p, const Row& w) {
+  return (uint32_t)((w.q_len + kTiles * p.tile - 1) / (kTiles * p.tile)) * p.hkv;
+}
+
+// Unit u of all rows' units end to end; false past the last.
+__device__ __forceinline__ bool find_unit(const Q4Params& p, const uint32_t* prefix, uint32_t u, Unit& w) {
+  if (u >= prefix[kThreads]) return false;
+  int lo = 0, hi = kThreads - 1;
+#pragma unroll 1
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (prefix[mid] <= u) lo = mid;
+    else hi = mid - 1;
+  }
+  const int chunk = (p.num_rows + kThreads - 1) / kThreads;
+  int r = lo * chunk;
+  uint32_t off = u - prefix[lo], bad = 0;
+  Row row = row_of<true>(p, r, &bad);
+  uint32_t len = units_of(p, row);
+#pragma unroll 1
+  while (off >= len && r + 1 < p.num_rows) {
+    off -= len;
+    row = row_of<true>(p, ++r, &bad);
+    len = units_of(p, row);
+  }
+  if (off >= len) return false;
+  const int pairs = len / p.hkv;
+  const int pr = pairs - 1 - off / p.hkv;  // a row's last tokens first: they see the most keys
+  w.row = r;
+  w.kvh = off % p.hkv;
+  w.k_len = row.k_len;
+  w.q_len = row.q_len;
+  w.tok0 = pr * kTiles * p.tile;
+  w.token = (int64_t)row.q_start + w.tok0;
+  w.sees = p.causal ? (int)min((int64_t)row.q_pos + w.tok0 + 1, (int64_t)(1 << 30)) : row.k_len;
+  const int toks = min(kTiles * p.tile, row.q_len - w.tok0);
+  w.tiles = toks > p.tile ? 2 : 1;
+  w.split = w.sees < kSplitBelow;
+  const int any = p.causal ? min(row.k_len, max(w.sees + toks - 1, 0)) : row.k_len;
+  w.nblk = (any + 15) >> 4;
+  w.ntiles = (w.nblk + 7) >> 3;
+  return true;
+}
+
+// Steps through a CTA's (unit, K / V tile) pairs.
+struct Walk {
+  Unit w;
+  uint32_t u;
+  int j;
+  // To the next tile, of this unit or of the next one that has any; first: to the first.
+  __device__ __forceinline__ bool next(const Q4Params& p, const uint32_t* prefix, bool first) {
+    if (!first && ++j < w.ntiles) return true;
+    u = first ? blockIdx.x : u + gridDim.x;
+    j = 0;
+#pragma unroll 1
+    for (; find_unit(p, prefix, u, w); u += gridDim.x)
+      if (w.ntiles > 0) return true;
+    return false;
+  }
+};
+
+// 8 codes of a word, two of each 16 bits (lowest first), times s plus l.
+template <bool CLAMP>
+__device__ __forceinline__ void decode8(uint32_t w, __half2 s, __half2 l, uint32_t (&v)[4]) {
+  const __half2 k1024 = __half2half2(__ushort_as_half(0x6400));
+  const __half2 k16th = __half2half2(__ushort_as_half(0x2c00)), k64 = __half2half2(__ushort_as_half(0xd400));
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    // 1024 + n and 1024 + 16 n
+    const uint32_t a = (w & 0x000f000fu) | 0x64006400u, b = (w & 0x00f000f0u) | 0x64006400u;
+    const __half2 na = __hsub2(*reinterpret_cast<const __half2*>(&a), k1024);
+    const __half2 nb = __hfma2(*reinterpret_cast<const __half2*>(&b), k16th, k64);
+    __half2 x = __hfma2(na, s, l), y = __hfma2(nb, s, l);
+    if constexpr (CLAMP) {
+      const __half2 top = __half2half2(__ushort_as_half(0x7bff));
+      x = __hmax2_nan(__hmin2_nan(x, top), __hneg2(top));
+      y = __hmax2_nan(__hmin2_nan(y, top), __hneg2(top));
+    }
+    v[2 * h] = *reinterpret_cast<const uint32_t*>(&x);
+    v[2 * h + 1] = *reinterpret_cast<const uint32_t*>(&y);
+    w >>= 8;
+  }
+}
+__device__ __forceinline__ __half2 as_half2(uint32_t x) { return *reinterpret_cast<const __half2*>(&x); }
+__device__ __forceinline__ bool is_nan_pair(uint32_t x) { return (x & 0x7fffu) > 0x7c00u; }  // the scale decides
+// Whether a group with this (scale, low), or the elementwise largest of several, may pass 65504.
+__device__ __forceinline__ bool may_overflow(__half2 most) {
+  return __hgt(__low2half(most), __ushort_as_half(0x6800)) || __hgt(__high2half(most), __ushort_as_half(0x7800));
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params p) {
+  using S = Smem<D>;
+  using L = q4::Layout<D>;
+  constexpr int G = L::kGroups;
+  static_assert(L::kPanels == 1, "head_dim 64 or 128");
+  extern __shared__ __align__(1024) char smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  char* sbase = smem_raw + (base - raw);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t bar = base + S::oBar;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sbase + S::oBar + 8 * kNumBars);
+  uint32_t* miss = reinterpret_cast<uint32_t*>(sbase + S::oMiss);
+  uint32_t* prefix = reinterpret_cast<uint32_t*>(sbase + S::oPrefix);
+
+  // ---- the rows' units; errors in rows are reported by the kernel for the other rows
+  {
+    const int chunk = (p.num_rows + kThreads - 1) / kThreads;
+    uint32_t sum = 0, bad = 0;
+#pragma unroll 1
+    for (int r = tid * chunk; r < min((tid + 1) * chunk, p.num_rows); ++r) sum += units_of(p, row_of<true>(p, r, &bad));
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const uint32_t o = __shfl_up_sync(kFull, sum, off);
+      if (lane >= off) sum += o;
+    }
+    prefix[tid + 1] = sum;
+    if (tid == 0) prefix[0] = 0;
+    __syncthreads();
+    uint32_t before = 0;
+#pragma unroll 1
+    for (int w = 0; w < warp; ++w) before += prefix[(w + 1) * 32];
+    __syncthreads();
+    prefix[tid + 1] += before;
+    if (tid < 4) miss[tid] = 0;
+  }
+  __syncthreads();
+  if (blockIdx.x >= prefix[kThreads]) return;
+
+  if (tid == 0) {
+    for (int t = 0; t < kTiles; ++t) {
+      mbar_init(bar + 8 * (kBarQFull + t), 128);
+      mbar_init(bar + 8 * (kBarSFull + t), 1);
+      mbar_init(bar + 8 * (kBarPFull + t), 4);
+      mbar_init(bar + 8 * (kBarODone + t), 1);
+    }
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(bar + 8 * (kBarKFull + s), 128);
+      mbar_init(bar + 8 * (kBarKEmpty + s), 1);
+      mbar_init(bar + 8 * (kBarVFull + s), 128);
+      mbar_init(bar + 8 * (kBarVEmpty + s), 1);
+    }
+    mbar_init(bar + 8 * kBarFinal, 1);
+    fence_mbar_init();
+  }
+  if (warp == 12) {
+    tc::tmem_alloc(smem_u32(tmem_slot), kTmemCols);
+    tc::tmem_relinquish();
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::fence_after_sync();
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
+  bool failed = false;
+
+  if (warp >= 8 && warp < 12) {
+    // ------------------------------------------------------------ K and V
+    const int th = tid - 256;
+    // K: for i < 4 token 32 i + th / 4 of the tile, chunk th % 4. V: half block vc (of 16) and dims 8 vg + ...
+    const int kt = th & 3, kr = th >> 2;
+    const int vc = (th & 7) + 8 * (th >> 6), vg = ((th >> 3) & 3) + 4 * ((th >> 5) & 1);
+    __align__(16) uint32_t kw[4][2 * G], kp[4][G], vw[4][2 * G], vp[8][G];
+    int limit_k = 0, limit_v = 0;  // keys of the loaded tile that exist
+    bool diag_k = false, diag_v = false;
+    unsigned miss_k = 0;
+    Walk at{};
+    int win = -1, wrow = -1;  // the block ids that the lanes hold: 32 from 32 win on of row wrow
+    int ids = -1;
+    auto block_ids = [&](const Walk& x) {  // ids of the 32 blocks that x's tile is among
+      if (win == (x.j >> 2) && wrow == x.w.row) return;
+      win = x.j >> 2;
+      wrow = x.w.row;
+      const int b = 32 * win + lane;
+      ids = -1;
+      if (b < x.w.nblk) {
+        ids = __ldg(p.block_table + (int64_t)x.w.row * p.bt_stride + b);
+        if (ids < 0 || ids >= p.num_blocks) {
+          atomic_or_err(p.err, SEB_ERRBIT_BLOCK_ID);
+          ids = -1;
+        }
+      }
+    };
+    // Tokens of the tile that some row does not see: there a NaN must not meet a weight of zero.
+    auto is_diag = [&](const Walk& x) { return (x.j + 1) * kKeys > min(x.w.sees, x.w.k_len); };
+    auto load_k = [&](const Walk& x) {
+      block_ids(x);
+      miss_k = ~(__ballot_sync(kFull, ids >= 0) >> ((x.j & 3) * 8)) & 0xffu;
+      limit_k = x.w.k_len - x.j * kKeys;
+      diag_k = is_diag(x);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int id = __shfl_sync(kFull, ids, (x.j & 3) * 8 + 2 * i + (th >> 6));
+#pragma unroll
+        for (int e = 0; e < 2 * G; ++e) kw[i][e] = 0;
+#pragma unroll
+        for (int e = 0; e < G; ++e) kp[i][e] = 0;
+        if (id >= 0) {
+          const char* row = p.k_cache + ((int64_t)id * p.hkv + x.w.kvh) * L::kRow;
+          const int r = kr & 15;
+          if constexpr (G == 2) {
+            *reinterpret_cast<uint4*>(kw[i]) = __ldg(reinterpret_cast<const uint4*>(row + r * 64 + kt * 16));
+            *reinterpret_cast<uint2*>(kp[i]) = __ldg(reinterpret_cast<const uint2*>(row + L::kCodes + r * 8));
+          } else {
+            *reinterpret_cast<uint2*>(kw[i]) = __ldg(reinterpret_cast<const uint2*>(row + r * 32 + kt * 8));
+            kp[i][0] = __ldg(reinterpret_cast<const uint32_t*>(row + L::kCodes + r * 4));
+          }
+          if (diag_k) {
+            const uint32_t* vq = reinterpret_cast<const uint32_t*>(p.v_cache + ((int64_t)id * p.hkv + x.w.kvh) * L::kRow +
+                                                                   L::kCodes + r * 4 * G);
+#pragma unroll
+            for (int e = 0; e < G; ++e)
+              if (is_nan_pair(__ldg(vq + e))) kp[i][0] = 0x7fff7fffu;  // whoever sees the token gets NaN
+          }
+        }
+      }
+    };
+    auto load_v = [&](const Walk& x) {
+      block_ids(x);
+      limit_v = x.w.k_len - x.j * kKeys;
+      diag_v = is_diag(x);
+      const int id = __shfl_sync(kFull, ids, (x.j & 3) * 8 + (vc >> 1));
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 2 * G; ++e) vw[i][e] = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int e = 0; e < G; ++e) vp[i][e] = 0;
+      if (id >= 0) {
+        const char* row = p.v_cache + ((int64_t)id * p.hkv + x.w.kvh) * L::kRow;
+        const int h = vc & 1;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const char* a = row + (4 * h + i) * L::kWidth + (vg ^ L::turn(4 * h + i)) * (8 * G);
+          if constexpr (G == 2) *reinterpret_cast<uint4*>(vw[i]) = __ldg(reinterpret_cast<const uint4*>(a));
+          else *reinterpret_cast<uint2*>(vw[i]) = __ldg(reinterpret_cast<const uint2*>(a));
+        }
+        const uint4* q = reinterpret_cast<const uint4*>(row + L::kCodes + h * 32 * G);
+#pragma unroll
+        for (int i = 0; i < 2 * G; ++i) *reinterpret_cast<uint4*>(&vp[0][0] + 4 * i) = __ldg(q + i);
+      }
+    };
+    // K(key, 16 dims of each group) -> two 16-byte chunks a group, 128-byte swizzled rows of 64 dims.
+    auto store_k = [&](char* tile, auto clamp) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = 32 * i + kr;
+#pragma unroll
+        for (int gi = 0; gi < G; ++gi) {
+          const __half2 pr = as_half2(kp[i][gi]);
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            uint32_t v[4];
+            decode8<decltype(clamp)::value>(kw[i][2 * gi + w], __low2half2(pr), __high2half2(pr), v);
+            *reinterpret_cast<uint4*>(tile + gi * S::kPanel + key * 128 + (((2 * kt + w) ^ (key & 7)) << 4)) =
+                make_uint4(v[0], v[1], v[2], v[3]);
+          }
+        }
+      }
+    };
+    // The same in two parts: one fp16 number, and the next for what it leaves.
+    auto store_k_split = [&](char* tile, bool rest) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = 32 * i + kr;
+#pragma unroll
+        for (int gi = 0; gi < G; ++gi) {
+          const float2 pr = __half22float2(as_half2(kp[i][gi]));
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            uint32_t v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              float x[2];
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const float y = fmaf((float)q4::k_code(kw[i][2 * gi + w], 2 * e + h), pr.x, pr.y);
+                const float top = q4::max_nan(q4::min_nan(y, 65504.f), -65504.f);
+                x[h] = rest ? top - __half2float(__float2half_rn(top)) : top;
+              }
+              v[e] = Mma<__half>::pack(x[0], x[1]);
+            }
+            *reinterpret_cast<uint4*>(tile + gi * S::kPanel + key * 128 + (((2 * kt + w) ^ (key & 7)) << 4)) =
+                make_uint4(v[0], v[1], v[2], v[3]);
+          }
+        }
+      }
+    };
+    // V of 8 tokens, 8 dims of each group -> one 16-byte chunk a dim, rows of 64 keys.
+    auto store_v = [&](char* tile, auto clamp) {
+#pragma unroll
+      for (int gi = 0; gi < G; ++gi) {
+        __half2 s[4], l[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const __half2 a = as_half2(vp[2 * i][gi]), b = as_half2(vp[2 * i + 1][gi]);
+          s[i] = __lows2half2(a, b);
+          l[i] = __highs2half2(a, b);
+        }
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          uint32_t v[4][4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) decode8<decltype(clamp)::value>(vw[i][2 * gi + w], s[i], l[i], v[i]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int dim = gi * 64 + vg * 8 + 4 * w + e;
+            *reinterpret_cast<uint4*>(tile + (vc >> 3) * (D * 128) + dim * 128 + (((vc & 7) ^ (dim & 7)) << 4)) =
+                make_uint4(v[0][e], v[1][e], v[2][e], v[3][e]);
+          }
+        }
+      }
+    };
+
+    // the ring's next place for K
+    int gk = 0;
+    auto k_place = [&]() -> char* {
+      const int s = gk % kStages;
+      if (gk >= kStages && !wait_or_flag(bar + 8 * (kBarKEmpty + s), (gk / kStages - 1) & 1, failed)) return nullptr;
+      return sbase + S::oK + s * S::kTile;
+    };
+    auto k_stored = [&]() {
+      fence_proxy_async_smem();
+      mbar_arrive(bar + 8 * (kBarKFull + gk % kStages));
+      ++gk;
+    };
+    bool have = at.next(p, prefix, true);
+    if (have) {
+      load_k(at);
+      load_v(at);
+    }
+#pragma unroll 1
+    for (int n = 0; have; ++n) {
+      const int s = n % kStages;
+      const bool split = at.w.split;
+      have = at.next(p, prefix, false);
+      char* tile = k_place();
+      if (!tile) break;
+      if (th == 0) miss[n & 3] = miss_k;
+      __half2 most = as_half2(0);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < G; ++e) {
+          if (32 * i + kr >= limit_k) kp[i][e] = 0;  // past the row's keys
+          most = __hmax2(most, __habs2(as_half2(kp[i][e])));
+        }
+      if (split) {
+#pragma unroll 1
+        for (int part = 0; part < 2 && tile; ++part) {
+          store_k_split(tile, part == 1);
+          k_stored();
+          if (part == 0) tile = k_place();
+        }
+        if (!tile) break;
+      } else {
+        if (__any_sync(kFull, may_overflow(most))) store_k(tile, std::true_type{});
+        else store_k(tile, std::false_type{});
+        k_stored();
+      }
+      if (have) load_k(at);
+      if (n >= kStages && !wait_or_flag(bar + 8 * (kBarVEmpty + s), (n / kStages - 1) & 1, failed)) break;
+      most = as_half2(0);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int e = 0; e < G; ++e) {
+          if (8 * vc + i >= limit_v || (diag_v && is_nan_pair(vp[i][e]))) vp[i][e] = 0;
+          most = __hmax2(most, __habs2(as_half2(vp[i][e])));
+        }
+      tile = sbase + S::oV + s * S::kTile;
+      if (__any_sync(kFull, may_overflow(most))) store_v(tile, std::true_type{});
+      else store_v(tile, std::false_type{});
+      fence_proxy_async_smem();
+      mbar_arrive(bar + 8 * (kBarVFull + s));
+      if (have) load_v(at);
+    }
+  } else if (warp == 12) {
+    // ---------------------------------------------------------------- MMA
+    constexpr uint32_t idesc_qk = tc::idesc_f16(false, false, kRows, kKeys);
+    constexpr uint32_t idesc_pv = tc::idesc_f16(false, false, kRows, D);
+    // S(t) from the K places g and, where K is in two parts, g + 1.
+    auto issue_s = [&](int t, int g, int parts) {
+      if (lane == 0) {
+#pragma unroll 1
+        for (int part = 0; part < parts; ++part)
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t off = (kk >> 2) * S::kPanel + (kk & 3) * 32;
+            tc::mma_ss(tmem + t * 128, tc::smem_desc_sw128(base + S::oQ + t * S::kTile + off, 16, 1024),
+                       tc::smem_desc_sw128(base + S::oK + (g + part) % kStages * S::kTile + off, 16, 1024), idesc_qk,
+                       part > 0 || kk > 0);
+          }
+        tc::commit(bar + 8 * (kBarSFull + t));
+      }
+      __syncwarp();
+    };
+    auto wait_k = [&](int g, int parts) {
+      for (int part = 0; part < parts; ++part)
+        if (!wait_or_flag(bar + 8 * (kBarKFull + (g + part) % kStages), ((g + part) / kStages) & 1, failed)) return false;
+      return true;
+    };
+    auto release_k = [&](int g, int parts) {
+      if (lane == 0)
+        for (int part = 0; part < parts; ++part) tc::commit(bar + 8 * (kBarKEmpty + (g + part) % kStages));
+    };
+    auto issue_pv = [&](int t, int s, bool first) {
+      if (lane == 0) {
+#pragma unroll
+        for (int kk = 0; kk < kKeys / 16; ++kk)
+          tc::mma_ts(tmem + kColO + t * D, tmem + t * 128 + 8 * kk,
+                     tc::smem_desc_sw128(base + S::oV + s * S::kTile + (kk >> 2) * (D * 128) + (kk & 3) * 32, 16, 1024),
+                     idesc_pv, !first || kk > 0);
+      }
+      __syncwarp();
+    };
+    // For each K / V tile j and query tile t: PV(t, j), then S(t, j + 1) over the columns that it
+    // read P from; one thread issues both, and its MMAs run in order.
+    int gk = 0, gv = 0, nu = 0;
+    uint32_t pphase = 0;
+    Unit w;
+#pragma unroll 1
+    for (uint32_t u = blockIdx.x; !failed && find_unit(p, prefix, u, w); u += gridDim.x) {
+      if (w.ntiles == 0) continue;
+      const int parts = w.split ? 2 : 1;
+      {
+        if (!wait_k(gk, parts)) break;
+        for (int t = 0; t < w.tiles && !failed; ++t) {
+          if (!wait_or_flag(bar + 8 * (kBarQFull + t), (nu >> t) & 1, failed)) break;
+          nu ^= 1 << t;
+          tc::fence_after_sync();
+          issue_s(t, gk, parts);
+        }
+        release_k(gk, parts);
+        __syncwarp();
+        gk += parts;
+      }
+#pragma unroll 1
+      for (int j = 0; j < w.ntiles && !failed; ++j) {
+        const int sv = gv % kStages;
+        if (!wait_or_flag(bar + 8 * (kBarVFull + sv), (gv / kStages) & 1, failed)) break;
+        const bool more = j + 1 < w.ntiles;
+        for (int t = 0; t < w.tiles && !failed; ++t) {
+          if (!wait_or_flag(bar + 8 * (kBarPFull + t), (pphase >> t) & 1, failed)) break;
+          pphase ^= 1u << t;
+          tc::fence_after_sync();
+          issue_pv(t, sv, j == 0);
+          if (!more) {
+            if (lane == 0) tc::commit(bar + 8 * (kBarODone + t));
+            __syncwarp();
+            continue;
+          }
+          if (t == 0 && !wait_k(gk, parts)) break;
+          tc::fence_after_sync();
+          issue_s(t, gk, parts);
+        }
+        if (lane == 0) tc::commit(bar + 8 * (kBarVEmpty + sv));
+        if (more) {
+          release_k(gk, parts);
+          gk += parts;
+        }
+        __syncwarp();
+        ++gv;
+      }
+    }
+    if (lane == 0) tc::commit(bar + 8 * kBarFinal);  // every MMA is complete before TMEM is released
+    __syncwarp();
+    mbar_wait_bounded(bar + 8 * kBarFinal, 0, 1u << 20);
+  } else {
+    // ------------------------------------------------------------ softmax
+    const int qt = warp >> 2;
+    const int m = (warp & 3) * 32 + lane;
+    const uint32_t taddr = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t col_s = qt * 128, col_o = kColO + qt * D;
+    const int tk = m / p.group, gh = m - tk * p.group;
+    int ns = 0, nd = 0;  // tiles of scores and units done, of this query tile
+    int nt = 0;          // K tiles of all units (the ring's count)
+    Unit w;
+#pragma unroll 1
+    for (uint32_t u = blockIdx.x; find_unit(p, prefix, u, w); u += gridDim.x) {
+      const int first_tile = nt;
+      nt += w.ntiles;
+      if (qt >= w.tiles) continue;
+      const int tok = qt * p.tile + tk;  // of the unit
+      const bool live = tk < p.tile && w.tok0 + tok < w.q_len;
+      const int head = w.kvh * p.group + gh;
+      T* op = reinterpret_cast<T*>(p.out) + (w.token + tok) * p.o_st + (int64_t)head * p.o_sh;
+      float* lp = p.lse + (w.token + tok) * p.lse_st + head;
+      if (w.ntiles == 0) {
+        if (live) {
+          for (int d = 0; d < D / 8; ++d) reinterpret_cast<uint4*>(op)[d] = make_uint4(0u, 0u, 0u, 0u);
+          *lp = -INFINITY;
+        }
+        continue;
+      }
+      // ---- the row's query, as fp16 after a power of two
+      float c;
+      {
+        using T2 = typename Two<T>::type;
+        __align__(16) T2 q[D / 2];
+        T2 most = Two<T>::zero();
+        const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.q) + (w.token + tok) * p.q_st +
+                                                          (int64_t)head * p.q_sh);
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i)
+          *reinterpret_cast<uint4*>(&q[4 * i]) = live ? __ldg(src + i) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+        for (int i = 0; i < D / 2; ++i) most = __hmax2_nan(most, __habs2(q[i]));
+        const float top = q4::max_nan(Elem<T>::to_float(low_of(most)), Elem<T>::to_float(high_of(most)));
+        const int ex = query_exponent(top);
+        const float down = power2(-ex);
+        c = copysignf(fminf(fabsf(p.scale_log2) * power2(ex), FLT_MAX), p.scale_log2);
+        char* row = sbase + S::oQ + qt * S::kTile + m * 128;
+#pragma unroll
+        for (int i = 0; i < D / 8; ++i) {
+          uint32_t v[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            v[e] = Mma<__half>::pack(Elem<T>::to_float(low_of(q[4 * i + e])) * down,
+                                     Elem<T>::to_float(high_of(q[4 * i + e])) * down);
+          *reinterpret_cast<uint4*>(row + (i >> 3) * S::kPanel + (((i & 7) ^ (m & 7)) << 4)) =
+              make_uint4(v[0], v[1], v[2], v[3]);
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(bar + 8 * (kBarQFull + qt));
+      }
+      const int vis = !live ? 0 : p.causal ? min(w.k_len, w.sees + tok) : w.k_len;
+      const int all_see = p.causal ? min(w.k_len, w.sees + qt * p.tile) : w.k_len;  // every row of the tile
+      float m_ref = -INFINITY, l = 0.f;
+#pragma unroll 1
+      for (int j = 0; j < w.ntiles; ++j, ++ns) {
+        wait_or_flag(bar + 8 * (kBarSFull + qt), ns & 1, failed);  // and PV(t, j - 1): O is stable
+        tc::fence_after_sync();
+        const unsigned none = miss[(first_tile + j) & 3];
+        const unsigned holes = none & ((1u << min(8, w.nblk - 8 * j)) - 1);
+        const bool plain = c > 0.f && (j + 1) * kKeys <= all_see && holes == 0;
+        const int lim = vis - j * kKeys;
+        auto mask = [&](float (&x)[32], int ch) {  // and into log2 units
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const bool seen = 32 * ch + i < lim && !((holes >> (2 * ch + (i >> 4))) & 1);
+            x[i] = seen ? x[i] * c : -INFINITY;
+          }
+        };
+        const float cm = plain ? c : 1.f;
+        float top = -INFINITY;
+#pragma unroll
+        for (int ch = 0; ch < 4; ++ch) {
+          float x[32];
+          tc::tmem_ld32(taddr + col_s + 32 * ch, x);
+          tc::tmem_wait_ld();
+          if (!plain) mask(x, ch);
+          float a = x[0], b = x[1];
+#pragma unroll
+          for (int i = 2; i < 30; i += 4) {
+            a = fmax3(a, x[i], x[i + 1]);
+            b = fmax3(b, x[i + 2], x[i + 3]);
+          }
+          top = fmax3(top, fmaxf(a, x[30]), fmaxf(b, x[31]));
+        }
+        top *= cm;
+        const bool move = top > m_ref + kLazy;
+        float factor = 1.f;
+        if (move) {
+          factor = fast_exp2(m_ref - top);
+          l *= factor;
+          m_ref = top;
+        }
+        const float neg = m_ref == -INFINITY ? 0.f : -m_ref;
+        // scores so large that a product's rounding matters: rounded as in the reference
+        const bool large = plain && fabsf(m_ref) > 1e6f;
+        const float cx = large ? 1.f : cm;
+        float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int ch = 0; ch < 4; ++ch) {
+          float x[32];
+          tc::tmem_ld32(taddr + col_s + 32 * ch, x);
+          tc::tmem_wait_ld();
+          if (!plain) mask(x, ch);
+          if (large) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) x[i] = __fmul_rn(x[i], c);
+          }
+          uint32_t hi[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const float2 d = fma2(make_float2(x[2 * e], x[2 * e + 1]), splat2(cx), splat2(neg));
+            float2 pr;
+            if (plain && ((kPolyPairs >> e) & 1)) pr = poly_exp2x2(d);
+            else pr = make_float2(fast_exp2(d.x), fast_exp2(d.y));
+            sum = add2(sum, pr);
+            hi[e] = Mma<__half>::pack(pr.x, pr.y);
+          }
+          tc::tmem_st16u(taddr + col_s + 16 * ch, hi);
+        }
+        l += sum.x + sum.y;
+        if (j > 0 && __any_sync(kFull, move)) {
+#pragma unroll 1
+          for (int cc = 0; cc < D / 16; ++cc) {
+            float o[16];
+            tc::tmem_ld16(taddr + col_o + 16 * cc, o);
+            tc::tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] *= factor;
+            tc::tmem_st16(taddr + col_o + 16 * cc, o);
+          }
+        }
+        tc::tmem_wait_st();
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar + 8 * (kBarPFull + qt));
+      }
+      // ---- O is final
+      wait_or_flag(bar + 8 * (kBarODone + qt), nd & 1, failed);
+      ++nd;
+      tc::fence_after_sync();
+      if (__any_sync(kFull, failed)) break;
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll 1
+      for (int cc = 0; cc < D / 32; ++cc) {
+        float o[32];
+        tc::tmem_ld32(taddr + col_o + 32 * cc, o);
+        tc::tmem_wait_ld();
+        if (live) {
+#pragma unroll
+          for (int v8 = 0; v8 < 4; ++v8) {
+            uint32_t v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = Mma<T>::pack(o[8 * v8 + 2 * e] * inv, o[8 * v8 + 2 * e + 1] * inv);
+            reinterpret_cast<uint4*>(op)[4 * cc + v8] = make_uint4(v[0], v[1], v[2], v[3]);
+          }
+        }
+      }
+      if (live) *lp = l == 0.f ? -INFINITY : fmaf(m_ref, kLn2, logf(l));
+      tc::fence_before_sync();  // the next unit's first PV overwrites O
+    }
+  }
+
+  if (failed && lane == 0) atomic_or_err(p.err, SEB_ERRBIT_TIMEOUT);
+  tc::fence_before_sync();
+  __syncthreads();
+  if (warp == 12) {
+    tc::fence_after_sync();
+    tc::tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+template <typename T, int D>
+int launch(Q4Params p, cudaStream_t s) {
+  constexpr auto kern = q4_prefill_kernel<T, D>;
+  constexpr int smem = Smem<D>::kBytes + 1024;
+  const int rc = set_smem_limit_once<kern>(smem);
+  if (rc != SEB_OK) return rc;
+  p.tile = kRows / p.group;
+  // no more CTAs than the tokens' units: at most one for each row and kv head beyond the full ones
+  const int64_t units = ((int64_t)p.total_query / (kTiles * p.tile) + p.num_rows) * p.hkv;
+  kern<<<(unsigned)std::min<int64_t>(num_sms(), units), kThreads, smem, s>>>(p);
+  return launch_status("q4_prefill_kernel");
+}
+
+}  // namespace
+
+int launch_q4_prefill(const Q4Params& p, int head_dim, int dtype, cudaStream_t s) {
+  if (dtype == SEB_BF16)
+    return head_dim == 64 ? launch<__nv_bfloat16, 64>(p, s) : launch<__nv_bfloat16, 128>(p, s);
+  return head_dim == 64 ? launch<__half, 64>(p, s) : launch<__half, 128>(p, s);
+}
+
+}  // namespace seb

@@ -258,7 +258,7 @@ def paged_attention_q4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
         1 if is_causal else 0, out.data_ptr(), out.stride(0), out.stride(1), lse.data_ptr(), lse.stride(0),
         ws.data_ptr(), ws.numel(), slot, err_word(dev).data_ptr(), stream)
     check("seb_paged_attention_q4", st)
-    LAUNCHES[0] += 1
+    LAUNCHES[0] += 2 if total_q > rows and d <= 128 else 1  # rows of many tokens have their own kernel
     _after(dev)
     if result is not out:
         result.copy_(out)

@@ -509,3 +509,75 @@ def test_empty_batches():
     z = torch.zeros(1, **i32)
     o, lse = b200.paged_attention_q4(q, pool[0], pool[1], torch.empty(1, 0, **i32), z, z + 1, z, z - 1, 2, 1, 1.0)
     assert (o == 0).all() and torch.isneginf(lse).all()
+
+
+# ------------------------------------------------------------------- prompt chunks
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d,hq,hkv", [(128, 8, 2), (64, 8, 2), (128, 7, 1), (64, 3, 3), (128, 16, 1)])
+@pytest.mark.parametrize("q_lens,k_lens", [
+    ([128], [128]), ([129, 200], [129, 1000]), ([65, 1, 0, 300, 4], [65, 700, 0, 317, 90]), ([257], [600])])
+def test_chunks(dtype, d, hq, hkv, q_lens, k_lens):
+    """Rows long enough for the tcgen05 kernel, beside rows that are not; tiles that end inside a block."""
+    b = make_batch(k_lens, q_lens, hq, hkv, d, dtype, seed=d + hq)
+    o, lse = b200.paged_flash_attention(b["q"], b["pool"][0], b["pool"][1], metadata(b), hq, hkv, b["scale"])
+    b200.check_device_errors()
+    check(b, o, lse)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+def test_chunks_with_odd_positions(causal):
+    """A chunk whose position is not k_len - q_len: tokens that see nothing, and tokens that see all keys."""
+    b = make_batch([150, 40], [140, 60], 4, 2, 128, torch.float16, seed=21)
+    b["pos"] = [-30, 20]
+    o, lse = b200.paged_flash_attention(b["q"], b["pool"][0], b["pool"][1], metadata(b), 4, 2, b["scale"], is_causal=causal)
+    b200.check_device_errors()
+    check(b, o, lse, causal=causal)
+
+
+def test_chunks_negative_scale_and_bad_blocks():
+    b = make_batch([400, 300], [100, 90], 4, 1, 64, torch.bfloat16, seed=22)
+    b["scale"] = -0.2
+    b["table"][0, 3], b["table"][1, 9] = -1, 10 ** 6
+    o, lse = b200.paged_flash_attention(b["q"], b["pool"][0], b["pool"][1], metadata(b), 4, 1, b["scale"])
+    with pytest.raises(RuntimeError, match="block id out of range"):
+        b200.check_device_errors()
+    check(b, o, lse)
+
+
+def test_chunk_nan_token_is_not_seen_before_it():
+    """A token whose K and V are NaN: the chunk's earlier tokens do not see it, its later ones do."""
+    b = make_batch([200], [150], 4, 2, 128, torch.bfloat16, seed=23)
+    at = 120  # key of the chunk's token 70
+    slot = int(b["table"][0, at // 16]) * 16 + at % 16
+    x = torch.full((1, 2, 128), float("nan"), device=DEV).bfloat16()
+    b200.kv_append_q4(x, x, b["pool"][0], b["pool"][1], torch.tensor([slot], device=DEV))
+    o, lse = b200.paged_flash_attention(b["q"], b["pool"][0], b["pool"][1], metadata(b), 4, 2, b["scale"])
+    assert torch.isnan(o[70:]).all()
+    check(b, o, lse, tokens=list(range(70)))
+
+
+@pytest.mark.parametrize("size", [1e30, 1e-30])
+def test_chunk_queries_beyond_fp16(size):
+    b = make_batch([150], [100], 2, 1, 64, torch.bfloat16, seed=24)
+    b["q"] = (b["q"].float() * size).bfloat16()
+    o, lse = b200.paged_flash_attention(b["q"], b["pool"][0], b["pool"][1], metadata(b), 2, 1, b["scale"])
+    assert torch.isfinite(o).all() and torch.isfinite(lse).all()
+    if size < 1:  # all scores are next to nothing: the mean of the values seen
+        check(b, o, lse)
+
+
+def test_chunk_values_beyond_fp16():
+    """Values between 65504 and what a group's codes can reach are clamped to 65504 for a chunk."""
+    n, d = 160, 128
+    b = make_batch([n], [n], 1, 1, d, torch.bfloat16, seed=25)
+    g = torch.Generator(device=DEV).manual_seed(1)
+    v = torch.randn(n, 1, d, generator=g, device=DEV)
+    v[:, 0, 3] = 90000.0
+    v[:, 0, 70] = -60000.0
+    slots = torch.tensor([int(b["table"][0, j // 16]) * 16 + j % 16 for j in range(n)], device=DEV)
+    k, _ = b200.kv_gather_q4(b["pool"][0], b["pool"][1], slots, d, torch.float32)
+    b200.kv_append_q4(k.bfloat16(), v.bfloat16(), b["pool"][0], b["pool"][1], slots)
+    o, lse = b200.paged_flash_attention(b["q"], b["pool"][0], b["pool"][1], metadata(b), 1, 1, b["scale"])
+    assert torch.isfinite(o).all()
+    assert ((o[:, 0, 3].float() - 65504).abs() <= 65504 * 2.0 ** -8).all()
+    assert ((o[:, 0, 70].float() + 60000).abs() <= 60000 * 2.0 ** -7).all()
