@@ -6,12 +6,17 @@
 //   warps 0-7   a warpgroup for each query tile, a thread for each row: brings its query to
 //               shared memory, then for every 128 keys reads its scores from TMEM, softmax
 //               with a lazily moved reference, writes P over them; at the end O / l and LSE;
-//   warps 8-11  read K and V codes of 8 blocks, turn them into fp16 and store them as the
-//               MMA's operands; the next 128 keys' codes are loaded meanwhile;
+//   warps 8-11  turn the codes of 8 blocks into fp16 and store them as the MMA's operands;
 //   warp 12     owns TMEM and issues S(t) = Q(t) K^T and O(t) += P(t) V, tile t's while the
-//               other tile's softmax runs.
+//               other tile's softmax runs;
+//   warp 13     copies the pool's rows of the next blocks to shared memory.
 // K is stored by keys, V by dims (V^T): both K-major, and both as the pool has them, so a
 // word of 8 codes becomes one 16-byte store (V: of 4 pairs of tokens, 4 such stores).
+// Registers are split between the roles (setmaxnreg); none may spill, with shared memory
+// taking what would be L1.
+//
+// In a tile key 16 b + r of block b has place 16 b + (r ^ 4) where r >= 8: V's rows in shared
+// memory are then read in an order that meets no bank twice.
 //
 // Rounding to 16 bits: a query to fp16 after a power of two of its own that puts its largest
 // element at 2^14 (exact, see q4_attention.cu; the power is part of the row's scale); K and
@@ -37,7 +42,8 @@ constexpr int kKeys = 128;     // keys of a K / V tile
 constexpr int kRows = 128;     // rows of a query tile
 constexpr int kTiles = 2;      // query tiles of a unit
 constexpr int kStages = 2;     // K tiles, and V tiles, in shared memory
-constexpr int kThreads = 416;  // 2 softmax warpgroups, 4 warps that decode, the MMA warp
+constexpr int kRawStages = 3;  // the pool's rows of K(0), V(0), K(1), ... before they are decoded
+constexpr int kThreads = 512;  // 2 softmax warpgroups, 4 warps that decode, the MMA warp, the copying one and 2 that idle
 constexpr int kTmemCols = 512;
 constexpr int kColO = 256;     // S of tile t at 128 t (P over its first 64 columns), O at 256 + t * D
 constexpr float kLazy = 8.f;   // scores may exceed the reference by 2^8 before it is moved
@@ -52,9 +58,12 @@ struct Smem {
   static constexpr int oQ = 0;
   static constexpr int oK = oQ + kTiles * kTile;
   static constexpr int oV = oK + kStages * kTile;
-  static constexpr int oBar = oV + kStages * kTile;
-  static constexpr int oMiss = oBar + 256;     // uint32 [4]: blocks of a tile without data
-  static constexpr int oPrefix = oMiss + 16;   // uint32 [kThreads + 1]
+  static constexpr int kRawRow = q4::Layout<D>::kRow + 16;  // 16 more: blocks start in different banks
+  static constexpr int kRaw = 8 * kRawRow;                  // K or V rows of a tile's 8 blocks
+  static constexpr int oRaw = oV + kStages * kTile;
+  static constexpr int oBar = oRaw + kRawStages * kRaw;
+  static constexpr int oInfo = oBar + 256;                  // TileInfo [4]
+  static constexpr int oPrefix = oInfo + 4 * 16;            // uint32 [kThreads + 1]
   static constexpr int kBytes = oPrefix + (kThreads + 1) * 4;
 };
 
@@ -67,7 +76,9 @@ enum {
   kBarSFull = kBarVEmpty + kStages,   // + tile: S(t, j) complete, and every MMA before it
   kBarPFull = kBarSFull + kTiles,     // + tile: P(t, j) stored
   kBarODone = kBarPFull + kTiles,     // + tile: the unit's last PV complete
-  kBarFinal = kBarODone + kTiles,
+  kBarRawFull = kBarODone + kTiles,   // + stage: rows have come
+  kBarRawEmpty = kBarRawFull + kRawStages,  // + stage: the 128 threads that decode have read them
+  kBarFinal = kBarRawEmpty + kRawStages,
   kNumBars = kBarFinal + 1
 };
 static_assert(kNumBars * 8 + 8 <= 256, "barrier region");
@@ -82,6 +93,17 @@ struct Unit {
   int tiles;           // query tiles, 1 or 2
   bool split;          // K in two parts: a tile of keys takes two places of the ring
 };
+
+// What the copying warp says of a tile of keys.
+struct TileInfo {
+  int limit;      // its keys below this exist
+  unsigned none;  // bit b: block b has no data
+  int kind;       // kSplit, kDiag, or kEnd: no more tiles
+  int pad;
+};
+constexpr int kSplit = 1;  // K in two parts
+constexpr int kDiag = 2;   // some token does not see all of it: there a NaN must not meet a weight of zero
+constexpr int kEnd = 4;
 
 __device__ __forceinline__ uint32_t units_of(const Q4Params& p, const Row& w) {
   return (uint32_t)((w.q_len + kTiles * p.tile - 1) / (kTiles * p.tile)) * p.hkv;
@@ -127,23 +149,6 @@ __device__ __forceinline__ bool find_unit(const Q4Params& p, const uint32_t* pre
   return true;
 }
 
-// Steps through a CTA's (unit, K / V tile) pairs.
-struct Walk {
-  Unit w;
-  uint32_t u;
-  int j;
-  // To the next tile, of this unit or of the next one that has any; first: to the first.
-  __device__ __forceinline__ bool next(const Q4Params& p, const uint32_t* prefix, bool first) {
-    if (!first && ++j < w.ntiles) return true;
-    u = first ? blockIdx.x : u + gridDim.x;
-    j = 0;
-#pragma unroll 1
-    for (; find_unit(p, prefix, u, w); u += gridDim.x)
-      if (w.ntiles > 0) return true;
-    return false;
-  }
-};
-
 // 8 codes of a word, two of each 16 bits (lowest first), times s plus l.
 template <bool CLAMP>
 __device__ __forceinline__ void decode8(uint32_t w, __half2 s, __half2 l, uint32_t (&v)[4]) {
@@ -173,6 +178,26 @@ __device__ __forceinline__ bool may_overflow(__half2 most) {
   return __hgt(__low2half(most), __ushort_as_half(0x6800)) || __hgt(__high2half(most), __ushort_as_half(0x7800));
 }
 
+// Registers of the warpgroup's threads, from 128 at the launch.
+template <int N>
+__device__ __forceinline__ void registers_up() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void registers_down() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+// True in one lane of a converged warp, the same one each time.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t yes;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(yes));
+  return yes != 0;
+}
+static_assert(256 * 120 + 128 * 152 + 128 * 120 <= kThreads * 128, "the roles' registers are those of the launch");
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params p) {
   using S = Smem<D>;
@@ -186,7 +211,7 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t bar = base + S::oBar;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sbase + S::oBar + 8 * kNumBars);
-  uint32_t* miss = reinterpret_cast<uint32_t*>(sbase + S::oMiss);
+  TileInfo* info = reinterpret_cast<TileInfo*>(sbase + S::oInfo);
   uint32_t* prefix = reinterpret_cast<uint32_t*>(sbase + S::oPrefix);
 
   // ---- the rows' units; errors in rows are reported by the kernel for the other rows
@@ -208,7 +233,6 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
     for (int w = 0; w < warp; ++w) before += prefix[(w + 1) * 32];
     __syncthreads();
     prefix[tid + 1] += before;
-    if (tid < 4) miss[tid] = 0;
   }
   __syncthreads();
   if (blockIdx.x >= prefix[kThreads]) return;
@@ -226,6 +250,10 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
       mbar_init(bar + 8 * (kBarVFull + s), 128);
       mbar_init(bar + 8 * (kBarVEmpty + s), 1);
     }
+    for (int s = 0; s < kRawStages; ++s) {
+      mbar_init(bar + 8 * (kBarRawFull + s), 1);
+      mbar_init(bar + 8 * (kBarRawEmpty + s), 128);
+    }
     mbar_init(bar + 8 * kBarFinal, 1);
     fence_mbar_init();
   }
@@ -241,166 +269,12 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
 
   if (warp >= 8 && warp < 12) {
     // ------------------------------------------------------------ K and V
+    registers_up<152>();
     const int th = tid - 256;
     // K: for i < 4 token 32 i + th / 4 of the tile, chunk th % 4. V: half block vc (of 16) and dims 8 vg + ...
     const int kt = th & 3, kr = th >> 2;
     const int vc = (th & 7) + 8 * (th >> 6), vg = ((th >> 3) & 3) + 4 * ((th >> 5) & 1);
-    __align__(16) uint32_t kw[4][2 * G], kp[4][G], vw[4][2 * G], vp[8][G];
-    int limit_k = 0, limit_v = 0;  // keys of the loaded tile that exist
-    bool diag_k = false, diag_v = false;
-    unsigned miss_k = 0;
-    Walk at{};
-    int win = -1, wrow = -1;  // the block ids that the lanes hold: 32 from 32 win on of row wrow
-    int ids = -1;
-    auto block_ids = [&](const Walk& x) {  // ids of the 32 blocks that x's tile is among
-      if (win == (x.j >> 2) && wrow == x.w.row) return;
-      win = x.j >> 2;
-      wrow = x.w.row;
-      const int b = 32 * win + lane;
-      ids = -1;
-      if (b < x.w.nblk) {
-        ids = __ldg(p.block_table + (int64_t)x.w.row * p.bt_stride + b);
-        if (ids < 0 || ids >= p.num_blocks) {
-          atomic_or_err(p.err, SEB_ERRBIT_BLOCK_ID);
-          ids = -1;
-        }
-      }
-    };
-    // Tokens of the tile that some row does not see: there a NaN must not meet a weight of zero.
-    auto is_diag = [&](const Walk& x) { return (x.j + 1) * kKeys > min(x.w.sees, x.w.k_len); };
-    auto load_k = [&](const Walk& x) {
-      block_ids(x);
-      miss_k = ~(__ballot_sync(kFull, ids >= 0) >> ((x.j & 3) * 8)) & 0xffu;
-      limit_k = x.w.k_len - x.j * kKeys;
-      diag_k = is_diag(x);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int id = __shfl_sync(kFull, ids, (x.j & 3) * 8 + 2 * i + (th >> 6));
-#pragma unroll
-        for (int e = 0; e < 2 * G; ++e) kw[i][e] = 0;
-#pragma unroll
-        for (int e = 0; e < G; ++e) kp[i][e] = 0;
-        if (id >= 0) {
-          const char* row = p.k_cache + ((int64_t)id * p.hkv + x.w.kvh) * L::kRow;
-          const int r = kr & 15;
-          if constexpr (G == 2) {
-            *reinterpret_cast<uint4*>(kw[i]) = __ldg(reinterpret_cast<const uint4*>(row + r * 64 + kt * 16));
-            *reinterpret_cast<uint2*>(kp[i]) = __ldg(reinterpret_cast<const uint2*>(row + L::kCodes + r * 8));
-          } else {
-            *reinterpret_cast<uint2*>(kw[i]) = __ldg(reinterpret_cast<const uint2*>(row + r * 32 + kt * 8));
-            kp[i][0] = __ldg(reinterpret_cast<const uint32_t*>(row + L::kCodes + r * 4));
-          }
-          if (diag_k) {
-            const uint32_t* vq = reinterpret_cast<const uint32_t*>(p.v_cache + ((int64_t)id * p.hkv + x.w.kvh) * L::kRow +
-                                                                   L::kCodes + r * 4 * G);
-#pragma unroll
-            for (int e = 0; e < G; ++e)
-              if (is_nan_pair(__ldg(vq + e))) kp[i][0] = 0x7fff7fffu;  // whoever sees the token gets NaN
-          }
-        }
-      }
-    };
-    auto load_v = [&](const Walk& x) {
-      block_ids(x);
-      limit_v = x.w.k_len - x.j * kKeys;
-      diag_v = is_diag(x);
-      const int id = __shfl_sync(kFull, ids, (x.j & 3) * 8 + (vc >> 1));
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int e = 0; e < 2 * G; ++e) vw[i][e] = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-#pragma unroll
-        for (int e = 0; e < G; ++e) vp[i][e] = 0;
-      if (id >= 0) {
-        const char* row = p.v_cache + ((int64_t)id * p.hkv + x.w.kvh) * L::kRow;
-        const int h = vc & 1;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const char* a = row + (4 * h + i) * L::kWidth + (vg ^ L::turn(4 * h + i)) * (8 * G);
-          if constexpr (G == 2) *reinterpret_cast<uint4*>(vw[i]) = __ldg(reinterpret_cast<const uint4*>(a));
-          else *reinterpret_cast<uint2*>(vw[i]) = __ldg(reinterpret_cast<const uint2*>(a));
-        }
-        const uint4* q = reinterpret_cast<const uint4*>(row + L::kCodes + h * 32 * G);
-#pragma unroll
-        for (int i = 0; i < 2 * G; ++i) *reinterpret_cast<uint4*>(&vp[0][0] + 4 * i) = __ldg(q + i);
-      }
-    };
-    // K(key, 16 dims of each group) -> two 16-byte chunks a group, 128-byte swizzled rows of 64 dims.
-    auto store_k = [&](char* tile, auto clamp) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int key = 32 * i + kr;
-#pragma unroll
-        for (int gi = 0; gi < G; ++gi) {
-          const __half2 pr = as_half2(kp[i][gi]);
-#pragma unroll
-          for (int w = 0; w < 2; ++w) {
-            uint32_t v[4];
-            decode8<decltype(clamp)::value>(kw[i][2 * gi + w], __low2half2(pr), __high2half2(pr), v);
-            *reinterpret_cast<uint4*>(tile + gi * S::kPanel + key * 128 + (((2 * kt + w) ^ (key & 7)) << 4)) =
-                make_uint4(v[0], v[1], v[2], v[3]);
-          }
-        }
-      }
-    };
-    // The same in two parts: one fp16 number, and the next for what it leaves.
-    auto store_k_split = [&](char* tile, bool rest) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int key = 32 * i + kr;
-#pragma unroll
-        for (int gi = 0; gi < G; ++gi) {
-          const float2 pr = __half22float2(as_half2(kp[i][gi]));
-#pragma unroll
-          for (int w = 0; w < 2; ++w) {
-            uint32_t v[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              float x[2];
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const float y = fmaf((float)q4::k_code(kw[i][2 * gi + w], 2 * e + h), pr.x, pr.y);
-                const float top = q4::max_nan(q4::min_nan(y, 65504.f), -65504.f);
-                x[h] = rest ? top - __half2float(__float2half_rn(top)) : top;
-              }
-              v[e] = Mma<__half>::pack(x[0], x[1]);
-            }
-            *reinterpret_cast<uint4*>(tile + gi * S::kPanel + key * 128 + (((2 * kt + w) ^ (key & 7)) << 4)) =
-                make_uint4(v[0], v[1], v[2], v[3]);
-          }
-        }
-      }
-    };
-    // V of 8 tokens, 8 dims of each group -> one 16-byte chunk a dim, rows of 64 keys.
-    auto store_v = [&](char* tile, auto clamp) {
-#pragma unroll
-      for (int gi = 0; gi < G; ++gi) {
-        __half2 s[4], l[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const __half2 a = as_half2(vp[2 * i][gi]), b = as_half2(vp[2 * i + 1][gi]);
-          s[i] = __lows2half2(a, b);
-          l[i] = __highs2half2(a, b);
-        }
-#pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          uint32_t v[4][4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) decode8<decltype(clamp)::value>(vw[i][2 * gi + w], s[i], l[i], v[i]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int dim = gi * 64 + vg * 8 + 4 * w + e;
-            *reinterpret_cast<uint4*>(tile + (vc >> 3) * (D * 128) + dim * 128 + (((vc & 7) ^ (dim & 7)) << 4)) =
-                make_uint4(v[0][e], v[1][e], v[2][e], v[3][e]);
-          }
-        }
-      }
-    };
-
-    // the ring's next place for K
-    int gk = 0;
+    int gk = 0;  // places of the K ring filled
     auto k_place = [&]() -> char* {
       const int s = gk % kStages;
       if (gk >= kStages && !wait_or_flag(bar + 8 * (kBarKEmpty + s), (gk / kStages - 1) & 1, failed)) return nullptr;
@@ -411,73 +285,268 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
       mbar_arrive(bar + 8 * (kBarKFull + gk % kStages));
       ++gk;
     };
-    bool have = at.next(p, prefix, true);
-    if (have) {
-      load_k(at);
-      load_v(at);
+    auto raw_full = [&](int i) {
+      return wait_or_flag(bar + 8 * (kBarRawFull + i % kRawStages), (i / kRawStages) & 1, failed);
+    };
+    // where this thread's chunk w of K's row i and its dims' rows of V go, but for the stage
+    int k_at[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int key = 32 * i + kr, at = key ^ ((key >> 1) & 4);
+      k_at[i] = at * 128 + (((2 * kt) ^ (at & 7)) << 4);  // chunk 2 kt; the other one is 16 bytes on or back
     }
+    const int v_at = (vc >> 3) * (D * 128) + vg * 1024 + ((vc & 7) << 4);
+
 #pragma unroll 1
-    for (int n = 0; have; ++n) {
+    for (int n = 0;; ++n) {
       const int s = n % kStages;
-      const bool split = at.w.split;
-      have = at.next(p, prefix, false);
-      char* tile = k_place();
-      if (!tile) break;
-      if (th == 0) miss[n & 3] = miss_k;
-      __half2 most = as_half2(0);
+      const int ik = 2 * n, iv = 2 * n + 1;  // K's and V's places in the run of rows
+      if (!raw_full(ik)) break;
+      const TileInfo ti = info[n & 3];
+      if (ti.kind & kEnd) break;
+      const bool diag = ti.kind & kDiag;
+      if (diag && !raw_full(iv)) break;
+      const bool ragged = ti.limit < kKeys || ti.none != 0;
+      // ---- K(key, 16 dims of each group): two 16-byte chunks a group, 128-byte swizzled rows of 64 dims
+      {
+        const char* raw_k = sbase + S::oRaw + ik % kRawStages * S::kRaw + (th >> 6) * S::kRawRow;
+        __align__(16) uint32_t kw[4][2 * G], kp[4][G];
+        __half2 most = as_half2(0);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 4; ++i) {
+          const char* row = raw_k + 2 * i * S::kRawRow;
+          const char* words = row + (kr & 15) * (L::kWidth / 2) + kt * (8 * G);
+          const char* pairs = row + L::kCodes + (kr & 15) * 4 * G;
+          if constexpr (G == 2) {
+            *reinterpret_cast<uint4*>(kw[i]) = *reinterpret_cast<const uint4*>(words);
+            *reinterpret_cast<uint2*>(kp[i]) = *reinterpret_cast<const uint2*>(pairs);
+          } else {
+            *reinterpret_cast<uint2*>(kw[i]) = *reinterpret_cast<const uint2*>(words);
+            kp[i][0] = *reinterpret_cast<const uint32_t*>(pairs);
+          }
+        }
+        if (diag) {  // whoever sees a token whose V is NaN gets NaN, by way of its score
 #pragma unroll
-        for (int e = 0; e < G; ++e) {
-          if (32 * i + kr >= limit_k) kp[i][e] = 0;  // past the row's keys
-          most = __hmax2(most, __habs2(as_half2(kp[i][e])));
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t* vq = reinterpret_cast<const uint32_t*>(sbase + S::oRaw + iv % kRawStages * S::kRaw +
+                                                                   (2 * i + (th >> 6)) * S::kRawRow + L::kCodes +
+                                                                   (kr & 15) * 4 * G);
+#pragma unroll
+            for (int e = 0; e < G; ++e)
+              if (is_nan_pair(vq[e])) kp[i][0] = 0x7fff7fffu;
+          }
         }
-      if (split) {
-#pragma unroll 1
-        for (int part = 0; part < 2 && tile; ++part) {
-          store_k_split(tile, part == 1);
-          k_stored();
-          if (part == 0) tile = k_place();
+        mbar_arrive(bar + 8 * (kBarRawEmpty + ik % kRawStages));
+        if (ragged) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (32 * i + kr >= ti.limit || ((ti.none >> (2 * i + (th >> 6))) & 1)) {
+#pragma unroll
+              for (int e = 0; e < G; ++e) kp[i][e] = 0;
+            }
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int e = 0; e < G; ++e) most = __hmax2(most, __habs2(as_half2(kp[i][e])));
+        const bool clamp = __any_sync(kFull, may_overflow(most));
+        char* tile = k_place();
         if (!tile) break;
-      } else {
-        if (__any_sync(kFull, may_overflow(most))) store_k(tile, std::true_type{});
-        else store_k(tile, std::false_type{});
-        k_stored();
-      }
-      if (have) load_k(at);
-      if (n >= kStages && !wait_or_flag(bar + 8 * (kBarVEmpty + s), (n / kStages - 1) & 1, failed)) break;
-      most = as_half2(0);
+        auto store = [&](int i, int gi, int w, const uint32_t (&v)[4]) {
+          *reinterpret_cast<uint4*>(tile + gi * S::kPanel + (k_at[i] ^ (w << 4))) = make_uint4(v[0], v[1], v[2], v[3]);
+        };
+        if (ti.kind & kSplit) {
+          // as two fp16 numbers: K rounded, then what that leaves
+#pragma unroll 1
+          for (int part = 0; part < 2 && tile; ++part) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
+            for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int e = 0; e < G; ++e) {
-          if (8 * vc + i >= limit_v || (diag_v && is_nan_pair(vp[i][e]))) vp[i][e] = 0;
-          most = __hmax2(most, __habs2(as_half2(vp[i][e])));
+              for (int gi = 0; gi < G; ++gi)
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                  const float2 pr = __half22float2(as_half2(kp[i][gi]));
+                  uint32_t v[4];
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) {
+                    float x[2];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                      const float y = fmaf((float)q4::k_code(kw[i][2 * gi + w], 2 * e + h), pr.x, pr.y);
+                      const float top = q4::max_nan(q4::min_nan(y, 65504.f), -65504.f);
+                      x[h] = part ? top - __half2float(__float2half_rn(top)) : top;
+                    }
+                    v[e] = Mma<__half>::pack(x[0], x[1]);
+                  }
+                  store(i, gi, w, v);
+                }
+            k_stored();
+            if (part == 0) tile = k_place();
+          }
+          if (!tile) break;
+        } else {
+          auto all = [&](auto limited) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+              for (int gi = 0; gi < G; ++gi) {
+                const __half2 pr = as_half2(kp[i][gi]);
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                  uint32_t v[4];
+                  decode8<decltype(limited)::value>(kw[i][2 * gi + w], __low2half2(pr), __high2half2(pr), v);
+                  store(i, gi, w, v);
+                }
+              }
+          };
+          if (clamp) all(std::true_type{});
+          else all(std::false_type{});
+          k_stored();
         }
-      tile = sbase + S::oV + s * S::kTile;
-      if (__any_sync(kFull, may_overflow(most))) store_v(tile, std::true_type{});
-      else store_v(tile, std::false_type{});
-      fence_proxy_async_smem();
-      mbar_arrive(bar + 8 * (kBarVFull + s));
-      if (have) load_v(at);
+      }
+      // ---- V of 8 tokens, 8 dims of each group: one 16-byte chunk a dim, rows of 64 keys. The tokens are in
+      // the places' order: of a block's second half the last four come first.
+      if (!raw_full(iv)) break;
+      {
+        const int h = vc & 1;
+        const char* raw_v = sbase + S::oRaw + iv % kRawStages * S::kRaw + (vc >> 1) * S::kRawRow;
+        __align__(16) uint32_t vw[4][2 * G], vp[8][G];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int pair = (4 * h + i) ^ (2 * h);
+          const char* src = raw_v + pair * L::kWidth + (vg ^ L::turn(pair)) * (8 * G);
+          if constexpr (G == 2) *reinterpret_cast<uint4*>(vw[i]) = *reinterpret_cast<const uint4*>(src);
+          else *reinterpret_cast<uint2*>(vw[i]) = *reinterpret_cast<const uint2*>(src);
+        }
+        const uint4* pairs = reinterpret_cast<const uint4*>(raw_v + L::kCodes + h * 32 * G);
+#pragma unroll
+        for (int i = 0; i < 2 * G; ++i) *reinterpret_cast<uint4*>(&vp[0][0] + 4 * i) = pairs[i ^ (h * G)];
+        mbar_arrive(bar + 8 * (kBarRawEmpty + iv % kRawStages));
+        if (ragged || diag) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const bool gone = 8 * vc + (i ^ (4 * h)) >= ti.limit || ((ti.none >> (vc >> 1)) & 1);
+#pragma unroll
+            for (int e = 0; e < G; ++e)
+              if (gone || (diag && is_nan_pair(vp[i][e]))) vp[i][e] = 0;
+          }
+        }
+        __half2 most = as_half2(0);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+          for (int e = 0; e < G; ++e) most = __hmax2(most, __habs2(as_half2(vp[i][e])));
+        const bool clamp = __any_sync(kFull, may_overflow(most));
+        if (n >= kStages && !wait_or_flag(bar + 8 * (kBarVEmpty + s), (n / kStages - 1) & 1, failed)) break;
+        char* tile = sbase + S::oV + s * S::kTile;
+        auto all = [&](auto limited) {
+#pragma unroll
+          for (int gi = 0; gi < G; ++gi) {
+            __half2 sc[4], lo[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const __half2 a = as_half2(vp[2 * i][gi]), b = as_half2(vp[2 * i + 1][gi]);
+              sc[i] = __lows2half2(a, b);
+              lo[i] = __highs2half2(a, b);
+            }
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+              uint32_t v[4][4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) decode8<decltype(limited)::value>(vw[i][2 * gi + w], sc[i], lo[i], v[i]);
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                *reinterpret_cast<uint4*>(tile + gi * 8192 + (4 * w + e) * 128 + (v_at ^ ((4 * w + e) << 4))) =
+                    make_uint4(v[0][e], v[1][e], v[2][e], v[3][e]);
+            }
+          }
+        };
+        if (clamp) all(std::true_type{});
+        else all(std::false_type{});
+        fence_proxy_async_smem();
+        mbar_arrive(bar + 8 * (kBarVFull + s));
+      }
     }
-  } else if (warp == 12) {
+  } else if (warp >= 12) {
+    registers_down<120>();
+    if (warp > 13) goto done;
+    if (warp == 13) {
+      // -------------------------------------------------------------- copies
+      int i = 0, n = 0;  // rows of K and V asked for, and tiles
+      Unit w;
+#pragma unroll 1
+      for (uint32_t u = blockIdx.x; !failed && find_unit(p, prefix, u, w); u += gridDim.x) {
+        const int32_t* table = p.block_table + (int64_t)w.row * p.bt_stride;
+        auto fetch = [&](int b) -> int {
+          if (b >= w.nblk) return -1;
+          const int id = __ldg(table + b);
+          if (id >= 0 && id < p.num_blocks) return id;
+          atomic_or_err(p.err, SEB_ERRBIT_BLOCK_ID);
+          return -1;
+        };
+        int ids = fetch(lane), next = fetch(32 + lane);  // of 32 blocks, and of the 32 after them
+#pragma unroll 1
+        for (int j = 0; j < w.ntiles && !failed; ++j, ++n) {
+          if (j > 0 && (j & 3) == 0) {
+            ids = next;
+            next = fetch(8 * j + 32 + lane);
+          }
+          const int id = __shfl_sync(kFull, ids, (j & 3) * 8 + (lane & 7));
+          const unsigned have = __ballot_sync(kFull, id >= 0) & 0xffu;
+#pragma unroll 1
+          for (int is_v = 0; is_v < 2; ++is_v, ++i) {
+            const int s = i % kRawStages;
+            if (i >= kRawStages && !wait_or_flag(bar + 8 * (kBarRawEmpty + s), (i / kRawStages - 1) & 1, failed)) break;
+            if (lane == 0) {
+              if (!is_v)
+                info[n & 3] = TileInfo{w.k_len - j * kKeys, ~have & 0xffu,
+                                       (w.split ? kSplit : 0) |
+                                           ((j + 1) * kKeys > min(w.sees, w.k_len) ? kDiag : 0), 0};
+              mbar_arrive_expect_tx(bar + 8 * (kBarRawFull + s), __popc(have) * L::kRow);
+            }
+            __syncwarp();
+            if (lane < 8 && id >= 0)
+              bulk_g2s(base + S::oRaw + s * S::kRaw + lane * S::kRawRow,
+                       (is_v ? p.v_cache : p.k_cache) + ((int64_t)id * p.hkv + w.kvh) * L::kRow, L::kRow,
+                       bar + 8 * (kBarRawFull + s));
+          }
+        }
+      }
+      const int s = i % kRawStages;
+      if (!failed && (i < kRawStages || wait_or_flag(bar + 8 * (kBarRawEmpty + s), (i / kRawStages - 1) & 1, failed))) {
+        if (lane == 0) {
+          info[n & 3].kind = kEnd;
+          mbar_arrive(bar + 8 * (kBarRawFull + s));
+        }
+      } else {  // whoever would have waited for the copies has given up: leave none in flight
+        for (int k = max(0, i - kRawStages); k < i; ++k)
+          mbar_wait_bounded(bar + 8 * (kBarRawFull + k % kRawStages), (k / kRawStages) & 1, 1u << 16);
+      }
+      goto done;
+    }
     // ---------------------------------------------------------------- MMA
     constexpr uint32_t idesc_qk = tc::idesc_f16(false, false, kRows, kKeys);
     constexpr uint32_t idesc_pv = tc::idesc_f16(false, false, kRows, D);
+    // Descriptors of the first tile of each operand; others are so many 16-byte units on.
+    const uint64_t desc_q = tc::smem_desc_sw128(base + S::oQ, 16, 1024);
+    const uint64_t desc_k = tc::smem_desc_sw128(base + S::oK, 16, 1024);
+    const uint64_t desc_v = tc::smem_desc_sw128(base + S::oV, 16, 1024);
     // S(t) from the K places g and, where K is in two parts, g + 1.
     auto issue_s = [&](int t, int g, int parts) {
-      if (lane == 0) {
-#pragma unroll 1
-        for (int part = 0; part < parts; ++part)
+      if (elect_one()) {
+        const uint64_t dq = desc_q + t * (S::kTile >> 4);
+        uint64_t dk = desc_k + g % kStages * (S::kTile >> 4);
 #pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t off = (kk >> 2) * S::kPanel + (kk & 3) * 32;
-            tc::mma_ss(tmem + t * 128, tc::smem_desc_sw128(base + S::oQ + t * S::kTile + off, 16, 1024),
-                       tc::smem_desc_sw128(base + S::oK + (g + part) % kStages * S::kTile + off, 16, 1024), idesc_qk,
-                       part > 0 || kk > 0);
-          }
+        for (int kk = 0; kk < D / 16; ++kk)
+          tc::mma_ss(tmem + t * 128, dq + (((kk >> 2) * S::kPanel + (kk & 3) * 32) >> 4),
+                     dk + (((kk >> 2) * S::kPanel + (kk & 3) * 32) >> 4), idesc_qk, kk > 0);
+        if (parts == 2) {
+          dk = desc_k + (g + 1) % kStages * (S::kTile >> 4);
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk)
+            tc::mma_ss(tmem + t * 128, dq + (((kk >> 2) * S::kPanel + (kk & 3) * 32) >> 4),
+                       dk + (((kk >> 2) * S::kPanel + (kk & 3) * 32) >> 4), idesc_qk, true);
+        }
         tc::commit(bar + 8 * (kBarSFull + t));
       }
       __syncwarp();
@@ -488,16 +557,16 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
       return true;
     };
     auto release_k = [&](int g, int parts) {
-      if (lane == 0)
+      if (elect_one())
         for (int part = 0; part < parts; ++part) tc::commit(bar + 8 * (kBarKEmpty + (g + part) % kStages));
     };
     auto issue_pv = [&](int t, int s, bool first) {
-      if (lane == 0) {
+      if (elect_one()) {
+        const uint64_t dv = desc_v + s * (S::kTile >> 4);
 #pragma unroll
         for (int kk = 0; kk < kKeys / 16; ++kk)
           tc::mma_ts(tmem + kColO + t * D, tmem + t * 128 + 8 * kk,
-                     tc::smem_desc_sw128(base + S::oV + s * S::kTile + (kk >> 2) * (D * 128) + (kk & 3) * 32, 16, 1024),
-                     idesc_pv, !first || kk > 0);
+                     dv + (((kk >> 2) * (D * 128) + (kk & 3) * 32) >> 4), idesc_pv, !first || kk > 0);
       }
       __syncwarp();
     };
@@ -533,7 +602,7 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
           tc::fence_after_sync();
           issue_pv(t, sv, j == 0);
           if (!more) {
-            if (lane == 0) tc::commit(bar + 8 * (kBarODone + t));
+            if (elect_one()) tc::commit(bar + 8 * (kBarODone + t));
             __syncwarp();
             continue;
           }
@@ -541,7 +610,7 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
           tc::fence_after_sync();
           issue_s(t, gk, parts);
         }
-        if (lane == 0) tc::commit(bar + 8 * (kBarVEmpty + sv));
+        if (elect_one()) tc::commit(bar + 8 * (kBarVEmpty + sv));
         if (more) {
           release_k(gk, parts);
           gk += parts;
@@ -550,11 +619,12 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
         ++gv;
       }
     }
-    if (lane == 0) tc::commit(bar + 8 * kBarFinal);  // every MMA is complete before TMEM is released
+    if (elect_one()) tc::commit(bar + 8 * kBarFinal);  // every MMA is complete before TMEM is released
     __syncwarp();
     mbar_wait_bounded(bar + 8 * kBarFinal, 0, 1u << 20);
   } else {
     // ------------------------------------------------------------ softmax
+    registers_down<120>();
     const int qt = warp >> 2;
     const int m = (warp & 3) * 32 + lane;
     const uint32_t taddr = tmem + ((uint32_t)((warp & 3) * 32) << 16);
@@ -618,32 +688,48 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
       for (int j = 0; j < w.ntiles; ++j, ++ns) {
         wait_or_flag(bar + 8 * (kBarSFull + qt), ns & 1, failed);  // and PV(t, j - 1): O is stable
         tc::fence_after_sync();
-        const unsigned none = miss[(first_tile + j) & 3];
-        const unsigned holes = none & ((1u << min(8, w.nblk - 8 * j)) - 1);
+        const unsigned holes = info[(first_tile + j) & 3].none & ((1u << min(8, w.nblk - 8 * j)) - 1);
         const bool plain = c > 0.f && (j + 1) * kKeys <= all_see && holes == 0;
         const int lim = vis - j * kKeys;
+        const float cm = plain ? c : 1.f;
+        // The row's scores, 32 at a time, twice: for their maximum, and for P; the next 32 are on
+        // their way meanwhile. Held all at once they would not fit beside what else a thread has.
+        float xa[32], xb[32];
+        auto fetch = [&](float (&x)[32], int ch) { tc::tmem_ld32(taddr + col_s + 32 * (ch & 3), x); };
         auto mask = [&](float (&x)[32], int ch) {  // and into log2 units
+          const int rest = lim - 32 * ch;
+          const unsigned h0 = (holes >> (2 * ch)) & 1, h1 = (holes >> (2 * ch + 1)) & 1;
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
-            const bool seen = 32 * ch + i < lim && !((holes >> (2 * ch + (i >> 4))) & 1);
+            const bool seen = (i ^ ((i >> 1) & 4)) < rest && !(i < 16 ? h0 : h1);
             x[i] = seen ? x[i] * c : -INFINITY;
           }
         };
-        const float cm = plain ? c : 1.f;
         float top = -INFINITY;
-#pragma unroll
-        for (int ch = 0; ch < 4; ++ch) {
-          float x[32];
-          tc::tmem_ld32(taddr + col_s + 32 * ch, x);
-          tc::tmem_wait_ld();
+        auto take_max = [&](float (&x)[32], int ch) {
           if (!plain) mask(x, ch);
-          float a = x[0], b = x[1];
+          float m0 = x[0], m1 = x[1], m2 = x[2], m3 = x[3];
 #pragma unroll
-          for (int i = 2; i < 30; i += 4) {
-            a = fmax3(a, x[i], x[i + 1]);
-            b = fmax3(b, x[i + 2], x[i + 3]);
+          for (int i = 4; i < 28; i += 8) {
+            m0 = fmax3(m0, x[i], x[i + 1]);
+            m1 = fmax3(m1, x[i + 2], x[i + 3]);
+            m2 = fmax3(m2, x[i + 4], x[i + 5]);
+            m3 = fmax3(m3, x[i + 6], x[i + 7]);
           }
-          top = fmax3(top, fmaxf(a, x[30]), fmaxf(b, x[31]));
+          m0 = fmax3(m0, x[28], x[29]);
+          m1 = fmax3(m1, x[30], x[31]);
+          top = fmax3(top, fmaxf(m0, m1), fmaxf(m2, m3));
+        };
+        fetch(xa, 0);
+        tc::tmem_wait_ld();
+#pragma unroll 1
+        for (int ch = 0; ch < 4; ch += 2) {
+          fetch(xb, ch + 1);
+          take_max(xa, ch);
+          tc::tmem_wait_ld();
+          fetch(xa, ch + 2);
+          take_max(xb, ch + 1);
+          tc::tmem_wait_ld();
         }
         top *= cm;
         const bool move = top > m_ref + kLazy;
@@ -657,12 +743,8 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
         // scores so large that a product's rounding matters: rounded as in the reference
         const bool large = plain && fabsf(m_ref) > 1e6f;
         const float cx = large ? 1.f : cm;
-        float2 sum = make_float2(0.f, 0.f);
-#pragma unroll
-        for (int ch = 0; ch < 4; ++ch) {
-          float x[32];
-          tc::tmem_ld32(taddr + col_s + 32 * ch, x);
-          tc::tmem_wait_ld();
+        float2 sum0 = make_float2(0.f, 0.f), sum1 = sum0;
+        auto take_p = [&](float (&x)[32], int ch) {
           if (!plain) mask(x, ch);
           if (large) {
 #pragma unroll
@@ -672,15 +754,25 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             const float2 d = fma2(make_float2(x[2 * e], x[2 * e + 1]), splat2(cx), splat2(neg));
-            float2 pr;
-            if (plain && ((kPolyPairs >> e) & 1)) pr = poly_exp2x2(d);
-            else pr = make_float2(fast_exp2(d.x), fast_exp2(d.y));
-            sum = add2(sum, pr);
+            // (a masked score weighs 2^-126 on the FMA pipe, and 0 as fp16)
+            const float2 pr = (kPolyPairs >> e) & 1 ? poly_exp2x2(d) : make_float2(fast_exp2(d.x), fast_exp2(d.y));
+            if (e & 1) sum1 = add2(sum1, pr);
+            else sum0 = add2(sum0, pr);
             hi[e] = Mma<__half>::pack(pr.x, pr.y);
           }
           tc::tmem_st16u(taddr + col_s + 16 * ch, hi);
+        };
+#pragma unroll 1
+        for (int ch = 0; ch < 4; ch += 2) {  // P of 32 keys covers 16 columns, of scores that were read
+          fetch(xb, ch + 1);
+          take_p(xa, ch);
+          tc::tmem_wait_ld();
+          if (ch == 0) fetch(xa, 2);
+          take_p(xb, ch + 1);
+          tc::tmem_wait_ld();
         }
-        l += sum.x + sum.y;
+        sum0 = add2(sum0, sum1);
+        l += sum0.x + sum0.y;
         if (j > 0 && __any_sync(kFull, move)) {
 #pragma unroll 1
           for (int cc = 0; cc < D / 16; ++cc) {
@@ -723,6 +815,7 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
     }
   }
 
+done:
   if (failed && lane == 0) atomic_or_err(p.err, SEB_ERRBIT_TIMEOUT);
   tc::fence_before_sync();
   __syncthreads();
