@@ -6,10 +6,11 @@
 //   warps 0-7   a warpgroup for each query tile, a thread for each row: brings its query to
 //               shared memory, then for every 128 keys reads its scores from TMEM, softmax
 //               with a lazily moved reference, writes P over them; at the end O / l and LSE;
-//   warps 8-11  turn the codes of 8 blocks into fp16 and store them as the MMA's operands;
-//   warp 12     owns TMEM and issues S(t) = Q(t) K^T and O(t) += P(t) V, tile t's while the
+//   warps 8-11  turn K's codes of 8 blocks into fp16 and store them as the MMA's operand,
+//   warps 12-15 V's;
+//   warp 16     owns TMEM and issues S(t) = Q(t) K^T and O(t) += P(t) V, tile t's while the
 //               other tile's softmax runs;
-//   warp 13     copies the pool's rows of the next blocks to shared memory.
+//   warp 17     copies the pool's rows of the next blocks to shared memory.
 // K is stored by keys, V by dims (V^T): both K-major, and both as the pool has them, so a
 // word of 8 codes becomes one 16-byte store (V: of 4 pairs of tokens, 4 such stores).
 // Registers are split between the roles (setmaxnreg); none may spill, with shared memory
@@ -43,13 +44,11 @@ constexpr int kRows = 128;     // rows of a query tile
 constexpr int kTiles = 2;      // query tiles of a unit
 constexpr int kStages = 2;     // K tiles, and V tiles, in shared memory
 constexpr int kRawStages = 3;  // the pool's rows of K(0), V(0), K(1), ... before they are decoded
-constexpr int kThreads = 512;  // 2 softmax warpgroups, 4 warps that decode, the MMA warp, the copying one and 2 that idle
+constexpr int kThreads = 640;  // 5 warpgroups; the last has the MMA warp, the copying one and 2 that idle
 constexpr int kTmemCols = 512;
 constexpr int kColO = 256;     // S of tile t at 128 t (P over its first 64 columns), O at 256 + t * D
 constexpr float kLazy = 8.f;   // scores may exceed the reference by 2^8 before it is moved
 constexpr int kSplitBelow = 512;  // keys seen by a unit's first token from which on K is rounded once
-// Of 16 pairs of scores, those whose exponentials run on the FMA pipe (poly_exp2x2) beside the MUFU's.
-constexpr unsigned kPolyPairs = 0x8888u;
 
 template <int D>
 struct Smem {
@@ -77,7 +76,7 @@ enum {
   kBarPFull = kBarSFull + kTiles,     // + tile: P(t, j) stored
   kBarODone = kBarPFull + kTiles,     // + tile: the unit's last PV complete
   kBarRawFull = kBarODone + kTiles,   // + stage: rows have come
-  kBarRawEmpty = kBarRawFull + kRawStages,  // + stage: the 128 threads that decode have read them
+  kBarRawEmpty = kBarRawFull + kRawStages,  // + stage: the 256 threads that decode are done with them
   kBarFinal = kBarRawEmpty + kRawStages,
   kNumBars = kBarFinal + 1
 };
@@ -178,7 +177,7 @@ __device__ __forceinline__ bool may_overflow(__half2 most) {
   return __hgt(__low2half(most), __ushort_as_half(0x6800)) || __hgt(__high2half(most), __ushort_as_half(0x7800));
 }
 
-// Registers of the warpgroup's threads, from 128 at the launch.
+// Registers of the warpgroup's threads.
 template <int N>
 __device__ __forceinline__ void registers_up() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
@@ -197,7 +196,9 @@ __device__ __forceinline__ bool elect_one() {
       : "=r"(yes));
   return yes != 0;
 }
-static_assert(256 * 120 + 128 * 152 + 128 * 120 <= kThreads * 128, "the roles' registers are those of the launch");
+// of the 96 that a thread has at the launch
+constexpr int kRegsSoftmax = 136, kRegsK = 64, kRegsV = 80, kRegsMma = 64;
+static_assert(2 * kRegsSoftmax + kRegsK + kRegsV + kRegsMma <= 5 * 96, "the roles' registers are those of the launch");
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params p) {
   using S = Smem<D>;
@@ -252,12 +253,12 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
     }
     for (int s = 0; s < kRawStages; ++s) {
       mbar_init(bar + 8 * (kBarRawFull + s), 1);
-      mbar_init(bar + 8 * (kBarRawEmpty + s), 128);
+      mbar_init(bar + 8 * (kBarRawEmpty + s), 256);
     }
     mbar_init(bar + 8 * kBarFinal, 1);
     fence_mbar_init();
   }
-  if (warp == 12) {
+  if (warp == 16) {
     tc::tmem_alloc(smem_u32(tmem_slot), kTmemCols);
     tc::tmem_relinquish();
   }
@@ -267,13 +268,14 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
   bool failed = false;
 
+  auto raw_full = [&](int i) {
+    return wait_or_flag(bar + 8 * (kBarRawFull + i % kRawStages), (i / kRawStages) & 1, failed);
+  };
   if (warp >= 8 && warp < 12) {
-    // ------------------------------------------------------------ K and V
-    registers_up<152>();
+    // ------------------------------------------------------------ K
+    registers_down<kRegsK>();
     const int th = tid - 256;
-    // K: for i < 4 token 32 i + th / 4 of the tile, chunk th % 4. V: half block vc (of 16) and dims 8 vg + ...
-    const int kt = th & 3, kr = th >> 2;
-    const int vc = (th & 7) + 8 * (th >> 6), vg = ((th >> 3) & 3) + 4 * ((th >> 5) & 1);
+    const int kt = th & 3, kr = th >> 2;  // for i < 4 token 32 i + kr of the tile, chunk kt of its dims
     int gk = 0;  // places of the K ring filled
     auto k_place = [&]() -> char* {
       const int s = gk % kStages;
@@ -285,192 +287,176 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
       mbar_arrive(bar + 8 * (kBarKFull + gk % kStages));
       ++gk;
     };
-    auto raw_full = [&](int i) {
-      return wait_or_flag(bar + 8 * (kBarRawFull + i % kRawStages), (i / kRawStages) & 1, failed);
-    };
-    // where this thread's chunk w of K's row i and its dims' rows of V go, but for the stage
-    int k_at[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int key = 32 * i + kr, at = key ^ ((key >> 1) & 4);
-      k_at[i] = at * 128 + (((2 * kt) ^ (at & 7)) << 4);  // chunk 2 kt; the other one is 16 bytes on or back
-    }
-    const int v_at = (vc >> 3) * (D * 128) + vg * 1024 + ((vc & 7) << 4);
-
+    // Where this thread's chunk 2 kt of K's row kr goes, in the stage; chunk 2 kt + 1 is 16 bytes on or
+    // back, and row 32 i + kr 4096 i bytes on.
+    const int at = kr ^ ((kr >> 1) & 4);
+    const int k_at = at * 128 + (((2 * kt) ^ (at & 7)) << 4);
 #pragma unroll 1
     for (int n = 0;; ++n) {
-      const int s = n % kStages;
       const int ik = 2 * n, iv = 2 * n + 1;  // K's and V's places in the run of rows
       if (!raw_full(ik)) break;
       const TileInfo ti = info[n & 3];
       if (ti.kind & kEnd) break;
       const bool diag = ti.kind & kDiag;
       if (diag && !raw_full(iv)) break;
-      const bool ragged = ti.limit < kKeys || ti.none != 0;
-      // ---- K(key, 16 dims of each group): two 16-byte chunks a group, 128-byte swizzled rows of 64 dims
-      {
-        const char* raw_k = sbase + S::oRaw + ik % kRawStages * S::kRaw + (th >> 6) * S::kRawRow;
-        __align__(16) uint32_t kw[4][2 * G], kp[4][G];
-        __half2 most = as_half2(0);
-#pragma unroll
+      char* tile = k_place();
+      if (!tile) break;
+      const char* raw_k = sbase + S::oRaw + ik % kRawStages * S::kRaw + (th >> 6) * S::kRawRow;
+      const char* raw_v = sbase + S::oRaw + iv % kRawStages * S::kRaw + (th >> 6) * S::kRawRow;
+      const int parts = ti.kind & kSplit ? 2 : 1;
+      // K(key, 16 dims of each group): two 16-byte chunks a group, 128-byte swizzled rows of 64 dims
+#pragma unroll 1
+      for (int part = 0; part < parts; ++part) {
+#pragma unroll 1
         for (int i = 0; i < 4; ++i) {
-          const char* row = raw_k + 2 * i * S::kRawRow;
-          const char* words = row + (kr & 15) * (L::kWidth / 2) + kt * (8 * G);
-          const char* pairs = row + L::kCodes + (kr & 15) * 4 * G;
+          const int row = 2 * i * S::kRawRow;
+          __align__(16) uint32_t kw[2 * G], kp[G];
+          const char* words = raw_k + row + (kr & 15) * (L::kWidth / 2) + kt * (8 * G);
+          const int pairs = row + L::kCodes + (kr & 15) * 4 * G;
           if constexpr (G == 2) {
-            *reinterpret_cast<uint4*>(kw[i]) = *reinterpret_cast<const uint4*>(words);
-            *reinterpret_cast<uint2*>(kp[i]) = *reinterpret_cast<const uint2*>(pairs);
+            *reinterpret_cast<uint4*>(kw) = *reinterpret_cast<const uint4*>(words);
+            *reinterpret_cast<uint2*>(kp) = *reinterpret_cast<const uint2*>(raw_k + pairs);
           } else {
-            *reinterpret_cast<uint2*>(kw[i]) = *reinterpret_cast<const uint2*>(words);
-            kp[i][0] = *reinterpret_cast<const uint32_t*>(pairs);
+            *reinterpret_cast<uint2*>(kw) = *reinterpret_cast<const uint2*>(words);
+            kp[0] = *reinterpret_cast<const uint32_t*>(raw_k + pairs);
           }
-        }
-        if (diag) {  // whoever sees a token whose V is NaN gets NaN, by way of its score
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t* vq = reinterpret_cast<const uint32_t*>(sbase + S::oRaw + iv % kRawStages * S::kRaw +
-                                                                   (2 * i + (th >> 6)) * S::kRawRow + L::kCodes +
-                                                                   (kr & 15) * 4 * G);
+          if (diag) {  // whoever sees a token whose V is NaN gets NaN, by way of its score
 #pragma unroll
             for (int e = 0; e < G; ++e)
-              if (is_nan_pair(vq[e])) kp[i][0] = 0x7fff7fffu;
+              if (is_nan_pair(*reinterpret_cast<const uint32_t*>(raw_v + pairs + 4 * e))) kp[0] = 0x7fff7fffu;
           }
-        }
-        mbar_arrive(bar + 8 * (kBarRawEmpty + ik % kRawStages));
-        if (ragged) {
+          const bool gone = 32 * i + kr >= ti.limit || ((ti.none >> (2 * i + (th >> 6))) & 1);
+          __half2 most = as_half2(0);
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (32 * i + kr >= ti.limit || ((ti.none >> (2 * i + (th >> 6))) & 1)) {
+          for (int e = 0; e < G; ++e) {
+            if (gone) kp[e] = 0;
+            most = __hmax2(most, __habs2(as_half2(kp[e])));
+          }
+          const bool clamp = __any_sync(kFull, may_overflow(most));
+          auto store = [&](int gi, int w, const uint32_t (&v)[4]) {
+            *reinterpret_cast<uint4*>(tile + i * 4096 + gi * S::kPanel + (k_at ^ (w << 4))) =
+                make_uint4(v[0], v[1], v[2], v[3]);
+          };
+          if (parts == 2) {  // as two fp16 numbers: K rounded, then what that leaves
 #pragma unroll
-              for (int e = 0; e < G; ++e) kp[i][e] = 0;
-            }
-        }
+            for (int gi = 0; gi < G; ++gi)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+              for (int w = 0; w < 2; ++w) {
+                const float2 pr = __half22float2(as_half2(kp[gi]));
+                uint32_t v[4];
 #pragma unroll
-          for (int e = 0; e < G; ++e) most = __hmax2(most, __habs2(as_half2(kp[i][e])));
-        const bool clamp = __any_sync(kFull, may_overflow(most));
-        char* tile = k_place();
-        if (!tile) break;
-        auto store = [&](int i, int gi, int w, const uint32_t (&v)[4]) {
-          *reinterpret_cast<uint4*>(tile + gi * S::kPanel + (k_at[i] ^ (w << 4))) = make_uint4(v[0], v[1], v[2], v[3]);
-        };
-        if (ti.kind & kSplit) {
-          // as two fp16 numbers: K rounded, then what that leaves
-#pragma unroll 1
-          for (int part = 0; part < 2 && tile; ++part) {
+                for (int e = 0; e < 4; ++e) {
+                  float x[2];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-              for (int gi = 0; gi < G; ++gi)
-#pragma unroll
-                for (int w = 0; w < 2; ++w) {
-                  const float2 pr = __half22float2(as_half2(kp[i][gi]));
-                  uint32_t v[4];
-#pragma unroll
-                  for (int e = 0; e < 4; ++e) {
-                    float x[2];
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                      const float y = fmaf((float)q4::k_code(kw[i][2 * gi + w], 2 * e + h), pr.x, pr.y);
-                      const float top = q4::max_nan(q4::min_nan(y, 65504.f), -65504.f);
-                      x[h] = part ? top - __half2float(__float2half_rn(top)) : top;
-                    }
-                    v[e] = Mma<__half>::pack(x[0], x[1]);
+                  for (int h = 0; h < 2; ++h) {
+                    const float y = fmaf((float)q4::k_code(kw[2 * gi + w], 2 * e + h), pr.x, pr.y);
+                    const float top = q4::max_nan(q4::min_nan(y, 65504.f), -65504.f);
+                    x[h] = part ? top - __half2float(__float2half_rn(top)) : top;
                   }
-                  store(i, gi, w, v);
+                  v[e] = Mma<__half>::pack(x[0], x[1]);
                 }
-            k_stored();
-            if (part == 0) tile = k_place();
-          }
-          if (!tile) break;
-        } else {
-          auto all = [&](auto limited) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
+                store(gi, w, v);
+              }
+          } else {
+            auto all = [&](auto limited) {
 #pragma unroll
               for (int gi = 0; gi < G; ++gi) {
-                const __half2 pr = as_half2(kp[i][gi]);
+                const __half2 pr = as_half2(kp[gi]);
 #pragma unroll
                 for (int w = 0; w < 2; ++w) {
                   uint32_t v[4];
-                  decode8<decltype(limited)::value>(kw[i][2 * gi + w], __low2half2(pr), __high2half2(pr), v);
-                  store(i, gi, w, v);
+                  decode8<decltype(limited)::value>(kw[2 * gi + w], __low2half2(pr), __high2half2(pr), v);
+                  store(gi, w, v);
                 }
               }
-          };
-          if (clamp) all(std::true_type{});
-          else all(std::false_type{});
-          k_stored();
-        }
-      }
-      // ---- V of 8 tokens, 8 dims of each group: one 16-byte chunk a dim, rows of 64 keys. The tokens are in
-      // the places' order: of a block's second half the last four come first.
-      if (!raw_full(iv)) break;
-      {
-        const int h = vc & 1;
-        const char* raw_v = sbase + S::oRaw + iv % kRawStages * S::kRaw + (vc >> 1) * S::kRawRow;
-        __align__(16) uint32_t vw[4][2 * G], vp[8][G];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int pair = (4 * h + i) ^ (2 * h);
-          const char* src = raw_v + pair * L::kWidth + (vg ^ L::turn(pair)) * (8 * G);
-          if constexpr (G == 2) *reinterpret_cast<uint4*>(vw[i]) = *reinterpret_cast<const uint4*>(src);
-          else *reinterpret_cast<uint2*>(vw[i]) = *reinterpret_cast<const uint2*>(src);
-        }
-        const uint4* pairs = reinterpret_cast<const uint4*>(raw_v + L::kCodes + h * 32 * G);
-#pragma unroll
-        for (int i = 0; i < 2 * G; ++i) *reinterpret_cast<uint4*>(&vp[0][0] + 4 * i) = pairs[i ^ (h * G)];
-        mbar_arrive(bar + 8 * (kBarRawEmpty + iv % kRawStages));
-        if (ragged || diag) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const bool gone = 8 * vc + (i ^ (4 * h)) >= ti.limit || ((ti.none >> (vc >> 1)) & 1);
-#pragma unroll
-            for (int e = 0; e < G; ++e)
-              if (gone || (diag && is_nan_pair(vp[i][e]))) vp[i][e] = 0;
+            };
+            if (clamp) all(std::true_type{});
+            else all(std::false_type{});
           }
         }
-        __half2 most = as_half2(0);
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-#pragma unroll
-          for (int e = 0; e < G; ++e) most = __hmax2(most, __habs2(as_half2(vp[i][e])));
-        const bool clamp = __any_sync(kFull, may_overflow(most));
+        k_stored();
+        if (part + 1 < parts) {
+          tile = k_place();
+          if (!tile) break;
+        }
+      }
+      if (!tile) break;
+      mbar_arrive(bar + 8 * (kBarRawEmpty + ik % kRawStages));
+      mbar_arrive(bar + 8 * (kBarRawEmpty + iv % kRawStages));
+    }
+  } else if (warp >= 12 && warp < 16) {
+    // ------------------------------------------------------------ V
+    registers_down<kRegsV>();
+    const int th = tid - 384;
+    // half block vc (of 16) and dims 8 vg ... of each group
+    const int vc = (th & 7) + 8 * (th >> 6), vg = ((th >> 3) & 3) + 4 * ((th >> 5) & 1);
+    const int h = vc & 1;
+    const int v_at = (vc >> 3) * (D * 128) + vg * 1024 + ((vc & 7) << 4);
+#pragma unroll 1
+    for (int n = 0;; ++n) {
+      const int s = n % kStages, ik = 2 * n, iv = 2 * n + 1;
+      if (!raw_full(ik)) break;
+      const TileInfo ti = info[n & 3];
+      mbar_arrive(bar + 8 * (kBarRawEmpty + ik % kRawStages));
+      if ((ti.kind & kEnd) || !raw_full(iv)) break;
+      const bool diag = ti.kind & kDiag;
+      // V of 8 tokens, 8 dims of each group: one 16-byte chunk a dim, rows of 64 keys. The tokens are in the
+      // places' order: of a block's second half the last four come first.
+      {
         if (n >= kStages && !wait_or_flag(bar + 8 * (kBarVEmpty + s), (n / kStages - 1) & 1, failed)) break;
+        const char* raw_v = sbase + S::oRaw + iv % kRawStages * S::kRaw + (vc >> 1) * S::kRawRow;
         char* tile = sbase + S::oV + s * S::kTile;
-        auto all = [&](auto limited) {
+        const bool none = (ti.none >> (vc >> 1)) & 1;
+#pragma unroll 1
+        for (int gi = 0; gi < G; ++gi) {
+          __align__(8) uint32_t vw[4][2];
+          uint32_t vp[8];
 #pragma unroll
-          for (int gi = 0; gi < G; ++gi) {
-            __half2 sc[4], lo[4];
+          for (int i = 0; i < 4; ++i) {
+            const int pair = (4 * h + i) ^ (2 * h);
+            *reinterpret_cast<uint2*>(vw[i]) =
+                *reinterpret_cast<const uint2*>(raw_v + pair * L::kWidth + (vg ^ L::turn(pair)) * (8 * G) + gi * 8);
+          }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const __half2 a = as_half2(vp[2 * i][gi]), b = as_half2(vp[2 * i + 1][gi]);
-              sc[i] = __lows2half2(a, b);
-              lo[i] = __highs2half2(a, b);
-            }
+          for (int i = 0; i < 8; ++i)
+            vp[i] = *reinterpret_cast<const uint32_t*>(raw_v + L::kCodes + (8 * h + (i ^ (4 * h))) * 4 * G + gi * 4);
+          if (ti.limit < kKeys || ti.none != 0 || diag) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (8 * vc + (i ^ (4 * h)) >= ti.limit || none || (diag && is_nan_pair(vp[i]))) vp[i] = 0;
+          }
+          __half2 most = as_half2(0), sc[4], lo[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const __half2 a = as_half2(vp[2 * i]), b = as_half2(vp[2 * i + 1]);
+            most = __hmax2(most, __hmax2(__habs2(a), __habs2(b)));
+            sc[i] = __lows2half2(a, b);
+            lo[i] = __highs2half2(a, b);
+          }
+          auto all = [&](auto limited) {
 #pragma unroll
             for (int w = 0; w < 2; ++w) {
               uint32_t v[4][4];
 #pragma unroll
-              for (int i = 0; i < 4; ++i) decode8<decltype(limited)::value>(vw[i][2 * gi + w], sc[i], lo[i], v[i]);
+              for (int i = 0; i < 4; ++i) decode8<decltype(limited)::value>(vw[i][w], sc[i], lo[i], v[i]);
 #pragma unroll
               for (int e = 0; e < 4; ++e)
                 *reinterpret_cast<uint4*>(tile + gi * 8192 + (4 * w + e) * 128 + (v_at ^ ((4 * w + e) << 4))) =
                     make_uint4(v[0][e], v[1][e], v[2][e], v[3][e]);
             }
-          }
-        };
-        if (clamp) all(std::true_type{});
-        else all(std::false_type{});
+          };
+          if (__any_sync(kFull, may_overflow(most))) all(std::true_type{});
+          else all(std::false_type{});
+        }
+        mbar_arrive(bar + 8 * (kBarRawEmpty + iv % kRawStages));
         fence_proxy_async_smem();
         mbar_arrive(bar + 8 * (kBarVFull + s));
       }
     }
-  } else if (warp >= 12) {
-    registers_down<120>();
-    if (warp > 13) goto done;
-    if (warp == 13) {
+  } else if (warp >= 16) {
+    registers_down<kRegsMma>();
+    if (warp > 17) goto done;
+    if (warp == 17) {
       // -------------------------------------------------------------- copies
       int i = 0, n = 0;  // rows of K and V asked for, and tiles
       Unit w;
@@ -624,63 +610,76 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
     mbar_wait_bounded(bar + 8 * kBarFinal, 0, 1u << 20);
   } else {
     // ------------------------------------------------------------ softmax
-    registers_down<120>();
+    registers_up<kRegsSoftmax>();
     const int qt = warp >> 2;
     const int m = (warp & 3) * 32 + lane;
     const uint32_t taddr = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t col_s = qt * 128, col_o = kColO + qt * D;
     const int tk = m / p.group, gh = m - tk * p.group;
+    const int tok = qt * p.tile + tk;  // the row's token, of the unit
     int ns = 0, nd = 0;  // tiles of scores and units done, of this query tile
     int nt = 0;          // K tiles of all units (the ring's count)
-    Unit w;
+    auto is_live = [&](const Unit& w) { return tk < p.tile && w.tok0 + tok < w.q_len; };
+    // The row's query to shared memory as fp16 after a power of two; returns what brings its scores to log2 units.
+    auto store_query = [&](const Unit& w) -> float {
+      using T2 = typename Two<T>::type;
+      const bool live = is_live(w);
+      __align__(16) T2 q[D / 2];
+      T2 most = Two<T>::zero();
+      const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.q) + (w.token + tok) * p.q_st +
+                                                        (int64_t)(w.kvh * p.group + gh) * p.q_sh);
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i)
+        *reinterpret_cast<uint4*>(&q[4 * i]) = live ? __ldg(src + i) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+      for (int i = 0; i < D / 2; ++i) most = __hmax2_nan(most, __habs2(q[i]));
+      const float top = q4::max_nan(Elem<T>::to_float(low_of(most)), Elem<T>::to_float(high_of(most)));
+      const int ex = query_exponent(top);
+      const float down = power2(-ex);
+      char* row = sbase + S::oQ + qt * S::kTile + m * 128;
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) {
+        uint32_t v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          v[e] = Mma<__half>::pack(Elem<T>::to_float(low_of(q[4 * i + e])) * down,
+                                   Elem<T>::to_float(high_of(q[4 * i + e])) * down);
+        *reinterpret_cast<uint4*>(row + (i >> 3) * S::kPanel + (((i & 7) ^ (m & 7)) << 4)) =
+            make_uint4(v[0], v[1], v[2], v[3]);
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(bar + 8 * (kBarQFull + qt));
+      return copysignf(fminf(fabsf(p.scale_log2) * power2(ex), FLT_MAX), p.scale_log2);
+    };
+    // The CTA's next unit from u on that has this query tile and keys; rows that see nothing are written here.
+    auto next_unit = [&](uint32_t& u, Unit& w) {
 #pragma unroll 1
-    for (uint32_t u = blockIdx.x; find_unit(p, prefix, u, w); u += gridDim.x) {
+      for (; find_unit(p, prefix, u, w); u += gridDim.x) {
+        if (qt < w.tiles && w.ntiles > 0) return true;
+        if (qt < w.tiles && is_live(w)) {
+          const int head = w.kvh * p.group + gh;
+          uint4* op = reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) + (w.token + tok) * p.o_st + (int64_t)head * p.o_sh);
+#pragma unroll 1
+          for (int d = 0; d < D / 8; ++d) op[d] = make_uint4(0u, 0u, 0u, 0u);
+          p.lse[(w.token + tok) * p.lse_st + head] = -INFINITY;
+        }
+        nt += w.ntiles;  // of the other query tile alone
+      }
+      return false;
+    };
+    uint32_t u = blockIdx.x;
+    Unit w;
+    bool have = next_unit(u, w);
+    float c_next = have ? store_query(w) : 0.f;
+#pragma unroll 1
+    while (have) {
+      const float c = c_next;
+      const bool live = is_live(w);
       const int first_tile = nt;
       nt += w.ntiles;
-      if (qt >= w.tiles) continue;
-      const int tok = qt * p.tile + tk;  // of the unit
-      const bool live = tk < p.tile && w.tok0 + tok < w.q_len;
       const int head = w.kvh * p.group + gh;
       T* op = reinterpret_cast<T*>(p.out) + (w.token + tok) * p.o_st + (int64_t)head * p.o_sh;
       float* lp = p.lse + (w.token + tok) * p.lse_st + head;
-      if (w.ntiles == 0) {
-        if (live) {
-          for (int d = 0; d < D / 8; ++d) reinterpret_cast<uint4*>(op)[d] = make_uint4(0u, 0u, 0u, 0u);
-          *lp = -INFINITY;
-        }
-        continue;
-      }
-      // ---- the row's query, as fp16 after a power of two
-      float c;
-      {
-        using T2 = typename Two<T>::type;
-        __align__(16) T2 q[D / 2];
-        T2 most = Two<T>::zero();
-        const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.q) + (w.token + tok) * p.q_st +
-                                                          (int64_t)head * p.q_sh);
-#pragma unroll
-        for (int i = 0; i < D / 8; ++i)
-          *reinterpret_cast<uint4*>(&q[4 * i]) = live ? __ldg(src + i) : make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-        for (int i = 0; i < D / 2; ++i) most = __hmax2_nan(most, __habs2(q[i]));
-        const float top = q4::max_nan(Elem<T>::to_float(low_of(most)), Elem<T>::to_float(high_of(most)));
-        const int ex = query_exponent(top);
-        const float down = power2(-ex);
-        c = copysignf(fminf(fabsf(p.scale_log2) * power2(ex), FLT_MAX), p.scale_log2);
-        char* row = sbase + S::oQ + qt * S::kTile + m * 128;
-#pragma unroll
-        for (int i = 0; i < D / 8; ++i) {
-          uint32_t v[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            v[e] = Mma<__half>::pack(Elem<T>::to_float(low_of(q[4 * i + e])) * down,
-                                     Elem<T>::to_float(high_of(q[4 * i + e])) * down);
-          *reinterpret_cast<uint4*>(row + (i >> 3) * S::kPanel + (((i & 7) ^ (m & 7)) << 4)) =
-              make_uint4(v[0], v[1], v[2], v[3]);
-        }
-        fence_proxy_async_smem();
-        mbar_arrive(bar + 8 * (kBarQFull + qt));
-      }
       const int vis = !live ? 0 : p.causal ? min(w.k_len, w.sees + tok) : w.k_len;
       const int all_see = p.causal ? min(w.k_len, w.sees + qt * p.tile) : w.k_len;  // every row of the tile
       float m_ref = -INFINITY, l = 0.f;
@@ -754,8 +753,7 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
             const float2 d = fma2(make_float2(x[2 * e], x[2 * e + 1]), splat2(cx), splat2(neg));
-            // (a masked score weighs 2^-126 on the FMA pipe, and 0 as fp16)
-            const float2 pr = (kPolyPairs >> e) & 1 ? poly_exp2x2(d) : make_float2(fast_exp2(d.x), fast_exp2(d.y));
+            const float2 pr = make_float2(fast_exp2(d.x), fast_exp2(d.y));
             if (e & 1) sum1 = add2(sum1, pr);
             else sum0 = add2(sum0, pr);
             hi[e] = Mma<__half>::pack(pr.x, pr.y);
@@ -789,6 +787,10 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
         __syncwarp();
         if (lane == 0) mbar_arrive(bar + 8 * (kBarPFull + qt));
       }
+      // ---- the next unit's query, so that its first scores come while this one's O is written
+      u += gridDim.x;
+      have = !__any_sync(kFull, failed) && next_unit(u, w);
+      if (have) c_next = store_query(w);
       // ---- O is final
       wait_or_flag(bar + 8 * (kBarODone + qt), nd & 1, failed);
       ++nd;
@@ -819,7 +821,7 @@ done:
   if (failed && lane == 0) atomic_or_err(p.err, SEB_ERRBIT_TIMEOUT);
   tc::fence_before_sync();
   __syncthreads();
-  if (warp == 12) {
+  if (warp == 16) {
     tc::fence_after_sync();
     tc::tmem_dealloc(tmem, kTmemCols);
   }
