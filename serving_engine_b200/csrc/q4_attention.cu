@@ -35,21 +35,24 @@ namespace seb {
 namespace {
 
 constexpr uint32_t kMinRun = 2;          // pairs of blocks of the shortest run worth a warp
+constexpr uint32_t kUnitCost = 2;        // what a unit's start and end cost a warp, in pairs of blocks
 constexpr float kNoMax = -FLT_MAX;       // no score yet: any score is above it by more than the threshold
 constexpr float kThreshold = 8.f;        // scores may exceed the reference by 2^8 before it is moved
 constexpr float kScaleThreshold = 64.f;  // p * V scale stays below 2^8 * 2^6
 
-// Arrivals at the units that span CTAs, one for each column, at the CTA that a unit
+// Arrivals at the units that span CTAs, one for each four columns, at the CTA that a unit
 // starts in. Zero when the library is loaded, and again after every call (the last to
 // arrive clears it); calls that may overlap use different slots.
 constexpr int kMaxCtas = 512;
-__device__ int32_t g_q4_counters[SEB_Q4_COUNTER_SLOTS][kMaxCtas * 32];
+__device__ int32_t g_q4_counters[SEB_Q4_COUNTER_SLOTS][kMaxCtas * 4];
 
-__device__ __forceinline__ uint32_t pairs_of(const Q4Params& p, const Row& w) { return w.tiles * p.hkv * w.pairs; }
+// A unit's length in the run of all units: kUnitCost places that stand for no blocks, then its pairs.
+__device__ __forceinline__ uint32_t length_of(const Row& w) { return w.pairs + kUnitCost; }
+__device__ __forceinline__ uint32_t pairs_of(const Q4Params& p, const Row& w) { return w.tiles * p.hkv * length_of(w); }
 
 // What a warp leaves of a unit that it did not do alone.
 struct Part {
-  uint32_t unit;  // the unit's first pair in the run of all units
+  uint32_t unit;  // the unit's first place in the run of all units
   uint32_t end;   // and past its last; 0: no part
   int64_t token;  // the tile's first
   int kvh, cols;
@@ -97,49 +100,58 @@ __device__ __forceinline__ void load_dims(const float* row, int lane, float (&v)
   }
 }
 
-// Joins `n` parts of one column: lane l gets its dims of the sum of O, against the largest
-// reference m, and the sum l. part(i, row, ml) finds part i's O and its (m, l). LANES: the
-// parts taken at a time.
-template <int D, int LANES, bool GLOBAL, typename F>
-__device__ __forceinline__ void join(int n, int lane, F part, float (&o)[D / 32], float& m, float& l) {
+// Joins `n` parts of up to four columns. Lane l gets its dims of each column's sum of O, and
+// lanes 8 c .. 8 c + 7 have column c's reference m and sum l. part(i) is where part i's O
+// rows and, `ml` floats on, (m, l) pairs begin, those of the first of the columns.
+template <int D, bool GLOBAL, typename F>
+__device__ __forceinline__ void join(int n, int cols, int lane, F part, int ml, float (&o)[4][D / 32], float& m,
+                                     float& l) {
   constexpr int DL = D / 32;
   m = -INFINITY;
   l = 0.f;
 #pragma unroll
-  for (int e = 0; e < DL; ++e) o[e] = 0.f;
-#pragma unroll 1
-  for (int i0 = 0; i0 < n; i0 += LANES) {
-    const float* row;
-    const float2* ml;
-    float2 mine = make_float2(-INFINITY, 0.f);
-    const int i = i0 + lane % LANES;
-    if (i < n) {
-      part(i, row, ml);
-      mine = GLOBAL ? __ldcg(ml) : *ml;
-    }
-    float top = mine.x;
+  for (int c = 0; c < 4; ++c)
 #pragma unroll
-    for (int off = LANES / 2; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, off));
-    top = fmaxf(top, m);
+    for (int e = 0; e < DL; ++e) o[c][e] = 0.f;
+#pragma unroll 1
+  for (int i0 = 0; i0 < n; i0 += 8) {
+    float2 mine = make_float2(-INFINITY, 0.f);
+    if (i0 + (lane & 7) < n && (lane >> 3) < cols) {
+      const float2* at = reinterpret_cast<const float2*>(part(i0 + (lane & 7)) + ml) + (lane >> 3);
+      mine = GLOBAL ? __ldcg(at) : *at;
+    }
+    float top = fmaxf(m, mine.x);
+#pragma unroll
+    for (int off = 4; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, off));
     const float ref = top == -INFINITY ? 0.f : top;
-    const float keep = exp2_fast(m - ref);
-    const float w = exp2_fast(mine.x - ref);
+    const float keep = exp2_fast(m - ref), w = exp2_fast(mine.x - ref);
     float sum = mine.y * w;
 #pragma unroll
-    for (int off = LANES / 2; off >= 1; off >>= 1) sum += __shfl_xor_sync(kFull, sum, off);
+    for (int off = 4; off >= 1; off >>= 1) sum += __shfl_xor_sync(kFull, sum, off);
     l = fmaf(l, keep, sum);
     m = top;
+    if (i0 > 0) {
 #pragma unroll
-    for (int e = 0; e < DL; ++e) o[e] *= keep;
-    const int cnt = min(LANES, n - i0);
+      for (int c = 0; c < 4; ++c) {
+        const float k = __shfl_sync(kFull, keep, 8 * c);
+#pragma unroll
+        for (int e = 0; e < DL; ++e) o[c][e] *= k;
+      }
+    }
+    const int cnt = min(8, n - i0);
 #pragma unroll(GLOBAL ? 4 : 2)
     for (int k = 0; k < cnt; ++k) {
-      part(i0 + k, row, ml);
-      float v[DL];
-      load_dims<D, GLOBAL>(row, lane, v);
-      const float wk = __shfl_sync(kFull, w, k);
+      const float* row = part(i0 + k);
 #pragma unroll
-      for (int e = 0; e < DL; ++e) o[e] = fmaf(wk, v[e], o[e]);
+      for (int c = 0; c < 4; ++c) {
+        const float wk = __shfl_sync(kFull, w, 8 * c + k);
+        if (c < cols) {
+          float v[DL];
+          load_dims<D, GLOBAL>(row + c * D, lane, v);
+#pragma unroll
+          for (int e = 0; e < DL; ++e) o[c][e] = fmaf(wk, v[e], o[c][e]);
+        }
+      }
     }
   }
 }
@@ -163,6 +175,15 @@ __device__ __forceinline__ void write_column(const Q4Params& p, int64_t token, i
   if (lane == 0) p.lse[tok * p.lse_st + head] = l == 0.f ? -INFINITY : fmaf(m, kLn2, logf(l));
 }
 
+// D = A B on fp16 operands, m16n8k16.
+__device__ __forceinline__ void mma_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                          uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+
 // What a warp keeps of the unit it is on.
 template <int D, int NT>
 struct Tile {
@@ -173,7 +194,7 @@ struct Tile {
   float m[NT][2], l[NT][2];   // reference, and this lane's share of the sum
   float low[GR][NT][2];       // this lane's share of sum p (low + 8 scale)
   float one[(GR + 1) / 2][NT][4];  // sum of the rounded p * scale, two groups to a tile
-  float o[GR][4][NT][4];      // sum of those and the codes
+  float o[GR][4][NT][4];      // sum of those and the codes: n + 16 n' of two dims, and 16 n'
   float v_down;               // power of two that V's scales are taken by
 };
 
@@ -286,18 +307,17 @@ __device__ __forceinline__ void take_blocks(Tile<D, NT>& u, const char* place, i
         const int gr = pn * G + gi;
         float acc[NT][4];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) acc[nt][c] = 0.f;
-#pragma unroll
         for (int i = 0; i < 2; ++i) {
           uint32_t k0 = w[0][gi * 2 + i], k1 = w[1][gi * 2 + i];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
+            const uint32_t a0 = k0 & 0x000f000fu, a1 = k1 & 0x000f000fu, a2 = k0 & 0x00f000f0u, a3 = k1 & 0x00f000f0u;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-              Mma<__half>::run(acc[nt], k0 & 0x000f000fu, k1 & 0x000f000fu, k0 & 0x00f000f0u, k1 & 0x00f000f0u,
-                               u.qf[gr][nt][2 * i + h][0], u.qf[gr][nt][2 * i + h][1]);
+            for (int nt = 0; nt < NT; ++nt) {
+              const uint32_t(&q)[2] = u.qf[gr][nt][2 * i + h];
+              if (i == 0 && h == 0) mma_first(acc[nt], a0, a1, a2, a3, q[0], q[1]);
+              else Mma<__half>::run(acc[nt], a0, a1, a2, a3, q[0], q[1]);
+            }
             k0 >>= 8, k1 >>= 8;
           }
         }
@@ -430,14 +450,15 @@ __device__ __forceinline__ void take_blocks(Tile<D, NT>& u, const char* place, i
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          uint32_t v0 = w[0][gi * 2 + i], v1 = w[1][gi * 2 + i];
+          // whole bytes, n + 16 n', and their upper codes, 16 n': the first less the second is n's sum
+          const uint32_t v0 = w[0][gi * 2 + i], v1 = w[1][gi * 2 + i];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
+            const uint32_t x0 = h ? __byte_perm(v0, 0, 0x4341) : v0 & 0x00ff00ffu;
+            const uint32_t x1 = h ? __byte_perm(v1, 0, 0x4341) : v1 & 0x00ff00ffu;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
-              Mma<__half>::run(u.o[gr][2 * i + h][nt], v0 & 0x000f000fu, v0 & 0x00f000f0u, v1 & 0x000f000fu,
-                               v1 & 0x00f000f0u, b0[nt], b1[nt]);
-            v0 >>= 8, v1 >>= 8;
+              Mma<__half>::run(u.o[gr][2 * i + h][nt], x0, x0 & 0x00f000f0u, x1, x1 & 0x00f000f0u, b0[nt], b1[nt]);
           }
         }
       }
@@ -451,6 +472,7 @@ __global__ void __launch_bounds__(NW * 32, CTAS) q4_attention_kernel(const Q4Par
   using S = Smem<D, NT, NW, STAGES>;
   constexpr int GR = D / q4::kGroup;
   constexpr int kCols = S::kCols;
+  constexpr int kPart = kCols * (D + 2);  // floats of a part: O, then (m, l)
   extern __shared__ __align__(128) char smem[];
   Part* parts = reinterpret_cast<Part*>(smem + S::kParts);
   uint32_t* prefix = reinterpret_cast<uint32_t*>(smem + S::kPrefix);
@@ -523,10 +545,11 @@ __global__ void __launch_bounds__(NW * 32, CTAS) q4_attention_kernel(const Q4Par
         len = pairs_of(p, row);
       }
       if (off >= len) break;  // rows that overlap, beyond what can be counted
-      const uint32_t unit = off / row.pairs;  // tiles of one kv head are neighbours: they read the same blocks
-      const uint32_t pair0 = off - unit * row.pairs, n = min(row.pairs - pair0, stop - pos);
+      const uint32_t length = length_of(row);
+      const uint32_t unit = off / length;  // tiles of one kv head are neighbours: they read the same blocks
+      const uint32_t place = off - unit * length, n = min(length - place, stop - pos);
       const int kvh = (int)(unit / row.tiles), tile = (int)(unit - kvh * row.tiles);
-      const int blk0 = 2 * (int)pair0;
+      const int blk0 = 2 * max((int)(place - kUnitCost), 0);
       const int tok0 = tile * p.tile;  // first token of the tile in the row
       const int toks = min(p.tile, row.q_len - tok0);
       const int cols = toks * p.group;
@@ -536,7 +559,7 @@ __global__ void __launch_bounds__(NW * 32, CTAS) q4_attention_kernel(const Q4Par
           p.causal ? (int)min((int64_t)row.q_pos + tok0 + 1, (int64_t)(1 << 30)) : row.k_len;
       const int see_all = min(row.k_len, max(first_sees, 0));
       const int see_any = p.causal ? min(row.k_len, max(first_sees + toks - 1, 0)) : row.k_len;
-      const int blk1 = min(blk0 + 2 * (int)n, (see_any + 15) >> 4);  // blocks from here on hold nothing for this tile
+      const int blk1 = min(2 * (int)(place + n - kUnitCost), (see_any + 15) >> 4);  // blocks from here on hold nothing for this tile
 
       // ---- block ids, 32 at a time; ring prologue
       const int32_t* table = p.block_table + (int64_t)r * p.bt_stride;
@@ -611,9 +634,9 @@ __global__ void __launch_bounds__(NW * 32, CTAS) q4_attention_kernel(const Q4Par
         const unsigned none = (unread >> (2 * s)) & 3;
         const char* place = ring + s * S::kStage;
         // two blocks at once where the tile leaves registers for it
-        constexpr int KB = GR * NT <= 2 ? 2 : 1;
+        constexpr int KB = GR * NT <= 1 ? 2 : 1;
         if (none == 0 && (b + 2) * 16 <= see_all) {
-#pragma unroll
+#pragma unroll 1
           for (int i = 0; i < 2; i += KB)
             take_blocks<D, NT, KB, false>(u, place + i * 2 * L::kRow, lane, (b + i) * 16, 0, end);
         } else {
@@ -628,7 +651,7 @@ __global__ void __launch_bounds__(NW * 32, CTAS) q4_attention_kernel(const Q4Par
         for (; it != issued; ++it) mbar_wait_bounded(bars + 8 * (it % STAGES), (it / STAGES) & 1, 1u << 16);
 
       // ---- the result, or this warp's part of it, by way of shared memory. Nothing is in flight to the ring now.
-      const bool whole = n == row.pairs;
+      const bool whole = n == length;
       const bool last_run = pos + n == stop;
       float* po = reinterpret_cast<float*>(whole || last_run ? ring : ring + S::kRing);
       const float v_up = power2(24) / u.v_down;
@@ -650,7 +673,7 @@ __global__ void __launch_bounds__(NW * 32, CTAS) q4_attention_kernel(const Q4Par
             float v[8];
 #pragma unroll
             for (int mt = 0; mt < 4; ++mt) {
-              v[2 * mt] = fmaf(u.o[gr][mt][nt][h] - one, v_up, z);
+              v[2 * mt] = fmaf(u.o[gr][mt][nt][h] - u.o[gr][mt][nt][h + 2] - one, v_up, z);
               v[2 * mt + 1] = fmaf(fmaf(u.o[gr][mt][nt][h + 2], 0.0625f, -one), v_up, z);
             }
             if (col < cols) {
@@ -673,7 +696,7 @@ __global__ void __launch_bounds__(NW * 32, CTAS) q4_attention_kernel(const Q4Par
           write_column<T, D>(p, token, kvh, col, lane, o, ml.x, ml.y);
         }
       } else if (lane == 0) {
-        parts[warp * 2 + (last_run ? 1 : 0)] = Part{pos - pair0, pos - pair0 + row.pairs, token, kvh, cols};
+        parts[warp * 2 + (last_run ? 1 : 0)] = Part{pos - place, pos - place + length, token, kvh, cols};
       }
       fence_proxy_async_smem();  // the ring is written by copies next
       __syncwarp();
@@ -684,7 +707,7 @@ __global__ void __launch_bounds__(NW * 32, CTAS) q4_attention_kernel(const Q4Par
 
   // ---- join the parts. A unit's parts are one of each of neighbouring warps, so in the list of
   // 2 NW places neighbours but for empty places; a bit of a mask stands for each place. A warp
-  // takes a column; of units that go on in other CTAs first, so that their arrival is early.
+  // takes four columns; of units that go on in other CTAs first, so that their arrival is early.
   __syncthreads();
   const float* base = reinterpret_cast<const float*>(smem + S::kWarps);
   uint32_t unit = 0, end = 0;
@@ -705,41 +728,46 @@ __global__ void __launch_bounds__(NW * 32, CTAS) q4_attention_kernel(const Q4Par
       const int i = __ffs(left) - 1, w0 = i >> 1;
       const unsigned later = starts & ~((2u << i) - 1);  // the next unit's first place and on
       const unsigned list = used & ~((1u << i) - 1) & (later ? (1u << (__ffs(later) - 1)) - 1 : ~0u);
-      const int n = __popc(list);
       const Part pt = parts[i];
 #pragma unroll 1
-      for (int col = (warp + NW - job % NW) % NW; col < pt.cols; col += NW) {
-        float o[D / 32], m, l;
-        join<D, 8, false>(n, lane, [&](int k, const float*& row, const float2*& ml) {
-          const float* at = base + ((w0 + k) * S::kWarp + (list >> (2 * (w0 + k)) & 1 ? S::kRing : 0)) / 4;
-          row = at + col * D;
-          ml = reinterpret_cast<const float2*>(at + kCols * D) + col;
-        }, o, m, l);
+      for (int col = 0; col < pt.cols; col += 4, ++job) {
+        if (job % NW != warp) continue;
+        const int cols = min(4, pt.cols - col);
+        float o[4][D / 32], m, l;
+        join<D, false>(__popc(list), cols, lane, [&](int k) {
+          return base + ((w0 + k) * S::kWarp + (list >> (2 * (w0 + k)) & 1 ? S::kRing : 0)) / 4 + col * D;
+        }, kCols * D - col * D + 2 * col, o, m, l);
         if (pass == 0) {
           const int first = pt.unit / span, last = (pt.end - 1) / span;
-          const int64_t slot = ((int64_t)blockIdx.x * 2 + (pt.unit >= cta0 ? 1 : 0)) * kCols + col;
-          float* dst = p.ws_o + slot * D + lane * (D / 32);
+          const int64_t slot = ((int64_t)blockIdx.x * 2 + (pt.unit >= cta0 ? 1 : 0)) * kPart;
 #pragma unroll
-          for (int e = 0; e < D / 32; ++e) dst[e] = o[e];
-          if (lane == 0) reinterpret_cast<float2*>(p.ws_ml)[slot] = make_float2(m, l);
+          for (int c = 0; c < 4; ++c)
+            if (c < cols) {
+              float* dst = p.ws + slot + (col + c) * D + lane * (D / 32);
+#pragma unroll
+              for (int e = 0; e < D / 32; ++e) dst[e] = o[c][e];
+            }
+          if ((lane & 7) == 0 && (lane >> 3) < cols)
+            reinterpret_cast<float2*>(p.ws + slot + kCols * D)[col + (lane >> 3)] = make_float2(m, l);
           __threadfence();
           __syncwarp();
-          int32_t* ctr = g_q4_counters[p.counter_slot] + first * kCols + col;
+          int32_t* ctr = g_q4_counters[p.counter_slot] + (first * kCols + col) / 4;
           int arrived = 0;
           if (lane == 0) arrived = atomicAdd(ctr, 1);
           arrived = __shfl_sync(kFull, arrived, 0);
           if (arrived != last - first) continue;
           if (lane == 0) *ctr = 0;
           __threadfence();
-          join<D, 32, true>(last - first + 1, lane, [&](int k, const float*& row, const float2*& ml) {
-            const int64_t at = ((int64_t)(first + k) * 2 + (k == 0 ? 1 : 0)) * kCols + col;
-            row = p.ws_o + at * D;
-            ml = reinterpret_cast<const float2*>(p.ws_ml) + at;
-          }, o, m, l);
+          join<D, true>(last - first + 1, cols, lane, [&](int k) {
+            return p.ws + ((int64_t)(first + k) * 2 + (k == 0 ? 1 : 0)) * kPart + col * D;
+          }, kCols * D - col * D + 2 * col, o, m, l);
         }
-        write_column<T, D>(p, pt.token, pt.kvh, col, lane, o, m, l);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const float mc = __shfl_sync(kFull, m, 8 * c), lc = __shfl_sync(kFull, l, 8 * c);
+          if (c < cols) write_column<T, D>(p, pt.token, pt.kvh, col + c, lane, o[c], mc, lc);
+        }
       }
-      job += pt.cols;
     }
   }
 }
@@ -749,7 +777,7 @@ template <int D, int NT>
 struct Shape {
   static constexpr int kSize = D / 64 * NT;  // a measure of the tile's accumulators
   static constexpr int kWarps = kSize <= 2 ? 8 : kSize <= 4 ? 4 : 6;
-  static constexpr int kCtas = kSize <= 2 ? 2 : kSize <= 4 ? 3 : 1;
+  static constexpr int kCtas = kSize <= 2 ? 2 : kSize <= 4 ? 2 : 1;
   static constexpr int kStages = D == 64 ? 4 : D == 128 ? 2 : 1;
 };
 
@@ -785,15 +813,14 @@ int launch(Q4Params& p, void* workspace, int64_t bytes, cudaStream_t s) {
     return SEB_EWORKSPACE;
   }
   const int ctas = grid_of<D, NT>();
-  p.ws_o = static_cast<float*>(workspace);
-  p.ws_ml = p.ws_o + (int64_t)ctas * 2 * 8 * NT * D;
+  p.ws = static_cast<float*>(workspace);
   p.tile = std::max(1, 8 * NT / p.group);
   p.by_group = (65536 + p.group - 1) / p.group;
   const int rc = set_smem_limit_once<kern>(smem);
   if (rc != SEB_OK) return rc;
   // no more CTAs than the longest rows that the table allows would fill
   const int64_t tiles = ((int64_t)p.total_query + (int64_t)p.num_rows * (p.tile - 1)) / p.tile;
-  const int64_t pairs = tiles * p.hkv * ((p.max_blocks + 1) / 2);
+  const int64_t pairs = tiles * p.hkv * ((p.max_blocks + 1) / 2 + kUnitCost);
   if (pairs > 0xffff0000ll) {
     set_error("seb_paged_attention_q4: %lld tiles of %lld blocks are too much work for one call", (long long)tiles * p.hkv,
               (long long)p.max_blocks);

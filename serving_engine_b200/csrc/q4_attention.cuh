@@ -36,8 +36,7 @@ struct Q4Params {
   float* lse;
   int64_t lse_st;
   int32_t counter_slot;
-  float* ws_o;        // [CTA][2][columns][D]
-  float* ws_ml;       // [CTA][2][columns][2]
+  float* ws;  // [CTA][2] parts: [columns][D], then [columns][2]
   int32_t* err;
 };
 
