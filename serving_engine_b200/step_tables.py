@@ -12,8 +12,8 @@ from __future__ import annotations
 
 import torch
 
-from . import ops
-from ._lib import check, lib
+from . import q4
+from ._lib import lib
 
 MAX_ROWS = 16384
 
@@ -38,6 +38,9 @@ class StepTables:
         self.item_row = narrow[3 * rows:3 * rows + tokens]
         self.free_state = narrow[3 * rows + tokens:]
         self.device = wide.device
+        if wide.get_device() < 0:
+            raise ValueError(f"StepTables: a CUDA device is required, got {wide.device}")
+        self._device = wide.get_device()
         self._out = tuple(t.data_ptr() for t in (self.q_starts, self.k_lens, self.q_pos_offsets, self.item_row,
                                                  self.positions, self.slot_mapping, self.free_state))
 
@@ -53,29 +56,38 @@ class StepTables:
         The host can follow without reading back: rows take ceil(k_len / 16) -
         ceil(context / 16) blocks each, in row order from the head of the ring.
         """
-        dev = self.device
-        for name, t, shape in (("q_lens", q_lens, (self.rows,)), ("context_lens", context_lens, (self.rows,)),
-                               ("free_state", free_state, (2,))):
-            if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous() or t.device != dev:
-                raise ValueError(f"StepTables.build: {name} must be int32 {list(shape)}, contiguous and on {dev}")
-        if (block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != self.rows
-                or block_table.shape[1] == 0 or block_table.stride(1) != 1 or block_table.device != dev
-                or block_table.stride(0) < block_table.shape[1]):
-            raise ValueError(f"StepTables.build: block_table must be int32 [{self.rows}, max_blocks >= 1] on {dev} "
-                             "with unit column stride and rows that do not overlap")
-        if (free_ids.dtype != torch.int32 or free_ids.dim() != 1 or free_ids.numel() == 0
-                or not free_ids.is_contiguous() or free_ids.device != dev):
-            raise ValueError(f"StepTables.build: free_ids must be a non-empty int32 vector, contiguous and on {dev}")
+        dev = self._device
+        rows = self.rows
+        shape, strides = block_table.shape, block_table.stride()
+        if not (q_lens.dtype == context_lens.dtype == block_table.dtype == free_ids.dtype == free_state.dtype == torch.int32
+                and q_lens.shape == context_lens.shape == (rows,) and free_state.shape == (2,) and free_ids.dim() == 1
+                and free_ids.numel() and q_lens.is_contiguous() and context_lens.is_contiguous()
+                and free_ids.is_contiguous() and free_state.is_contiguous() and len(shape) == 2 and shape[0] == rows
+                and shape[1] and strides[1] == 1 and (rows == 1 or strides[0] >= shape[1])
+                and q_lens.get_device() == context_lens.get_device() == block_table.get_device()
+                == free_ids.get_device() == free_state.get_device() == dev):
+            self._refuse(q_lens, context_lens, block_table, free_ids, free_state)
         if free_state.data_ptr() == self._out[-1]:
             raise ValueError("StepTables.build: free_state must not be this object's own free_state")
-        width = block_table.shape[1]
-        st = lib().seb_step_tables(q_lens.data_ptr(), context_lens.data_ptr(), self.rows, self.tokens,
-                                   block_table.data_ptr(), block_table.stride(0), width, free_ids.data_ptr(),
-                                   free_ids.numel(), free_state.data_ptr(), *self._out,
-                                   ops.err_word(dev).data_ptr(), ops._stream(dev))
-        check("seb_step_tables", st)
-        ops.LAUNCHES[0] += 1
-        ops._after(dev)
+        width = shape[1]
+        st = lib().seb_step_tables(q_lens.data_ptr(), context_lens.data_ptr(), rows, self.tokens,
+                                   block_table.data_ptr(), max(strides[0], width), width, free_ids.data_ptr(),
+                                   free_ids.numel(), free_state.data_ptr(), *self._out, q4._err_ptr(dev),
+                                   q4._raw_stream(dev))
+        q4._done("seb_step_tables", st, dev)
         return {"q_lens": q_lens, "k_lens": self.k_lens, "q_starts": self.q_starts,
                 "q_pos_offsets": self.q_pos_offsets, "block_table": block_table, "block_table_row_stride": width,
                 "total_query": self.tokens}
+
+    def _refuse(self, q_lens, context_lens, block_table, free_ids, free_state):
+        """Says what is wrong with build's arguments."""
+        dev, rows = self.device, self.rows
+        for name, t, shape in (("q_lens", q_lens, (rows,)), ("context_lens", context_lens, (rows,)),
+                               ("free_state", free_state, (2,))):
+            if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous() or t.device != dev:
+                raise ValueError(f"StepTables.build: {name} must be int32 {list(shape)}, contiguous and on {dev}")
+        if (free_ids.dtype != torch.int32 or free_ids.dim() != 1 or free_ids.numel() == 0
+                or not free_ids.is_contiguous() or free_ids.device != dev):
+            raise ValueError(f"StepTables.build: free_ids must be a non-empty int32 vector, contiguous and on {dev}")
+        raise ValueError(f"StepTables.build: block_table must be int32 [{rows}, max_blocks >= 1] on {dev} with unit "
+                         "column stride and rows that do not overlap")
