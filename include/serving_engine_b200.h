@@ -335,7 +335,8 @@ SEB_API int seb_allreduce_add_rmsnorm(void* const* partial, void* const* x, void
 
 /* seb_kv_append for a 4-bit pool: quantises k_new and v_new (bf16 or fp16) into the
  * tokens' slots. Values beyond +-65504 are clamped; a group that holds an infinity or
- * a NaN reads back as NaN. Out-of-range slots set SEB_ERRBIT_SLOT and are skipped. */
+ * a NaN reads back as NaN. Slot -1 is a token of no row (seb_step_tables) and is
+ * skipped; other slots out of range set SEB_ERRBIT_SLOT and are skipped. */
 SEB_API int seb_kv_append_q4(const void* k_new, int64_t k_stride_token, int64_t k_stride_head,
                              const void* v_new, int64_t v_stride_token, int64_t v_stride_head,
                              int64_t n_tokens, const int64_t* slot_mapping, void* k_cache, void* v_cache,
@@ -343,8 +344,8 @@ SEB_API int seb_kv_append_q4(const void* k_new, int64_t k_stride_token, int64_t 
                              int32_t* err, void* stream);
 
 /* The values of the given slots: k_out, v_out [n_tokens, num_kv_heads, head_dim] of
- * any element type, contiguous and 16-byte aligned. An out-of-range slot sets
- * SEB_ERRBIT_SLOT and gives zeros. */
+ * any element type, contiguous and 16-byte aligned. Slot -1 gives zeros; another slot
+ * out of range does too and sets SEB_ERRBIT_SLOT. */
 SEB_API int seb_kv_gather_q4(const void* k_cache, const void* v_cache, int64_t num_blocks,
                              int32_t num_kv_heads, int32_t head_dim, const int64_t* slots, int64_t n_tokens,
                              void* k_out, void* v_out, int32_t dtype, int32_t* err, void* stream);
@@ -354,7 +355,8 @@ SEB_API int seb_kv_gather_q4(const void* k_cache, const void* v_cache, int64_t n
  * then y * cos + rotate_half(y) * sin, all in fp32 and rounded once to the element
  * type. q_weight, k_weight: [head_dim], either may be NULL (that kind of head is not
  * normed). cache_bits: 16 (a pool of the element type, as seb_kv_append) or 4 (a 4-bit
- * pool; keys are rounded to the element type, then quantised). */
+ * pool; keys are rounded to the element type, then quantised). Slots as in
+ * seb_kv_append_q4; a skipped token's queries are written all the same. */
 SEB_API int seb_qk_norm_rope_append(const void* qkv, int64_t qkv_stride_token, int64_t n_tokens,
                                     int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim, const void* cos,
                                     const void* sin, int64_t cos_sin_stride_token, const void* q_weight,

@@ -12,12 +12,17 @@
 //
 // Bound: HBM. Every input is read once and every output written once; head_dim / 16
 // threads hold a head as two 16-byte vectors each, one from each half, so that the
-// rotation needs no exchange and a group's extremes three shuffles.
+// rotation needs no exchange and a group's extremes three shuffles. 8192 tokens, 32/8
+// heads of 128 into the 4-bit pool: 41 us, 4.4 TB/s (two and four heads to a thread, which
+// load the token's cos and sin once, took 56 and 71 us: fewer threads fit an SM).
 #include "q4_format.cuh"
 #include "seb_vec.cuh"
 
 namespace seb {
 namespace {
+
+// 8192 tokens, 32/8 heads of 128: 41.3 us at 128 threads, 44.0 at 256.
+constexpr int kAppendThreads = 128;
 
 struct QkvParams {
   const char* qkv;
@@ -34,7 +39,7 @@ struct QkvParams {
   int64_t q_st;
   char* k_cache;
   char* v_cache;
-  int64_t units;
+  uint32_t units;
   int32_t hq, hkv;
   int32_t* err;
 };
@@ -48,7 +53,7 @@ struct KvParams {
   int64_t num_slots;
   char* k_cache;
   char* v_cache;
-  int64_t units;
+  uint32_t units;
   int32_t hkv;
   int32_t* err;
 };
@@ -128,15 +133,15 @@ __device__ __forceinline__ void quantise_row(const Vec8<T>& a, const Vec8<T>& b,
 
 // D / 16 lanes per (token, head): heads [0, hq) are queries, [hq, hq + hkv) keys, the rest values.
 template <typename T, int D, bool POOL4, bool VEC>
-__global__ void __launch_bounds__(256) qk_norm_rope_append_kernel(QkvParams p) {
+__global__ void __launch_bounds__(kAppendThreads) qk_norm_rope_append_kernel(QkvParams p) {
   constexpr int kLanes = D / 16;
-  const int64_t u = (int64_t)blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
+  const uint32_t u = blockIdx.x * (kAppendThreads / kLanes) + threadIdx.x / kLanes;
   if (u >= p.units) return;
   const int sub = threadIdx.x % kLanes;
   const unsigned mask = (unsigned)(((1ull << kLanes) - 1) << (threadIdx.x % 32 / kLanes * kLanes));
-  const int heads = p.hq + 2 * p.hkv;
-  const int64_t t = u / heads;
-  const int h = (int)(u - t * heads);
+  const uint32_t heads = p.hq + 2 * p.hkv, tok = u / heads;
+  const int64_t t = tok;
+  const int h = (int)(u - tok * heads);
   const int i = 8 * sub;
   const T* src = reinterpret_cast<const T*>(p.qkv) + t * p.qkv_st + (int64_t)h * D;
   Vec8<T> a = load8<T, VEC>(src + i), b = load8<T, VEC>(src + D / 2 + i);
@@ -182,7 +187,7 @@ __global__ void __launch_bounds__(256) qk_norm_rope_append_kernel(QkvParams p) {
   }
   const int64_t slot = __ldg(p.slots + t);
   if (slot < 0 || slot >= p.num_slots) {
-    if (h == p.hq && sub == 0) atomic_or_err(p.err, SEB_ERRBIT_SLOT);
+    if (slot != -1 && h == p.hq && sub == 0) atomic_or_err(p.err, SEB_ERRBIT_SLOT);
     return;
   }
   const bool is_v = h >= p.hq + p.hkv;
@@ -204,15 +209,16 @@ __global__ void __launch_bounds__(256) qk_norm_rope_append_kernel(QkvParams p) {
 template <typename T, int D, bool VEC>
 __global__ void __launch_bounds__(256) kv_append_q4_kernel(KvParams p) {
   constexpr int kLanes = D / 16;
-  const int64_t u = (int64_t)blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
+  const uint32_t u = blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
   if (u >= p.units) return;
   const int sub = threadIdx.x % kLanes;
   const unsigned mask = (unsigned)(((1ull << kLanes) - 1) << (threadIdx.x % 32 / kLanes * kLanes));
-  const int64_t t = u / (2 * p.hkv);
-  const int h = (int)(u - t * 2 * p.hkv);
+  const uint32_t tok = u / (2 * p.hkv);
+  const int64_t t = tok;
+  const int h = (int)(u - tok * 2 * p.hkv);
   const int64_t slot = __ldg(p.slots + t);
   if (slot < 0 || slot >= p.num_slots) {
-    if (h == 0 && sub == 0) atomic_or_err(p.err, SEB_ERRBIT_SLOT);
+    if (slot != -1 && h == 0 && sub == 0) atomic_or_err(p.err, SEB_ERRBIT_SLOT);
     return;
   }
   const bool is_v = h >= p.hkv;
@@ -227,70 +233,94 @@ __global__ void __launch_bounds__(256) kv_append_q4_kernel(KvParams p) {
   else quantise_row<T, D, false>(a, b, i, row, r, mask);
 }
 
-// One thread per (token, plane, kv head, 8 dims): the values that the pool's slots stand for.
+// The values that the pool's slots stand for: 4 threads per (token, plane, kv head), each with
+// 16 dims of every group of a panel, as K's chunks have them (V: two neighbouring chunks).
 template <typename T, int D>
 __global__ void __launch_bounds__(256) kv_gather_q4_kernel(const char* k_cache, const char* v_cache, int64_t num_slots,
-                                                           const int64_t* slots, int64_t n_tokens, int hkv, T* k_out,
+                                                           const int64_t* slots, uint32_t units, int hkv, T* k_out,
                                                            T* v_out, int32_t* err) {
   using L = q4::Layout<D>;
-  constexpr int kChunks = D / 8;
-  const int64_t g = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t per_token = 2 * (int64_t)hkv * kChunks;
-  const int64_t t = g / per_token;
-  if (t >= n_tokens) return;
-  const int rest = (int)(g - t * per_token);
-  const int dim = rest % kChunks * 8;
-  const int h = rest / kChunks;
+  constexpr int G = L::kGroups;
+  const uint32_t u = blockIdx.x * 64 + threadIdx.x / 4;
+  if (u >= units) return;
+  const int c = threadIdx.x & 3;
+  const uint32_t tok = u / (2 * hkv);
+  const int64_t t = tok;
+  const int h = (int)(u - tok * 2 * hkv);
   const bool is_v = h >= hkv;
   const int kvh = h - (is_v ? hkv : 0);
-  T* dst = (is_v ? v_out : k_out) + (t * hkv + kvh) * D + dim;
+  T* dst = (is_v ? v_out : k_out) + (t * hkv + kvh) * D + 16 * c;
   const int64_t slot = __ldg(slots + t);
-  float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (slot >= 0 && slot < num_slots) {
-    const char* row = (is_v ? v_cache : k_cache) + (slot / kBlockSize * hkv + kvh) * (int64_t)L::kRow;
-    const int r = (int)(slot % kBlockSize);
-    const __half2 p = *reinterpret_cast<const __half2*>(row + L::pair(r, dim));
-    const float scale = __low2float(p), low = __high2float(p);
+  const bool ok = slot >= 0 && slot < num_slots;
+  if (!ok && slot != -1 && h == 0 && c == 0) atomic_or_err(err, SEB_ERRBIT_SLOT);
+  const char* row = (is_v ? v_cache : k_cache) + ((ok ? slot : 0) / kBlockSize * hkv + kvh) * (int64_t)L::kRow;
+  const int r = (int)(slot & (kBlockSize - 1));
+#pragma unroll
+  for (int pn = 0; pn < L::kPanels; ++pn) {
+    // words: K's [group][8 dims], each dims 0 2 4 6 1 3 5 7; V's [chunk][group][4 dims], both tokens of a pair
+    __align__(16) uint32_t w[4 * G];
+    __half2 pr[G];
+    const char* codes = row + pn * 8 * L::kWidth;
     if (is_v) {
-      const char* at = row + L::v_half(r, dim);
-      const uint32_t n0 = *reinterpret_cast<const uint16_t*>(at), n1 = *reinterpret_cast<const uint16_t*>(at + 4);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = q4::value_of(q4::v_code(e < 4 ? n0 : n1, e & 3), scale, low);
+      for (int k = 0; k < 2; ++k) {
+        const char* at = codes + (r >> 1) * L::kWidth + ((2 * c + k) ^ L::turn(r >> 1)) * (8 * G);
+        if constexpr (G == 2) *reinterpret_cast<uint4*>(w + 4 * k) = *reinterpret_cast<const uint4*>(at);
+        else *reinterpret_cast<uint2*>(w + 2 * k) = *reinterpret_cast<const uint2*>(at);
+      }
     } else {
-      const uint32_t n = *reinterpret_cast<const uint32_t*>(row + L::k_word(r, dim));
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = q4::value_of(q4::k_code(n, e), scale, low);
+      const char* at = codes + r * (L::kWidth / 2) + c * (8 * G);
+      if constexpr (G == 2) *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(at);
+      else *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(at);
     }
-  } else if (rest == 0) {
-    atomic_or_err(err, SEB_ERRBIT_SLOT);
-  }
-  if constexpr (sizeof(T) == 2) {
-    Vec8<T> o;
+    const char* pairs = row + L::kCodes + pn * 64 * G + r * 4 * G;
+    if constexpr (G == 2) *reinterpret_cast<uint2*>(pr) = *reinterpret_cast<const uint2*>(pairs);
+    else *reinterpret_cast<uint32_t*>(pr) = *reinterpret_cast<const uint32_t*>(pairs);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) o.set(e, x[e]);
-    *reinterpret_cast<uint4*>(dst) = o.raw;
-  } else {
-    *reinterpret_cast<float4*>(dst) = make_float4(x[0], x[1], x[2], x[3]);
-    *reinterpret_cast<float4*>(dst + 4) = make_float4(x[4], x[5], x[6], x[7]);
+    for (int g = 0; g < G; ++g) {
+      const float scale = ok ? __low2float(pr[g]) : 0.f, low = ok ? __high2float(pr[g]) : 0.f;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {  // 8 dims
+        float x[8];
+        if (is_v) {
+          const uint32_t lo = w[k * 2 * G + 2 * g] >> (16 * (r & 1)), hi = w[k * 2 * G + 2 * g + 1] >> (16 * (r & 1));
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = q4::value_of(q4::v_code(e < 4 ? lo : hi, e & 3), scale, low);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = q4::value_of(q4::k_code(w[2 * g + k], e), scale, low);
+        }
+        T* out = dst + pn * L::kWidth + g * q4::kGroup + 8 * k;
+        if constexpr (sizeof(T) == 2) {
+          Vec8<T> o;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) o.set(e, x[e]);
+          *reinterpret_cast<uint4*>(out) = o.raw;
+        } else {
+          *reinterpret_cast<float4*>(out) = make_float4(x[0], x[1], x[2], x[3]);
+          *reinterpret_cast<float4*>(out + 4) = make_float4(x[4], x[5], x[6], x[7]);
+        }
+      }
+    }
   }
 }
 
-int blocks_for(int64_t units, int per_block, const char* what, unsigned* grid) {
-  const int64_t n = (units + per_block - 1) / per_block;
-  SEB_CHECK_ARG(n < (1ll << 31), "%s: too many tokens", what);
-  *grid = (unsigned)n;
+unsigned blocks_for(uint32_t units, int per_block) { return (unsigned)(((int64_t)units + per_block - 1) / per_block); }
+
+// Heads of all tokens, which the kernels count in 32 bits; past that, an error.
+int units_of(int64_t n_tokens, int64_t heads, const char* what, uint32_t* units) {
+  SEB_CHECK_ARG(n_tokens <= (int64_t)0x7fffffff / heads, "%s: too many tokens", what);
+  *units = (uint32_t)(n_tokens * heads);
   return SEB_OK;
 }
 
 template <typename T, int D>
 int launch_qkv(const QkvParams& p, bool pool4, bool vec, cudaStream_t s) {
-  unsigned grid;
-  const int rc = blocks_for(p.units, 256 / (D / 16), "seb_qk_norm_rope_append", &grid);
-  if (rc != SEB_OK) return rc;
-  if (pool4 && vec) qk_norm_rope_append_kernel<T, D, true, true><<<grid, 256, 0, s>>>(p);
-  else if (pool4) qk_norm_rope_append_kernel<T, D, true, false><<<grid, 256, 0, s>>>(p);
-  else if (vec) qk_norm_rope_append_kernel<T, D, false, true><<<grid, 256, 0, s>>>(p);
-  else qk_norm_rope_append_kernel<T, D, false, false><<<grid, 256, 0, s>>>(p);
+  const unsigned grid = blocks_for(p.units, kAppendThreads / (D / 16));
+  if (pool4 && vec) qk_norm_rope_append_kernel<T, D, true, true><<<grid, kAppendThreads, 0, s>>>(p);
+  else if (pool4) qk_norm_rope_append_kernel<T, D, true, false><<<grid, kAppendThreads, 0, s>>>(p);
+  else if (vec) qk_norm_rope_append_kernel<T, D, false, true><<<grid, kAppendThreads, 0, s>>>(p);
+  else qk_norm_rope_append_kernel<T, D, false, false><<<grid, kAppendThreads, 0, s>>>(p);
   return launch_status("qk_norm_rope_append_kernel");
 }
 
@@ -302,9 +332,7 @@ int launch_qkv_dim(const QkvParams& p, int d, bool pool4, bool vec, cudaStream_t
 
 template <typename T, int D>
 int launch_kv(const KvParams& p, bool vec, cudaStream_t s) {
-  unsigned grid;
-  const int rc = blocks_for(p.units, 256 / (D / 16), "seb_kv_append_q4", &grid);
-  if (rc != SEB_OK) return rc;
+  const unsigned grid = blocks_for(p.units, 256 / (D / 16));
   if (vec) kv_append_q4_kernel<T, D, true><<<grid, 256, 0, s>>>(p);
   else kv_append_q4_kernel<T, D, false><<<grid, 256, 0, s>>>(p);
   return launch_status("kv_append_q4_kernel");
@@ -362,7 +390,8 @@ extern "C" int seb_qk_norm_rope_append(const void* qkv, int64_t qkv_stride_token
   p.q_st = q_out_stride_token;
   p.k_cache = static_cast<char*>(k_cache);
   p.v_cache = static_cast<char*>(v_cache);
-  p.units = n_tokens * (num_q_heads + 2 * (int64_t)num_kv_heads);
+  const int rc = units_of(n_tokens, num_q_heads + 2 * (int64_t)num_kv_heads, "seb_qk_norm_rope_append", &p.units);
+  if (rc != SEB_OK) return rc;
   p.hq = num_q_heads;
   p.hkv = num_kv_heads;
   p.err = err;
@@ -401,7 +430,8 @@ extern "C" int seb_kv_append_q4(const void* k_new, int64_t k_stride_token, int64
   p.num_slots = num_blocks * kBlockSize;
   p.k_cache = static_cast<char*>(k_cache);
   p.v_cache = static_cast<char*>(v_cache);
-  p.units = n_tokens * 2 * num_kv_heads;
+  const int rc = units_of(n_tokens, 2 * (int64_t)num_kv_heads, "seb_kv_append_q4", &p.units);
+  if (rc != SEB_OK) return rc;
   p.hkv = num_kv_heads;
   p.err = err;
   const bool vec = aligned(k_new, 16) && aligned(v_new, 16) && k_stride_token % 8 == 0 && k_stride_head % 8 == 0 &&
@@ -417,16 +447,17 @@ namespace {
 template <typename T>
 int launch_gather(const void* k, const void* v, int64_t num_slots, const int64_t* slots, int64_t n, int hkv, int d,
                   void* k_out, void* v_out, int32_t* err, cudaStream_t s) {
-  unsigned grid;
-  const int rc = blocks_for(n * 2 * hkv * (d / 8), 256, "seb_kv_gather_q4", &grid);
+  uint32_t units;
+  const int rc = units_of(n, 2 * (int64_t)hkv, "seb_kv_gather_q4", &units);
   if (rc != SEB_OK) return rc;
+  const unsigned grid = blocks_for(units, 64);
   const char* kc = static_cast<const char*>(k);
   const char* vc = static_cast<const char*>(v);
   T* ko = static_cast<T*>(k_out);
   T* vo = static_cast<T*>(v_out);
-  if (d == 64) kv_gather_q4_kernel<T, 64><<<grid, 256, 0, s>>>(kc, vc, num_slots, slots, n, hkv, ko, vo, err);
-  else if (d == 128) kv_gather_q4_kernel<T, 128><<<grid, 256, 0, s>>>(kc, vc, num_slots, slots, n, hkv, ko, vo, err);
-  else kv_gather_q4_kernel<T, 256><<<grid, 256, 0, s>>>(kc, vc, num_slots, slots, n, hkv, ko, vo, err);
+  if (d == 64) kv_gather_q4_kernel<T, 64><<<grid, 256, 0, s>>>(kc, vc, num_slots, slots, units, hkv, ko, vo, err);
+  else if (d == 128) kv_gather_q4_kernel<T, 128><<<grid, 256, 0, s>>>(kc, vc, num_slots, slots, units, hkv, ko, vo, err);
+  else kv_gather_q4_kernel<T, 256><<<grid, 256, 0, s>>>(kc, vc, num_slots, slots, units, hkv, ko, vo, err);
   return launch_status("kv_gather_q4_kernel");
 }
 
