@@ -12,8 +12,9 @@ Public API mirrors the reference's hot-path modules:
   decoder;
 * a KV pool held in 4 bits: ``new_q4_pool``, ``kv_append_q4``, ``kv_gather_q4``,
   ``qk_norm_rope_append`` (head norms, rotary embedding and the write to a 4-bit or
-  16-bit pool), ``paged_attention_q4`` (``paged_flash_attention`` and ``PagedKVCache``
-  take such a pool as well), and ``StepTables``, a step's tables built on the GPU.
+  16-bit pool), ``paged_attention_q4`` (``paged_flash_attention``, ``PagedKVCache`` and
+  the registered attention function take such a pool as well), and ``StepTables``, a
+  step's tables built on the GPU; ``q4_serve.Q4Batch`` runs a model with all of them.
 
 Importing the package does not load the CUDA library; the first op does, and
 raises if it has not been built (``python -m serving_engine_b200.build``).

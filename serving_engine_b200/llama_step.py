@@ -14,6 +14,9 @@ twenty kernels per layer, most of them elementwise passes over the step's tokens
   paged attention (decode rows on the split-K kernel, prefill rows on tcgen05),
   o_proj, add_rmsnorm, one GEMM for gate/up (concatenated), swiglu, down_proj,
 
+(over a pool held in 4 bits, and for models that norm their query and key heads, the
+embedding and the write are qk_norm_rope_append, which norms in the same pass),
+
 then the final norm and lm_head on each row's last token only. Every kernel works
 row by row, so one step may mix prefill chunks and decode rows. Rotary embedding
 is bit-identical to HF's; RMSNorm and SiLU * up are computed in fp32 and rounded
@@ -26,6 +29,7 @@ import torch
 
 from . import ops
 from .paged_attention import paged_flash_attention
+from .q4 import qk_norm_rope_append
 
 
 class FusedLlamaStep:
@@ -66,6 +70,9 @@ class FusedLlamaStep:
                     "wd": mlp.down_proj.weight,
                     "n1": layer.input_layernorm.weight,
                     "n2": layer.post_attention_layernorm.weight,
+                    # norms of query and key heads, [head_dim], where the model has them
+                    "qn": getattr(getattr(at, "q_norm", None), "weight", None),
+                    "kn": getattr(getattr(at, "k_norm", None), "weight", None),
                 })
 
     def rotary(self, positions: torch.Tensor):
@@ -79,8 +86,8 @@ class FusedLlamaStep:
     def logits(self, tokens: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor, kv_cache: torch.Tensor,
                metadata: dict, last: torch.Tensor | None = None) -> torch.Tensor:
         """tokens, positions, slots: [n_tokens] int64, the step's flattened tokens;
-        kv_cache: [layers, 2, num_blocks, 16, kv heads, head_dim]; metadata: the
-        step's paged metadata; last: the index of each row's last token (default:
+        kv_cache: [layers, 2, num_blocks, 16, kv heads, head_dim], or a 4-bit pool
+        (q4.new_q4_pool); metadata: the step's paged metadata; last: the index of each row's last token (default:
         every token is a row's last, as in a decode step). Returns the logits of
         those tokens [rows, vocab]."""
         b = tokens.shape[0]
@@ -90,7 +97,10 @@ class FusedLlamaStep:
         for li, w in enumerate(self.layers):
             qkv = h @ w["wqkv"].t()
             kc, vc = kv_cache[li, 0], kv_cache[li, 1]
-            q = ops.rope_kv_append(qkv, cos, sin, slots, kc, vc, self.hq, self.hkv)
+            if kv_cache.dtype == torch.uint8 or w["qn"] is not None or w["kn"] is not None:
+                q = qk_norm_rope_append(qkv, cos, sin, slots, kc, vc, self.hq, self.hkv, w["qn"], w["kn"], self.eps)
+            else:
+                q = ops.rope_kv_append(qkv, cos, sin, slots, kc, vc, self.hq, self.hkv)
             o, _ = paged_flash_attention(q, kc, vc, metadata, self.hq, self.hkv, self.scale)
             a = o.view(b, self.hq * self.head_dim) @ w["wo"].t()
             h = ops.add_rmsnorm(x, a, w["n2"], self.eps)

@@ -162,13 +162,15 @@ def kv_append(k_new: torch.Tensor, v_new: torch.Tensor, k_cache: torch.Tensor, v
 @_nvtx
 def copy_blocks(kv_cache: torch.Tensor, src, dst) -> None:
     """kv_cache[:, :, dst] = kv_cache[:, :, src] for the engine pool
-    [L, 2, num_blocks, 16, H, D] (model_runner.py:101-110), one launch.
+    [L, 2, num_blocks, 16, H, D] (model_runner.py:101-110) or a 4-bit pool
+    [L, 2, num_blocks, H, 9 * D] of uint8 (q4.new_q4_pool), one launch.
 
     src/dst: sequences of block ids or int64 tensors. dst ids must be distinct
     and disjoint from src ids; host lists are validated here.
     """
     dev = _require_cuda("copy_blocks", kv_cache)
-    if kv_cache.dim() != 6 or kv_cache.shape[1] != 2 or kv_cache.shape[3] != BLOCK_SIZE:
+    q4_pool = kv_cache.dim() == 5 and kv_cache.dtype == torch.uint8
+    if kv_cache.dim() != (5 if q4_pool else 6) or kv_cache.shape[1] != 2 or not (q4_pool or kv_cache.shape[3] == BLOCK_SIZE):
         raise ValueError(f"copy_blocks: pool must be [L, 2, num_blocks, {BLOCK_SIZE}, H, D], got {tuple(kv_cache.shape)}")
     if not kv_cache.is_contiguous():
         raise ValueError("copy_blocks: pool must be contiguous")
@@ -188,7 +190,7 @@ def copy_blocks(kv_cache: torch.Tensor, src, dst) -> None:
     n = src_t.numel()
     if n == 0:
         return
-    block_bytes = BLOCK_SIZE * kv_cache.shape[4] * kv_cache.shape[5] * kv_cache.element_size()
+    block_bytes = kv_cache.stride(2) * kv_cache.element_size()
     layer_stride = kv_cache.stride(0) * kv_cache.element_size()
     st = lib().seb_copy_blocks(kv_cache.data_ptr(), kv_cache.shape[0], layer_stride, nb, block_bytes,
                                src_t.data_ptr(), dst_t.data_ptr(), n, err_word(dev).data_ptr(), _stream(dev))
