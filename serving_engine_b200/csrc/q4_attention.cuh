@@ -36,7 +36,9 @@ struct Q4Params {
   float* lse;
   int64_t lse_st;
   int32_t counter_slot;
-  float* ws;  // [CTA][2] parts: [columns][D], then [columns][2]
+  float* ws;           // what CTAs leave of units that others share; each kernel has its own layout
+  int32_t* chunk_arrivals;  // [kChunkArrivals], zeroed by the kernel for the other rows, which runs first
+  uint32_t cut_below;       // chunks: fewer units than this are cut between CTAs
   int32_t* err;
 };
 
@@ -95,7 +97,11 @@ __device__ __forceinline__ int query_exponent(float top) {
   return top > 0.f ? min(max(exponent(top) - 14, -100), 112) : 0;
 }
 
-// The kernel for chunks (q4_prefill.cu); p is complete but for its tile and workspace.
+// The kernel for chunks (q4_prefill.cu); p is complete but for its tile and cut_below, and p.ws
+// has room for as many bytes as the second says, the arrivals behind them.
+constexpr int kMaxChunkCtas = 256;
+constexpr int kChunkArrivals = kMaxChunkCtas * 8;
 int launch_q4_prefill(const Q4Params& p, int head_dim, int dtype, cudaStream_t s);
+int64_t q4_prefill_workspace(int head_dim);
 
 }  // namespace seb

@@ -10,7 +10,8 @@
 //   warps 12-15 V's;
 //   warp 16     owns TMEM and issues S(t) = Q(t) K^T and O(t) += P(t) V, tile t's while the
 //               other tile's softmax runs;
-//   warp 17     copies the pool's rows of the next blocks to shared memory.
+//   warp 17     copies the pool's rows of the next blocks to shared memory;
+//   warp 18     finds the CTA's next units, or pieces of them, and says what they are.
 // K is stored by keys, V by dims (V^T): both K-major, and both as the pool has them, so a
 // word of 8 codes becomes one 16-byte store (V: of 4 pairs of tokens, 4 such stores).
 // Registers are split between the roles (setmaxnreg); none may spill, with shared memory
@@ -44,7 +45,8 @@ constexpr int kRows = 128;     // rows of a query tile
 constexpr int kTiles = 2;      // query tiles of a unit
 constexpr int kStages = 2;     // K tiles, and V tiles, in shared memory
 constexpr int kRawStages = 3;  // the pool's rows of K(0), V(0), K(1), ... before they are decoded
-constexpr int kThreads = 640;  // 5 warpgroups; the last has the MMA warp, the copying one and 2 that idle
+constexpr int kThreads = 640;  // 5 warpgroups; the last has the MMA warp, the copying one, the one that plans, an idle one
+constexpr int kPieces = 4;     // places for what the planning warp says of pieces
 constexpr int kTmemCols = 512;
 constexpr int kColO = 256;     // S of tile t at 128 t (P over its first 64 columns), O at 256 + t * D
 constexpr float kLazy = 8.f;   // scores may exceed the reference by 2^8 before it is moved
@@ -61,9 +63,11 @@ struct Smem {
   static constexpr int kRaw = 8 * kRawRow;                  // K or V rows of a tile's 8 blocks
   static constexpr int oRaw = oV + kStages * kTile;
   static constexpr int oBar = oRaw + kRawStages * kRaw;
-  static constexpr int oInfo = oBar + 256;                  // TileInfo [4]
-  static constexpr int oPrefix = oInfo + 4 * 16;            // uint32 [kThreads + 1]
-  static constexpr int kBytes = oPrefix + (kThreads + 1) * 4;
+  static constexpr int oInfo = oBar + 384;                  // TileInfo [4]
+  static constexpr int oPieces = oInfo + 4 * 16;            // Unit [kPieces], 96 bytes each
+  static constexpr int oPrefix = oPieces + kPieces * 96;    // uint32 [kThreads + 1]
+  static constexpr int oMl = (oPrefix + (kThreads + 1) * 4 + 7) / 8 * 8;  // float2 [2][kRows]
+  static constexpr int kBytes = oMl + 2 * kRows * 8;
 };
 
 enum {
@@ -77,19 +81,29 @@ enum {
   kBarODone = kBarPFull + kTiles,     // + tile: the unit's last PV complete
   kBarRawFull = kBarODone + kTiles,   // + stage: rows have come
   kBarRawEmpty = kBarRawFull + kRawStages,  // + stage: the 256 threads that decode are done with them
-  kBarFinal = kBarRawEmpty + kRawStages,
+  kBarMerge = kBarRawEmpty + kRawStages,  // both warpgroups have come to this point of a unit that they share
+  kBarPieceFull,                            // + place: a piece, or the end, is described there
+  kBarPieceEmpty = kBarPieceFull + kPieces,  // + place: the copying, the MMA and the 8 softmax warps are done with it
+  kBarFinal = kBarPieceEmpty + kPieces,
   kNumBars = kBarFinal + 1
 };
-static_assert(kNumBars * 8 + 8 <= 256, "barrier region");
+static_assert(kNumBars * 8 + 8 <= 384, "barrier region");
 
-// A unit as every role sees it.
+// A unit, or a CTA's piece of it, as every role sees it.
 struct Unit {
-  int row, kvh, k_len, q_len;
+  int row;             // -1: there are no more
+  int kvh, k_len, q_len;
   int64_t token;       // the first of the unit's tokens
   int tok0;            // and its place in the row
   int sees;            // keys that it sees; each later token sees one more (causal)
   int nblk, ntiles;    // blocks that some token sees, and tiles of 128 keys
   int tiles;           // query tiles, 1 or 2
+  int j0, n;           // the piece: n key tiles from j0 on
+  int tile0;           // key tiles of the CTA's pieces before it
+  int slots;           // warpgroups that have some of it
+  bool twin;           // one query tile, whose key tiles the two warpgroups take in turn
+  bool start;          // the piece is the unit's first
+  uint32_t first, last;  // CTAs with key tiles of the unit (0, 0 where units are not cut)
   bool split;          // K in two parts: a tile of keys takes two places of the ring
 };
 
@@ -104,47 +118,105 @@ constexpr int kSplit = 1;  // K in two parts
 constexpr int kDiag = 2;   // some token does not see all of it: there a NaN must not meet a weight of zero
 constexpr int kEnd = 4;
 
-__device__ __forceinline__ uint32_t units_of(const Q4Params& p, const Row& w) {
-  return (uint32_t)((w.q_len + kTiles * p.tile - 1) / (kTiles * p.tile)) * p.hkv;
+// Units are whole where there are at least as many as CTAs (each takes every so manieth).
+// Fewer are laid end to end, kUnitPlaces places for a start and one for each key tile, and
+// cut in equal runs, one for each CTA; what is left of a unit that was cut is joined by
+// the last of its CTAs to come, in order of the parts' places. Measured, whole and cut (bf16,
+// 32/8 heads of 128): 1 row of 512 tokens that sees 32,768 keys 720 and 367 us, 1 of 64 and 131,072
+// keys 2776 and 221; but 4 rows of 512 and 4096 keys (256 units) 206 and 227. A start, with a
+// part's join, costs as much as 10 key tiles (48 rows of drafts: 3 places 205 us, 6 202, 10 196).
+constexpr uint32_t kUnitPlaces = 10;
+constexpr uint32_t kMinPlaces = 20;  // shortest run worth a CTA
+
+__device__ __forceinline__ int pairs_of(const Q4Params& p, const Row& w) {
+  return (w.q_len + kTiles * p.tile - 1) / (kTiles * p.tile);
+}
+// Blocks that some token of a row's pair of query tiles sees.
+__device__ __forceinline__ int blocks_of(const Q4Params& p, const Row& w, int pair) {
+  if (!p.causal) return (w.k_len + 15) >> 4;
+  const int64_t past = (int64_t)w.q_pos + min((pair + 1) * kTiles * p.tile, w.q_len);
+  return (int)((max(min(past, (int64_t)w.k_len), (int64_t)0) + 15) >> 4);
+}
+__device__ __forceinline__ uint32_t places_of(int blocks) { return (uint32_t)((blocks + 7) >> 3) + kUnitPlaces; }
+
+// How all rows are shared out.
+struct Plan {
+  bool cut;            // units are cut
+  uint32_t per;        // places of a CTA's run
+  uint32_t pos, stop;  // the CTA's next unit or place, and where to stop
+};
+__device__ __forceinline__ uint32_t length_of(const Q4Params& p, const Row& w, bool cut) {
+  const int pairs = pairs_of(p, w);
+  if (!cut) return (uint32_t)pairs * p.hkv;
+  uint32_t sum = 0;
+#pragma unroll 1
+  for (int i = 0; i < pairs; ++i) sum += places_of(blocks_of(p, w, i));
+  return sum * p.hkv;
 }
 
-// Unit u of all rows' units end to end; false past the last.
-__device__ __forceinline__ bool find_unit(const Q4Params& p, const uint32_t* prefix, uint32_t u, Unit& w) {
-  if (u >= prefix[kThreads]) return false;
+// The CTA's next unit, or piece of one; false past the last.
+__device__ __forceinline__ bool next_piece(const Q4Params& p, const uint32_t* prefix, Plan& plan, Unit& w) {
+  if (plan.pos >= plan.stop) return false;
   int lo = 0, hi = kThreads - 1;
 #pragma unroll 1
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (prefix[mid] <= u) lo = mid;
+    if (prefix[mid] <= plan.pos) lo = mid;
     else hi = mid - 1;
   }
   const int chunk = (p.num_rows + kThreads - 1) / kThreads;
   int r = lo * chunk;
-  uint32_t off = u - prefix[lo], bad = 0;
+  uint32_t off = plan.pos - prefix[lo], bad = 0;
   Row row = row_of<true>(p, r, &bad);
-  uint32_t len = units_of(p, row);
+  uint32_t len = length_of(p, row, plan.cut);
 #pragma unroll 1
   while (off >= len && r + 1 < p.num_rows) {
     off -= len;
     row = row_of<true>(p, ++r, &bad);
-    len = units_of(p, row);
+    len = length_of(p, row, plan.cut);
   }
   if (off >= len) return false;
-  const int pairs = len / p.hkv;
-  const int pr = pairs - 1 - off / p.hkv;  // a row's last tokens first: they see the most keys
+  int pr = pairs_of(p, row) - 1;  // a row's last tokens first: they see the most keys
+  uint32_t place = 0;
+  if (plan.cut) {
+#pragma unroll 1
+    for (;; --pr) {
+      len = places_of(blocks_of(p, row, pr));
+      if (off < len * p.hkv || pr == 0) break;
+      off -= len * p.hkv;
+    }
+    w.kvh = off / len;
+    place = off - w.kvh * len;
+  } else {
+    pr -= off / p.hkv;
+    w.kvh = off % p.hkv;
+  }
   w.row = r;
-  w.kvh = off % p.hkv;
   w.k_len = row.k_len;
   w.q_len = row.q_len;
   w.tok0 = pr * kTiles * p.tile;
   w.token = (int64_t)row.q_start + w.tok0;
   w.sees = p.causal ? (int)min((int64_t)row.q_pos + w.tok0 + 1, (int64_t)(1 << 30)) : row.k_len;
-  const int toks = min(kTiles * p.tile, row.q_len - w.tok0);
-  w.tiles = toks > p.tile ? 2 : 1;
+  w.tiles = min(kTiles * p.tile, row.q_len - w.tok0) > p.tile ? 2 : 1;
   w.split = w.sees < kSplitBelow;
-  const int any = p.causal ? min(row.k_len, max(w.sees + toks - 1, 0)) : row.k_len;
-  w.nblk = (any + 15) >> 4;
+  w.nblk = blocks_of(p, row, pr);
   w.ntiles = (w.nblk + 7) >> 3;
+  w.start = place == 0;
+  w.first = w.last = 0;
+  if (plan.cut) {
+    const uint32_t n = min(len - place, plan.stop - plan.pos), at = plan.pos - place;
+    w.j0 = max((int)(place - kUnitPlaces), 0);
+    w.n = max((int)(place + n - kUnitPlaces), 0) - w.j0;
+    w.first = (at + kUnitPlaces) / plan.per;
+    w.last = (at + len - 1) / plan.per;
+    plan.pos += n;
+  } else {
+    w.j0 = 0;
+    w.n = w.ntiles;
+    plan.pos += gridDim.x;
+  }
+  w.twin = w.tiles == 1 && w.n > 1;
+  w.slots = w.n == 0 ? 0 : w.twin ? 2 : w.tiles;
   return true;
 }
 
@@ -197,7 +269,7 @@ __device__ __forceinline__ bool elect_one() {
   return yes != 0;
 }
 // of the 96 that a thread has at the launch
-constexpr int kRegsSoftmax = 136, kRegsK = 64, kRegsV = 80, kRegsMma = 64;
+constexpr int kRegsSoftmax = 120, kRegsK = 80, kRegsV = 80, kRegsMma = 80;
 static_assert(2 * kRegsSoftmax + kRegsK + kRegsV + kRegsMma <= 5 * 96, "the roles' registers are those of the launch");
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params p) {
@@ -214,13 +286,19 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sbase + S::oBar + 8 * kNumBars);
   TileInfo* info = reinterpret_cast<TileInfo*>(sbase + S::oInfo);
   uint32_t* prefix = reinterpret_cast<uint32_t*>(sbase + S::oPrefix);
+  Unit* pieces = reinterpret_cast<Unit*>(sbase + S::oPieces);
+  static_assert(sizeof(Unit) <= 96, "room for pieces");
 
-  // ---- the rows' units; errors in rows are reported by the kernel for the other rows
-  {
+  // ---- the rows' units, and where there are few their places; errors in rows are reported by
+  // the kernel for the other rows
+  Plan plan;
+#pragma unroll 1
+  for (int cut = 0; cut < 2; ++cut) {
     const int chunk = (p.num_rows + kThreads - 1) / kThreads;
     uint32_t sum = 0, bad = 0;
 #pragma unroll 1
-    for (int r = tid * chunk; r < min((tid + 1) * chunk, p.num_rows); ++r) sum += units_of(p, row_of<true>(p, r, &bad));
+    for (int r = tid * chunk; r < min((tid + 1) * chunk, p.num_rows); ++r)
+      sum += length_of(p, row_of<true>(p, r, &bad), cut);
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
       const uint32_t o = __shfl_up_sync(kFull, sum, off);
@@ -234,9 +312,16 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
     for (int w = 0; w < warp; ++w) before += prefix[(w + 1) * 32];
     __syncthreads();
     prefix[tid + 1] += before;
+    __syncthreads();
+    const uint32_t total = prefix[kThreads];
+    plan.cut = cut;
+    plan.per = cut ? max((total + gridDim.x - 1) / gridDim.x, kMinPlaces) : 1;
+    plan.pos = blockIdx.x * plan.per;
+    plan.stop = cut ? min(plan.pos + plan.per, total) : total;
+    if (cut || total == 0 || total >= p.cut_below) break;
+    __syncthreads();
   }
-  __syncthreads();
-  if (blockIdx.x >= prefix[kThreads]) return;
+  if (plan.pos >= plan.stop) return;
 
   if (tid == 0) {
     for (int t = 0; t < kTiles; ++t) {
@@ -255,6 +340,11 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
       mbar_init(bar + 8 * (kBarRawFull + s), 1);
       mbar_init(bar + 8 * (kBarRawEmpty + s), 256);
     }
+    for (int s = 0; s < kPieces; ++s) {
+      mbar_init(bar + 8 * (kBarPieceFull + s), 1);
+      mbar_init(bar + 8 * (kBarPieceEmpty + s), 10);
+    }
+    mbar_init(bar + 8 * kBarMerge, 8);
     mbar_init(bar + 8 * kBarFinal, 1);
     fence_mbar_init();
   }
@@ -268,6 +358,16 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
   bool failed = false;
 
+  // The CTA's i-th piece, and word that this warp is done with it.
+  auto piece = [&](int i) -> const Unit* {
+    if (!wait_or_flag(bar + 8 * (kBarPieceFull + i % kPieces), (i / kPieces) & 1, failed)) return nullptr;
+    const Unit* w = pieces + i % kPieces;
+    return w->row < 0 ? nullptr : w;
+  };
+  auto piece_done = [&](int i) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar + 8 * (kBarPieceEmpty + i % kPieces));
+  };
   auto raw_full = [&](int i) {
     return wait_or_flag(bar + 8 * (kBarRawFull + i % kRawStages), (i / kRawStages) & 1, failed);
   };
@@ -337,42 +437,37 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
             *reinterpret_cast<uint4*>(tile + i * 4096 + gi * S::kPanel + (k_at ^ (w << 4))) =
                 make_uint4(v[0], v[1], v[2], v[3]);
           };
-          if (parts == 2) {  // as two fp16 numbers: K rounded, then what that leaves
+          auto all = [&](auto limited) {
+            constexpr bool kLimited = decltype(limited)::value;
 #pragma unroll
-            for (int gi = 0; gi < G; ++gi)
+            for (int gi = 0; gi < G; ++gi) {
+              const __half2 pr = as_half2(kp[gi]);
+              const float2 prf = __half22float2(pr);
 #pragma unroll
               for (int w = 0; w < 2; ++w) {
-                const float2 pr = __half22float2(as_half2(kp[gi]));
                 uint32_t v[4];
+                decode8<kLimited>(kw[2 * gi + w], __low2half2(pr), __high2half2(pr), v);
+                if (part == 1) {  // what that rounding left
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  float x[2];
+                  for (int e = 0; e < 4; ++e) {
+                    const float2 hi = __half22float2(as_half2(v[e]));
+                    float x[2];
 #pragma unroll
-                  for (int h = 0; h < 2; ++h) {
-                    const float y = fmaf((float)q4::k_code(kw[2 * gi + w], 2 * e + h), pr.x, pr.y);
-                    const float top = q4::max_nan(q4::min_nan(y, 65504.f), -65504.f);
-                    x[h] = part ? top - __half2float(__float2half_rn(top)) : top;
+                    for (int h = 0; h < 2; ++h) {  // 2^23 + code, an integer's float without a conversion
+                      const float code = __uint_as_float(q4::k_code(kw[2 * gi + w], 2 * e + h) | 0x4b000000u) - 8388608.f;
+                      x[h] = fmaf(code, prf.x, prf.y);
+                      if (kLimited) x[h] = q4::max_nan(q4::min_nan(x[h], 65504.f), -65504.f);
+                      x[h] -= h ? hi.y : hi.x;
+                    }
+                    v[e] = Mma<__half>::pack(x[0], x[1]);
                   }
-                  v[e] = Mma<__half>::pack(x[0], x[1]);
                 }
                 store(gi, w, v);
               }
-          } else {
-            auto all = [&](auto limited) {
-#pragma unroll
-              for (int gi = 0; gi < G; ++gi) {
-                const __half2 pr = as_half2(kp[gi]);
-#pragma unroll
-                for (int w = 0; w < 2; ++w) {
-                  uint32_t v[4];
-                  decode8<decltype(limited)::value>(kw[2 * gi + w], __low2half2(pr), __high2half2(pr), v);
-                  store(gi, w, v);
-                }
-              }
-            };
-            if (clamp) all(std::true_type{});
-            else all(std::false_type{});
-          }
+            }
+          };
+          if (clamp) all(std::true_type{});
+          else all(std::false_type{});
         }
         k_stored();
         if (part + 1 < parts) {
@@ -455,13 +550,53 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
     }
   } else if (warp >= 16) {
     registers_down<kRegsMma>();
-    if (warp > 17) goto done;
+    if (warp > 18) goto done;
+    if (warp == 18) {
+      // --------------------------------------------------------------- plan
+      int tiles = 0, i = 0;
+#pragma unroll 1
+      for (bool more = true; more && !failed; ++i) {
+        const int s = i % kPieces;
+        Unit w;
+        w.n = 0;
+        more = next_piece(p, prefix, plan, w);
+        if (!more) w.row = -1;
+        w.tile0 = tiles;
+        tiles += w.n;
+        // its queries on their way to L2 meanwhile
+        if (more && w.slots > 0) {
+          const int tokens = min(kTiles * p.tile, w.q_len - w.tok0), lines = D / 64;
+#pragma unroll 1
+          for (int k = lane; k < tokens * p.group * lines; k += 32) {
+            const int line = k % lines, at = k / lines, tk = at / p.group;
+            const T* q = reinterpret_cast<const T*>(p.q) + (w.token + tk) * p.q_st +
+                         (int64_t)(w.kvh * p.group + at - tk * p.group) * p.q_sh + 64 * line;
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(q));
+          }
+        }
+        if (i >= kPieces) {  // a piece may take long: as many waits as its tiles
+          const uint32_t empty = bar + 8 * (kBarPieceEmpty + s), parity = (i / kPieces - 1) & 1;
+          int tries = pieces[s].n + 1;
+          while (tries > 0 && !mbar_wait_bounded(empty, parity)) --tries;
+          if (tries == 0) failed = true;
+          __syncwarp();
+        }
+        if (lane == 0) {
+          pieces[s] = w;
+          mbar_arrive(bar + 8 * (kBarPieceFull + s));
+        }
+      }
+      goto done;
+    }
     if (warp == 17) {
       // -------------------------------------------------------------- copies
       int i = 0, n = 0;  // rows of K and V asked for, and tiles
-      Unit w;
 #pragma unroll 1
-      for (uint32_t u = blockIdx.x; !failed && find_unit(p, prefix, u, w); u += gridDim.x) {
+      for (int ip = 0;; ++ip) {
+        const Unit* at = piece(ip);
+        if (!at) break;
+        const Unit w = *at;
+        piece_done(ip);
         const int32_t* table = p.block_table + (int64_t)w.row * p.bt_stride;
         auto fetch = [&](int b) -> int {
           if (b >= w.nblk) return -1;
@@ -470,14 +605,16 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
           atomic_or_err(p.err, SEB_ERRBIT_BLOCK_ID);
           return -1;
         };
-        int ids = fetch(lane), next = fetch(32 + lane);  // of 32 blocks, and of the 32 after them
+        if (w.n == 0) continue;
+        int ids = fetch(8 * w.j0 + lane), next = fetch(8 * w.j0 + 32 + lane);  // of 32 blocks, and of the 32 after them
 #pragma unroll 1
-        for (int j = 0; j < w.ntiles && !failed; ++j, ++n) {
-          if (j > 0 && (j & 3) == 0) {
+        for (int k = 0; k < w.n && !failed; ++k, ++n) {
+          const int j = w.j0 + k;
+          if (k > 0 && (k & 3) == 0) {
             ids = next;
             next = fetch(8 * j + 32 + lane);
           }
-          const int id = __shfl_sync(kFull, ids, (j & 3) * 8 + (lane & 7));
+          const int id = __shfl_sync(kFull, ids, (k & 3) * 8 + (lane & 7));
           const unsigned have = __ballot_sync(kFull, id >= 0) & 0xffu;
 #pragma unroll 1
           for (int is_v = 0; is_v < 2; ++is_v, ++i) {
@@ -560,29 +697,58 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
     // read P from; one thread issues both, and its MMAs run in order.
     int gk = 0, gv = 0, nu = 0;
     uint32_t pphase = 0;
-    Unit w;
 #pragma unroll 1
-    for (uint32_t u = blockIdx.x; !failed && find_unit(p, prefix, u, w); u += gridDim.x) {
-      if (w.ntiles == 0) continue;
+    for (int ip = 0;; ++ip) {
+      const Unit* at = piece(ip);
+      if (!at) break;
+      const struct {
+        int n, slots;
+        bool twin, split;
+      } w = {at->n, at->slots, at->twin, at->split};
+      piece_done(ip);
       const int parts = w.split ? 2 : 1;
-      {
-        if (!wait_k(gk, parts)) break;
-        for (int t = 0; t < w.tiles && !failed; ++t) {
-          if (!wait_or_flag(bar + 8 * (kBarQFull + t), (nu >> t) & 1, failed)) break;
-          nu ^= 1 << t;
+      for (int t = 0; t < w.slots && !failed; ++t) {
+        if ((t == 0 || w.twin) && !wait_k(gk, parts)) break;
+        if (!wait_or_flag(bar + 8 * (kBarQFull + t), (nu >> t) & 1, failed)) break;
+        nu ^= 1 << t;
+        tc::fence_after_sync();
+        issue_s(t, gk, parts);
+        if (w.twin || t + 1 == w.slots) {
+          release_k(gk, parts);
+          __syncwarp();
+          gk += parts;
+        }
+      }
+      if (w.twin) {  // tile j by warpgroup j & 1, with its O
+#pragma unroll 1
+        for (int j = 0; j < w.n && !failed; ++j, ++gv) {
+          const int sv = gv % kStages, t = j & 1;
+          if (!wait_or_flag(bar + 8 * (kBarVFull + sv), (gv / kStages) & 1, failed)) break;
+          if (!wait_or_flag(bar + 8 * (kBarPFull + t), (pphase >> t) & 1, failed)) break;
+          pphase ^= 1u << t;
+          tc::fence_after_sync();
+          issue_pv(t, sv, j < 2);
+          if (elect_one()) {
+            tc::commit(bar + 8 * (kBarVEmpty + sv));
+            if (j + 2 >= w.n) tc::commit(bar + 8 * (kBarODone + t));
+          }
+          __syncwarp();
+          if (j + 2 >= w.n) continue;
+          if (!wait_k(gk, parts)) break;
           tc::fence_after_sync();
           issue_s(t, gk, parts);
+          release_k(gk, parts);
+          __syncwarp();
+          gk += parts;
         }
-        release_k(gk, parts);
-        __syncwarp();
-        gk += parts;
+        continue;
       }
 #pragma unroll 1
-      for (int j = 0; j < w.ntiles && !failed; ++j) {
+      for (int j = 0; j < w.n && !failed; ++j) {
         const int sv = gv % kStages;
         if (!wait_or_flag(bar + 8 * (kBarVFull + sv), (gv / kStages) & 1, failed)) break;
-        const bool more = j + 1 < w.ntiles;
-        for (int t = 0; t < w.tiles && !failed; ++t) {
+        const bool more = j + 1 < w.n;
+        for (int t = 0; t < w.slots && !failed; ++t) {
           if (!wait_or_flag(bar + 8 * (kBarPFull + t), (pphase >> t) & 1, failed)) break;
           pphase ^= 1u << t;
           tc::fence_after_sync();
@@ -616,17 +782,18 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
     const uint32_t taddr = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t col_s = qt * 128, col_o = kColO + qt * D;
     const int tk = m / p.group, gh = m - tk * p.group;
-    const int tok = qt * p.tile + tk;  // the row's token, of the unit
-    int ns = 0, nd = 0;  // tiles of scores and units done, of this query tile
-    int nt = 0;          // K tiles of all units (the ring's count)
-    auto is_live = [&](const Unit& w) { return tk < p.tile && w.tok0 + tok < w.q_len; };
+    auto tile_of = [&](const Unit& w) { return w.twin ? 0 : qt; };  // the query tile
+    auto token_of = [&](const Unit& w) { return tile_of(w) * p.tile + tk; };  // the row's token, of the unit
+    int ns = 0, nd = 0;  // tiles of scores and pieces done by this warpgroup
+    int nm = 0;          // times that it met the other one
+    auto is_live = [&](const Unit& w) { return tk < p.tile && w.tok0 + token_of(w) < w.q_len; };
     // The row's query to shared memory as fp16 after a power of two; returns what brings its scores to log2 units.
     auto store_query = [&](const Unit& w) -> float {
       using T2 = typename Two<T>::type;
       const bool live = is_live(w);
       __align__(16) T2 q[D / 2];
       T2 most = Two<T>::zero();
-      const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.q) + (w.token + tok) * p.q_st +
+      const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.q) + (w.token + token_of(w)) * p.q_st +
                                                         (int64_t)(w.kvh * p.group + gh) * p.q_sh);
 #pragma unroll
       for (int i = 0; i < D / 8; ++i)
@@ -651,43 +818,47 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
       mbar_arrive(bar + 8 * (kBarQFull + qt));
       return copysignf(fminf(fabsf(p.scale_log2) * power2(ex), FLT_MAX), p.scale_log2);
     };
-    // The CTA's next unit from u on that has this query tile and keys; rows that see nothing are written here.
-    auto next_unit = [&](uint32_t& u, Unit& w) {
+    // The CTA's first piece from the ip-th on that has work for this warpgroup; rows that see nothing are written here.
+    auto next_unit = [&](int& ip) -> const Unit* {
 #pragma unroll 1
-      for (; find_unit(p, prefix, u, w); u += gridDim.x) {
-        if (qt < w.tiles && w.ntiles > 0) return true;
-        if (qt < w.tiles && is_live(w)) {
+      for (;; ++ip) {
+        const Unit* at = piece(ip);
+        if (!at || qt < at->slots) return at;
+        const Unit& w = *at;
+        if (qt < w.tiles && w.ntiles == 0 && w.start && is_live(w)) {
           const int head = w.kvh * p.group + gh;
-          uint4* op = reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) + (w.token + tok) * p.o_st + (int64_t)head * p.o_sh);
+          const int64_t token = w.token + token_of(w);
+          uint4* op = reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) + token * p.o_st + (int64_t)head * p.o_sh);
 #pragma unroll 1
           for (int d = 0; d < D / 8; ++d) op[d] = make_uint4(0u, 0u, 0u, 0u);
-          p.lse[(w.token + tok) * p.lse_st + head] = -INFINITY;
+          p.lse[token * p.lse_st + head] = -INFINITY;
         }
-        nt += w.ntiles;  // of the other query tile alone
+        piece_done(ip);
       }
-      return false;
     };
-    uint32_t u = blockIdx.x;
-    Unit w;
-    bool have = next_unit(u, w);
-    float c_next = have ? store_query(w) : 0.f;
+    int ip = 0, ip_next = 0;
+    const Unit* at = next_unit(ip_next);
+    float c_next = at ? store_query(*at) : 0.f;
 #pragma unroll 1
-    while (have) {
+    while (at) {
+      const Unit& w = *at;
+      ip = ip_next;
       const float c = c_next;
       const bool live = is_live(w);
-      const int first_tile = nt;
-      nt += w.ntiles;
+      const int first_tile = w.tile0 - w.j0;
       const int head = w.kvh * p.group + gh;
-      T* op = reinterpret_cast<T*>(p.out) + (w.token + tok) * p.o_st + (int64_t)head * p.o_sh;
-      float* lp = p.lse + (w.token + tok) * p.lse_st + head;
-      const int vis = !live ? 0 : p.causal ? min(w.k_len, w.sees + tok) : w.k_len;
-      const int all_see = p.causal ? min(w.k_len, w.sees + qt * p.tile) : w.k_len;  // every row of the tile
+      const int64_t token = w.token + token_of(w);
+      const int vis = !live ? 0 : p.causal ? min(w.k_len, w.sees + token_of(w)) : w.k_len;
+      const int all_see = p.causal ? min(w.k_len, w.sees + tile_of(w) * p.tile) : w.k_len;  // every row of the tile
+      const bool twin = w.twin;
+      const int nblk = w.nblk;
       float m_ref = -INFINITY, l = 0.f;
+      const int j_first = w.j0 + (twin ? qt : 0), j_end = w.j0 + w.n, j_step = twin ? 2 : 1;
 #pragma unroll 1
-      for (int j = 0; j < w.ntiles; ++j, ++ns) {
+      for (int j = j_first; j < j_end; j += j_step, ++ns) {
         wait_or_flag(bar + 8 * (kBarSFull + qt), ns & 1, failed);  // and PV(t, j - 1): O is stable
         tc::fence_after_sync();
-        const unsigned holes = info[(first_tile + j) & 3].none & ((1u << min(8, w.nblk - 8 * j)) - 1);
+        const unsigned holes = info[(first_tile + j) & 3].none & ((1u << min(8, nblk - 8 * j)) - 1);
         const bool plain = c > 0.f && (j + 1) * kKeys <= all_see && holes == 0;
         const int lim = vis - j * kKeys;
         const float cm = plain ? c : 1.f;
@@ -771,7 +942,7 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
         }
         sum0 = add2(sum0, sum1);
         l += sum0.x + sum0.y;
-        if (j > 0 && __any_sync(kFull, move)) {
+        if (j > j_first && __any_sync(kFull, move)) {
 #pragma unroll 1
           for (int cc = 0; cc < D / 16; ++cc) {
             float o[16];
@@ -788,31 +959,138 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
         if (lane == 0) mbar_arrive(bar + 8 * (kBarPFull + qt));
       }
       // ---- the next unit's query, so that its first scores come while this one's O is written
-      u += gridDim.x;
-      have = !__any_sync(kFull, failed) && next_unit(u, w);
-      if (have) c_next = store_query(w);
+      ++ip_next;
+      at = __any_sync(kFull, failed) ? nullptr : next_unit(ip_next);
+      if (at) c_next = store_query(*at);
       // ---- O is final
       wait_or_flag(bar + 8 * (kBarODone + qt), nd & 1, failed);
       ++nd;
       tc::fence_after_sync();
       if (__any_sync(kFull, failed)) break;
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll 1
-      for (int cc = 0; cc < D / 32; ++cc) {
-        float o[32];
-        tc::tmem_ld32(taddr + col_o + 32 * cc, o);
+      // Both warpgroups have a sum: they tell each other of their references, and each takes half of
+      // the dims of both.
+      float f0 = 1.f, f1 = 0.f;
+      auto meet = [&]() {
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar + 8 * kBarMerge);
+        wait_or_flag(bar + 8 * kBarMerge, nm & 1, failed);
+        ++nm;
+        tc::fence_after_sync();
+      };
+      if (twin) {
+        float2* ml = reinterpret_cast<float2*>(sbase + S::oMl);
+        ml[qt * kRows + m] = make_float2(m_ref, l);
+        meet();
+        const float2 other = ml[(qt ^ 1) * kRows + m];
+        const float top = fmaxf(m_ref, other.x), ref = top == -INFINITY ? 0.f : top;
+        f0 = fast_exp2(m_ref - ref);
+        f1 = fast_exp2(other.x - ref);
+        l = fmaf(other.y, f1, l * f0);
+        m_ref = top;
+      }
+      const int col_mine = col_o, col_other = kColO + (qt ^ 1) * D;
+      auto take_o = [&](float (&o)[32], int d) {  // dims d .. d + 31 of the sum
+        tc::tmem_ld32(taddr + col_mine + d, o);
         tc::tmem_wait_ld();
-        if (live) {
+        if (twin) {
+          float x[32];
+          tc::tmem_ld32(taddr + col_other + d, x);
+          tc::tmem_wait_ld();
 #pragma unroll
-          for (int v8 = 0; v8 < 4; ++v8) {
-            uint32_t v[4];
+          for (int i = 0; i < 32; ++i) o[i] = fmaf(x[i], f1, o[i] * f0);
+        }
+      };
+      T* op = reinterpret_cast<T*>(p.out) + token * p.o_st + (int64_t)head * p.o_sh;
+      auto write_o = [&](const float (&o)[32], int d, float inv) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = Mma<T>::pack(o[8 * v8 + 2 * e] * inv, o[8 * v8 + 2 * e + 1] * inv);
-            reinterpret_cast<uint4*>(op)[4 * cc + v8] = make_uint4(v[0], v[1], v[2], v[3]);
+        for (int v8 = 0; v8 < 4; ++v8) {
+          uint32_t v[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = Mma<T>::pack(o[8 * v8 + 2 * e] * inv, o[8 * v8 + 2 * e + 1] * inv);
+          *reinterpret_cast<uint4*>(op + d + 8 * v8) = make_uint4(v[0], v[1], v[2], v[3]);
+        }
+      };
+      auto write_lse = [&](float top, float sum) {
+        p.lse[token * p.lse_st + head] = sum == 0.f ? -INFINITY : fmaf(top, kLn2, logf(sum));
+      };
+      const int d0 = twin ? qt * (D / 2) : 0, d1 = twin ? d0 + D / 2 : D;
+      const uint32_t first = w.first, last = w.last;
+      if (first == last) {
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll 1
+        for (int d = d0; d < d1; d += 32) {
+          float o[32];
+          take_o(o, d);
+          if (live) write_o(o, d, inv);
+        }
+        if (live && d0 == 0) write_lse(m_ref, l);
+      } else {
+        // A part: of each row its dims in fours, then (m, l). Units of one query tile have two, of
+        // half the dims each, so that either warpgroup or both can leave them.
+        const bool one = w.tiles == 1;
+        const int width = one ? D / 2 : D;
+        auto part_of = [&](uint32_t cta, int part) {
+          return p.ws + (((int64_t)cta * 2 + (cta == first)) * 2 + part) * (kRows * (D + 2));
+        };
+        const int part0 = one ? d0 / (D / 2) : qt, parts = (d1 - d0) / width;
+#pragma unroll 1
+        for (int d = d0; d < d1; d += 32) {
+          float o[32];
+          take_o(o, d);
+          if (live) {
+            float4* dst = reinterpret_cast<float4*>(part_of(blockIdx.x, part0 + (d - d0) / width)) + m;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              __stcg(dst + ((d - d0) % width / 4 + i) * kRows, make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]));
+          }
+        }
+#pragma unroll 1
+        for (int part = part0; part < part0 + parts; ++part) {
+          if (live) __stcg(reinterpret_cast<float2*>(part_of(blockIdx.x, part) + kRows * D) + m, make_float2(m_ref, l));
+          __threadfence();
+          __syncwarp();
+          int32_t* ctr = p.chunk_arrivals + (first * 2 + part) * 4 + (warp & 3);
+          int arrived = 0;
+          if (lane == 0) arrived = atomicAdd(ctr, 1);
+          arrived = __shfl_sync(kFull, arrived, 0);
+          if (arrived != (int)(last - first)) continue;
+          // the last to come joins the rows of its warp, in order of the parts' places
+          __threadfence();
+          if (!live) continue;
+          float top = -INFINITY;
+#pragma unroll 4
+          for (uint32_t c = first; c <= last; ++c)
+            top = fmaxf(top, __ldcg(reinterpret_cast<const float2*>(part_of(c, part) + kRows * D) + m).x);
+          const float ref = top == -INFINITY ? 0.f : top;
+          const int from = one ? part * width : 0;
+#pragma unroll 1
+          for (int d = 0; d < width; d += 32) {
+            float o[32], sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = 0.f;
+#pragma unroll 1
+            for (uint32_t c = first; c <= last; ++c) {
+              const float* src = part_of(c, part);
+              const float2 ml = __ldcg(reinterpret_cast<const float2*>(src + kRows * D) + m);
+              const float weight = fast_exp2(ml.x - ref);
+              sum = fmaf(ml.y, weight, sum);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const float4 x = __ldcg(reinterpret_cast<const float4*>(src) + (d / 4 + i) * kRows + m);
+                o[4 * i] = fmaf(x.x, weight, o[4 * i]);
+                o[4 * i + 1] = fmaf(x.y, weight, o[4 * i + 1]);
+                o[4 * i + 2] = fmaf(x.z, weight, o[4 * i + 2]);
+                o[4 * i + 3] = fmaf(x.w, weight, o[4 * i + 3]);
+              }
+            }
+            write_o(o, from + d, sum == 0.f ? 0.f : 1.f / sum);
+            if (from + d == 0) write_lse(top, sum);
           }
         }
       }
-      if (live) *lp = l == 0.f ? -INFINITY : fmaf(m_ref, kLn2, logf(l));
+      if (twin) meet();  // the other's O has been read
+      piece_done(ip);
       tc::fence_before_sync();  // the next unit's first PV overwrites O
     }
   }
@@ -827,16 +1105,23 @@ done:
   }
 }
 
+int ctas_of() { return std::min(num_sms(), kMaxChunkCtas); }
+
 template <typename T, int D>
 int launch(Q4Params p, cudaStream_t s) {
   constexpr auto kern = q4_prefill_kernel<T, D>;
   constexpr int smem = Smem<D>::kBytes + 1024;
+  static_assert(smem <= 227 * 1024, "shared memory of an SM");
   const int rc = set_smem_limit_once<kern>(smem);
   if (rc != SEB_OK) return rc;
   p.tile = kRows / p.group;
-  // no more CTAs than the tokens' units: at most one for each row and kv head beyond the full ones
+  // no more CTAs than the tokens' units have key tiles; units: at most one for each row and kv head beyond the full ones
   const int64_t units = ((int64_t)p.total_query / (kTiles * p.tile) + p.num_rows) * p.hkv;
-  kern<<<(unsigned)std::min<int64_t>(num_sms(), units), kThreads, smem, s>>>(p);
+  const int64_t places = (p.max_blocks + 7) / 8 + kUnitPlaces;
+  const int64_t grid = std::min<int64_t>(ctas_of(), units * places);
+  // places are counted in 32 bits
+  p.cut_below = (uint32_t)std::min<int64_t>(grid, (int64_t)0x7fffffff / places);
+  kern<<<(unsigned)grid, kThreads, smem, s>>>(p);
   return launch_status("q4_prefill_kernel");
 }
 
@@ -847,5 +1132,7 @@ int launch_q4_prefill(const Q4Params& p, int head_dim, int dtype, cudaStream_t s
     return head_dim == 64 ? launch<__nv_bfloat16, 64>(p, s) : launch<__nv_bfloat16, 128>(p, s);
   return head_dim == 64 ? launch<__half, 64>(p, s) : launch<__half, 128>(p, s);
 }
+
+int64_t q4_prefill_workspace(int head_dim) { return ctas_of() * 4ll * kRows * (head_dim + 2) * 4; }
 
 }  // namespace seb
