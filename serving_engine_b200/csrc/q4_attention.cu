@@ -34,8 +34,12 @@
 namespace seb {
 namespace {
 
-constexpr uint32_t kMinRun = 2;          // pairs of blocks of the shortest run worth a warp
-constexpr uint32_t kUnitCost = 2;        // what a unit's start and end cost a warp, in pairs of blocks
+// Pairs of blocks of the shortest run worth a warp. One row of 75 / 200 / 1500 / 6000 keys, 8 kv heads of
+// 128, us: 1: 7.7 / 10.6 / 12.0 / 19.8; 2: 8.9 / 8.6 / 12.9 / 16.0; 4: 15.0 / 16.3 / 15.3 / 16.4.
+constexpr uint32_t kMinRun = 2;
+// What a unit's start and end cost a warp, in pairs of blocks. 256 rows of 32 to 4352 keys, heads of 64:
+// 0: 55.6 us, 1: 49.2, 2: 45.1, 3: 44.8, 4: 44.6, 6: 45.9; 64 rows of 1024 to 8192, heads of 128: 1 84.2, 2 83.6, 3 83.6.
+constexpr uint32_t kUnitCost = 2;
 constexpr float kNoMax = -FLT_MAX;       // no score yet: any score is above it by more than the threshold
 constexpr float kThreshold = 8.f;        // scores may exceed the reference by 2^8 before it is moved
 constexpr float kScaleThreshold = 64.f;  // p * V scale stays below 2^8 * 2^6
@@ -510,7 +514,11 @@ __global__ void __launch_bounds__(NW * 32, CTAS) q4_attention_kernel(const Q4Par
   {
     uint32_t sum = 0, bad = 0;
 #pragma unroll 1
-    for (int r = tid * chunk; r < min((tid + 1) * chunk, p.num_rows); ++r) sum += pairs_of(p, row_of<false>(p, r, &bad));
+    for (int r = tid * chunk; r < min((tid + 1) * chunk, p.num_rows); ++r) {
+      const Row row = row_of<false>(p, r, &bad);
+      sum += pairs_of(p, row);
+      if (r == 0) prefix[NW * 32 + 1] = length_of(row);
+    }
     if (bad && blockIdx.x == 0) atomic_or_err(p.err, bad);
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
@@ -532,11 +540,16 @@ __global__ void __launch_bounds__(NW * 32, CTAS) q4_attention_kernel(const Q4Par
   prefix[tid + 1] += before;
   __syncthreads();
   const uint32_t warps = gridDim.x * NW;
-  const uint32_t per = max((total + warps - 1) / warps, kMinRun), span = NW * per;
+  const uint32_t per = max((total + warps - 1) / warps, kMinRun);
+  uint32_t span = NW * per;
+  // Where CTAs are left over, those of whole units of the first row's length: no unit of that length is
+  // then joined over CTAs (one row of 75 keys, 8 kv heads of 128: 13.0 us with such joins, 9 without).
+  const uint32_t unit0 = prefix[NW * 32 + 1], even = span - span % unit0;
+  if (per == kMinRun && even > 0 && (uint64_t)even * gridDim.x >= total) span = even;
   const uint32_t cta0 = blockIdx.x * span, cta1 = min(cta0 + span, total);
   if (cta0 >= total) return;
   uint32_t pos = cta0 + warp * per;
-  const uint32_t stop = min(pos + per, total);
+  const uint32_t stop = min(pos + per, cta1);
 
   const uint32_t bars = smem_u32(smem + S::kBars) + warp * STAGES * 8;
   char* ring = smem + S::kWarps + warp * S::kWarp;
@@ -660,7 +673,7 @@ __global__ void __launch_bounds__(NW * 32, CTAS) q4_attention_kernel(const Q4Par
         const unsigned none = (unread >> (2 * s)) & 3;
         const char* place = ring + s * S::kStage;
         // two blocks at once where the tile leaves registers for it
-        constexpr int KB = GR * NT <= 1 ? 2 : 1;
+        constexpr int KB = GR * NT <= 2 ? 2 : 1;
         if (none == 0 && (b + 2) * 16 <= see_all) {
 #pragma unroll 1
           for (int i = 0; i < 2; i += KB)
@@ -799,11 +812,18 @@ __global__ void __launch_bounds__(NW * 32, CTAS) q4_attention_kernel(const Q4Par
   }
 }
 
-// Warps of a CTA and CTAs of an SM by the columns of a warp's tile, as registers allow.
+// Warps of a CTA and CTAs of an SM by the columns of a warp's tile, as registers allow: the more
+// warps the more hides a warp's waits, until two blocks at once, which do as much, no longer fit. Heads
+// of 128, one tile of columns (64 rows of 1024 to 8192 keys; 2 of 120,000 to 131,072; 1 of 75), us:
+// 2 x 8 warps, a block at a time 87.5, 77.1, 14.0; 2 x 7 96.3, 83.8, 14.1; 2 x 6 87.3, 76.7, 12.9; 2 x 6, two
+// blocks 83.7, 73.7, 13.0; 2 x 5, two blocks 98.1, 85.3, 8.8; 1 x 12, two blocks 83.4, 71.5, 14.3.
+// Heads of 64: 2 x 8 44.6 (256 rows), 2 x 7 48.7, 2 x 6 47.8; two tiles of columns of 64 (48 rows of 2
+// tokens, 3000 keys): 2 x 6, two blocks 48.7, one 49.4; 2 x 8 51.2. Two tiles of 128: 2 x 4 196 (48 rows of
+// drafts, with their chunks), 2 x 5 214.
 template <int D, int NT>
 struct Shape {
   static constexpr int kSize = D / 64 * NT;  // a measure of the tile's accumulators
-  static constexpr int kWarps = kSize <= 2 ? 8 : kSize <= 4 ? 4 : 6;
+  static constexpr int kWarps = kSize == 1 ? 8 : kSize == 2 ? 6 : kSize <= 4 ? 4 : 6;
   static constexpr int kCtas = kSize <= 2 ? 2 : kSize <= 4 ? 2 : 1;
   static constexpr int kStages = D == 64 ? 4 : D == 128 ? 2 : 1;
 };
@@ -856,7 +876,8 @@ int launch(Q4Params& p, void* workspace, int64_t bytes, cudaStream_t s) {
               (long long)p.max_blocks);
     return SEB_EUNSUPPORTED;
   }
-  const int64_t most = (pairs + Sh::kWarps * kMinRun - 1) / (Sh::kWarps * kMinRun);
+  // (a CTA may take little more than half of its warps' shortest runs, see `even`)
+  const int64_t most = 2 * pairs / (Sh::kWarps * kMinRun) + 1;
   kern<<<(unsigned)std::min<int64_t>(ctas, most), Sh::kWarps * 32, smem, s>>>(p);
   return launch_status("q4_attention_kernel");
 }
