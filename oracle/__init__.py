@@ -13,5 +13,6 @@ Pinning: tests/golden/ holds outputs of the reference itself run in this
 container (its eager paged-attention path, its Triton kernel under the Triton
 interpreter, its index_copy_ KV write and its build_paged_batch_metadata),
 made by tests/golden/make_golden.py; tests/test_oracle_golden.py checks every
-function here against them.
+function here against them. q4.py, the 4-bit pool's format, has no counterpart
+in the reference: it restates what the library's header says of it.
 """

@@ -12,7 +12,8 @@
 // Bound: latency. The rows are few (their arrays stay in L2), so every CTA does the
 // whole scan in its own shared memory and then takes its share of the tokens and of
 // the new blocks, each found by binary search: one launch and no wait between CTAs.
-// 4.6 us for 256 rows of one token, a launch's own time.
+// 4.9 us for 256 rows of one token, of which 2.3 are an empty launch's; 9.7 us for 4096 rows,
+// whose scan, eight rows to a thread, every CTA repeats.
 #include "seb_common.cuh"
 
 #include <algorithm>
