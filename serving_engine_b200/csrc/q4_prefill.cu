@@ -72,7 +72,8 @@ struct Smem {
   static constexpr int oInfo = oBar + 384;                  // TileInfo [4]
   static constexpr int oPieces = oInfo + 4 * 16;            // Unit [kPieces], 96 bytes each
   static constexpr int oPrefix = oPieces + kPieces * 96;    // uint32 [kThreads + 1]
-  static constexpr int oMl = (oPrefix + (kThreads + 1) * 4 + 7) / 8 * 8;  // float2 [2][kRows]
+  static constexpr int oLongest = oPrefix + (kThreads + 1) * 4;            // uint32
+  static constexpr int oMl = (oLongest + 4 + 7) / 8 * 8;    // float2 [2][kRows]
   static constexpr int kBytes = oMl + 2 * kRows * 8;
 };
 
@@ -132,7 +133,10 @@ constexpr int kEnd = 4;
 // keys 2776 and 221; but 4 rows of 512 and 4096 keys (256 units) 206 and 227. A start, with a
 // part's join, costs as much as 10 key tiles (48 rows of drafts: 3 places 205 us, 6 202, 10 196).
 constexpr uint32_t kUnitPlaces = 10;
-constexpr uint32_t kMinPlaces = 20;  // shortest run worth a CTA
+// Shortest run worth a CTA. One row of 64 tokens that sees 2000 / 4000 / 8000 keys, us: 4: 40.8 / 48.4 / 66.3;
+// 8: 49.9 / 53.1 / 60.5; 12: 61.4 / 63.8 / 66.3; 20: 65.5 / 85.7 / 84.3. Where such a run would be as long as the
+// longest unit, units stay whole (one row of 200 tokens and 400 keys: 64 us cut, 39 whole).
+constexpr uint32_t kMinPlaces = 4;
 
 __device__ __forceinline__ int pairs_of(const Q4Params& p, const Row& w) {
   return (w.q_len + kTiles * p.tile - 1) / (kTiles * p.tile);
@@ -299,13 +303,19 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
   // ---- the rows' units, and where there are few their places; errors in rows are reported by
   // the kernel for the other rows
   Plan plan;
+  uint32_t units = 0;  // of the rows up to this thread's
+  uint32_t* longest = reinterpret_cast<uint32_t*>(sbase + S::oLongest);
+  if (tid == 0) *longest = 0;
 #pragma unroll 1
   for (int cut = 0; cut < 2; ++cut) {
     const int chunk = (p.num_rows + kThreads - 1) / kThreads;
     uint32_t sum = 0, bad = 0;
 #pragma unroll 1
-    for (int r = tid * chunk; r < min((tid + 1) * chunk, p.num_rows); ++r)
-      sum += length_of(p, row_of<true>(p, r, &bad), cut);
+    for (int r = tid * chunk; r < min((tid + 1) * chunk, p.num_rows); ++r) {
+      const Row row = row_of<true>(p, r, &bad);
+      sum += length_of(p, row, cut);
+      if (cut && row.q_len > 0) atomicMax(longest, places_of(blocks_of(p, row, pairs_of(p, row) - 1)));
+    }
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
       const uint32_t o = __shfl_up_sync(kFull, sum, off);
@@ -325,8 +335,16 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
     plan.per = cut ? max((total + gridDim.x - 1) / gridDim.x, kMinPlaces) : 1;
     plan.pos = blockIdx.x * plan.per;
     plan.stop = cut ? min(plan.pos + plan.per, total) : total;
-    if (cut || total == 0 || total >= p.cut_below) break;
-    __syncthreads();
+    if (cut == 0) {
+      units = prefix[tid + 1];
+      if (total == 0 || total >= p.cut_below) break;
+      __syncthreads();
+    } else if (plan.per >= *longest) {  // a CTA for each unit is done sooner
+      __syncthreads();
+      prefix[tid + 1] = units;
+      __syncthreads();
+      plan = Plan{false, 1, blockIdx.x, prefix[kThreads]};
+    }
   }
   if (plan.pos >= plan.stop) return;
 
