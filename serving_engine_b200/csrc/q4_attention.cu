@@ -17,8 +17,11 @@
 //
 // Rounding to 16 bits: q becomes fp16 after a power of two per head that puts its
 // largest element at 2^14 (exact for bf16 and fp16 down to 2^-28 of that element);
-// p_j sV_jG becomes fp16 (unit 2^-11) after a power of two that keeps it below 2^15.
-// Scores, maxima, sums and O are fp32.
+// p_j sV_jG becomes fp16 (unit 2^-11) after a power of two that keeps it below 2^15, and
+// where O is fp16 the sum of two such numbers, a product for each: with one, O was off by 2.9e-4
+// and 3.7e-4 (256 rows, heads of 64; 2 of 120,000 keys) where its own rounding is 2.1e-4, with two by 2.1e-4
+// and 2.6e-4, for 48 us instead of 45 and 85 instead of 73. In bf16 its own rounding (1.7e-3) hides
+// either. Scores, maxima, sums and O are fp32.
 //
 // Work: a unit is (row, tile of tokens, kv head) and its blocks, taken in pairs; the units
 // of all rows laid end to end are cut in equal runs of pairs, one per resident warp,
@@ -30,6 +33,7 @@
 
 #include <algorithm>
 #include <cfloat>
+#include <type_traits>
 
 namespace seb {
 namespace {
@@ -206,8 +210,9 @@ struct Tile {
 // from here. The tensor cores cut a sum off where they add to it, so that each step costs it up
 // to 2^-23 of itself, always towards zero. The codes' sums only grow, and what they stand for is
 // the small rest once 8 of each code is taken off: over a long run the cuts would be what is
-// left (120,000 keys: 1.1e-2 of O; taken off every 256 keys: 3.7e-4, where O in fp16 alone is 2.1e-4).
-constexpr int kCentreBlocks = 16;
+// left (120,000 keys: 1.1e-2 of O; taken off every 256 keys 2.9e-4, 128 2.8e-4, 64 2.6e-4, where O in fp16
+// alone is 2.1e-4; the last costs 0.4 us of 83.4 at 64 decode rows).
+constexpr int kCentreBlocks = 4;
 template <int D, int NT>
 __device__ __forceinline__ void centre(Tile<D, NT>& u) {
 #pragma unroll
@@ -303,10 +308,17 @@ __device__ __forceinline__ void load_pairs(const char* at, __half2 (&a)[G]) {
   else *reinterpret_cast<uint32_t*>(a) = *reinterpret_cast<const uint32_t*>(at);
 }
 
+// What rounding two numbers to fp16 leaves of them.
+__device__ __forceinline__ uint32_t rest(float a, float b) {
+  const uint32_t w = Mma<__half>::pack(a, b);
+  const float2 r = __half22float2(*reinterpret_cast<const __half2*>(&w));
+  return Mma<__half>::pack(a - r.x, b - r.y);
+}
+
 // KB blocks of 16 keys. `place` holds their rows, K and V of one after the other. MASK: some
 // key is not for every column; of keys key0 and on a column then sees those below its
-// `end`, and none of block i where bit i of `unread` says that it has no data.
-template <int D, int NT, int KB, bool MASK>
+// `end`, and none of block i where bit i of `unread` says that it has no data. FINE: p * scale in two parts.
+template <bool FINE, int D, int NT, int KB, bool MASK>
 __device__ __forceinline__ void take_blocks(Tile<D, NT>& u, const char* place, int lane, int key0, unsigned unread,
                                             const int (&end)[NT][2]) {
   using L = q4::Layout<D>;
@@ -453,7 +465,7 @@ __device__ __forceinline__ void take_blocks(Tile<D, NT>& u, const char* place, i
 #pragma unroll
       for (int gi = 0; gi < G; ++gi) {
         const int gr = pn * G + gi;
-        uint32_t b0[NT], b1[NT];
+        uint32_t b0[NT], b1[NT], r0[NT], r1[NT];
         float z[NT][4];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -475,6 +487,12 @@ __device__ __forceinline__ void take_blocks(Tile<D, NT>& u, const char* place, i
           constexpr uint32_t kOnes = 0x3c003c00u;
           Mma<__half>::run(u.one[gr / 2][nt], gr & 1 ? 0u : kOnes, gr & 1 ? kOnes : 0u, gr & 1 ? 0u : kOnes,
                            gr & 1 ? kOnes : 0u, b0[nt], b1[nt]);
+          if constexpr (FINE) {  // and what its rounding left
+            r0[nt] = movmatrix_trans(rest(z[nt][0], z[nt][1]));
+            r1[nt] = movmatrix_trans(rest(z[nt][2], z[nt][3]));
+            Mma<__half>::run(u.one[gr / 2][nt], gr & 1 ? 0u : kOnes, gr & 1 ? kOnes : 0u, gr & 1 ? 0u : kOnes,
+                             gr & 1 ? kOnes : 0u, r0[nt], r1[nt]);
+          }
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -483,9 +501,13 @@ __device__ __forceinline__ void take_blocks(Tile<D, NT>& u, const char* place, i
           for (int h = 0; h < 2; ++h) {
             const uint32_t x0 = h ? v0 >> 8 : v0, x1 = h ? v1 >> 8 : v1;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            for (int nt = 0; nt < NT; ++nt) {
               Mma<__half>::run(u.o[gr][2 * i + h][nt], x0 & 0x000f000fu, x0 & 0x00f000f0u, x1 & 0x000f000fu,
                                x1 & 0x00f000f0u, b0[nt], b1[nt]);
+              if constexpr (FINE)
+                Mma<__half>::run(u.o[gr][2 * i + h][nt], x0 & 0x000f000fu, x0 & 0x00f000f0u, x1 & 0x000f000fu,
+                                 x1 & 0x00f000f0u, r0[nt], r1[nt]);
+            }
           }
         }
       }
@@ -673,15 +695,16 @@ __global__ void __launch_bounds__(NW * 32, CTAS) q4_attention_kernel(const Q4Par
         const unsigned none = (unread >> (2 * s)) & 3;
         const char* place = ring + s * S::kStage;
         // two blocks at once where the tile leaves registers for it
+        constexpr bool kFine = std::is_same<T, __half>::value;
         constexpr int KB = GR * NT <= 2 ? 2 : 1;
         if (none == 0 && (b + 2) * 16 <= see_all) {
 #pragma unroll 1
           for (int i = 0; i < 2; i += KB)
-            take_blocks<D, NT, KB, false>(u, place + i * 2 * L::kRow, lane, (b + i) * 16, 0, end);
+            take_blocks<kFine, D, NT, KB, false>(u, place + i * 2 * L::kRow, lane, (b + i) * 16, 0, end);
         } else {
 #pragma unroll 1
           for (int i = 0; i < 2; ++i)
-            take_blocks<D, NT, 1, true>(u, place + i * 2 * L::kRow, lane, (b + i) * 16, (none >> i) & 1, end);
+            take_blocks<kFine, D, NT, 1, true>(u, place + i * 2 * L::kRow, lane, (b + i) * 16, (none >> i) & 1, end);
         }
         __syncwarp();  // every lane has read the place: it may be filled again
         if (((b - blk0) & (kCentreBlocks - 1)) == kCentreBlocks - 2) centre(u);
