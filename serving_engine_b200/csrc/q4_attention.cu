@@ -837,7 +837,8 @@ __global__ void __launch_bounds__(NW * 32, CTAS) q4_attention_kernel(const Q4Par
 
 // Warps of a CTA and CTAs of an SM by the columns of a warp's tile, as registers allow: the more
 // warps the more hides a warp's waits, until two blocks at once, which do as much, no longer fit. Heads
-// of 128, one tile of columns (64 rows of 1024 to 8192 keys; 2 of 120,000 to 131,072; 1 of 75), us:
+// of 128, one tile of columns (64 rows of 1024 to 8192 keys; 2 of 120,000 to 131,072; 1 of 75), us, all with
+// p * scale in one part:
 // 2 x 8 warps, a block at a time 87.5, 77.1, 14.0; 2 x 7 96.3, 83.8, 14.1; 2 x 6 87.3, 76.7, 12.9; 2 x 6, two
 // blocks 83.7, 73.7, 13.0; 2 x 5, two blocks 98.1, 85.3, 8.8; 1 x 12, two blocks 83.4, 71.5, 14.3.
 // Heads of 64: 2 x 8 44.6 (256 rows), 2 x 7 48.7, 2 x 6 47.8; two tiles of columns of 64 (48 rows of 2
