@@ -17,7 +17,10 @@
 //
 // Rounding to 16 bits: q becomes fp16 after a power of two per head that puts its
 // largest element at 2^14 (exact for bf16 and fp16 down to 2^-28 of that element);
-// p_j sV_jG becomes fp16 (unit 2^-11) after a power of two that keeps it below 2^15, and
+// p_j sV_jG becomes fp16 (unit 2^-11) after a power of two that keeps it below 2^15: each column has its
+// own, from the largest p_j sV_jG of the keys that it sees, so that no other key, and none of no weight,
+// costs those that count their bits (one power for a warp, from V's scales alone, took 1 to 2 % less time,
+// 84.2 us instead of 85.1 at 64 decode rows, but a stale slot could cost a few per cent of O). And
 // where O is fp16 the sum of two such numbers, a product for each: with one, O was off by 2.9e-4
 // and 3.7e-4 (256 rows, heads of 64; 2 of 120,000 keys) where its own rounding is 2.1e-4, with two by 2.1e-4
 // and 2.6e-4, for 48 us instead of 45 and 85 instead of 73. In bf16 its own rounding (1.7e-3) hides
@@ -30,6 +33,7 @@
 // Parts of a unit are joined in shared memory, and over CTAs in the workspace by the
 // last to arrive, in order of their place, so results do not depend on timing.
 #include "q4_attention.cuh"
+#include "seb_softmax.cuh"
 
 #include <algorithm>
 #include <cfloat>
@@ -44,9 +48,10 @@ constexpr uint32_t kMinRun = 2;
 // What a unit's start and end cost a warp, in pairs of blocks. 256 rows of 32 to 4352 keys, heads of 64:
 // 0: 55.6 us, 1: 49.2, 2: 45.1, 3: 44.8, 4: 44.6, 6: 45.9; 64 rows of 1024 to 8192, heads of 128: 1 84.2, 2 83.6, 3 83.6.
 constexpr uint32_t kUnitCost = 2;
-constexpr float kNoMax = -FLT_MAX;       // no score yet: any score is above it by more than the threshold
-constexpr float kThreshold = 8.f;        // scores may exceed the reference by 2^8 before it is moved
-constexpr float kScaleThreshold = 64.f;  // p * V scale stays below 2^8 * 2^6
+constexpr float kThreshold = 8.f;  // scores may exceed the reference by 2^8 before it is moved
+// p * V's scale stays below 2^15, and the largest of them is put at [2^8, 2^9) when its power of two is
+// taken: what is 2^-22 of that one is still not subnormal.
+constexpr float kScaleTop = 15.f, kScalePlace = 8.f;
 
 // Arrivals at the units that span CTAs, one for each four columns, at the CTA that a unit
 // starts in. Zero when the library is loaded, and again after every call (the last to
@@ -82,10 +87,14 @@ struct Smem {
   static constexpr int kBytes = kWarps + NW * kWarp;
 };
 
-__device__ __forceinline__ float exp2_fast(float x) {
+__device__ __forceinline__ float log2_fast(float x) {
   float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// 2^e of a whole e in [-126, 127]: the sum holds 127 + e in its lowest bits. 0 for an infinity.
+__device__ __forceinline__ float power_of(float e) {
+  return __uint_as_float(__float_as_uint(e + (12582912.f + 127.f)) << 23);
 }
 // The token, of its tile, of a column.
 __device__ __forceinline__ int token_of(const Q4Params& p, int col) { return (int)(col * p.by_group >> 16); }
@@ -132,7 +141,7 @@ __device__ __forceinline__ void join(int n, int cols, int lane, F part, int ml, 
 #pragma unroll
     for (int off = 4; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, off));
     const float ref = top == -INFINITY ? 0.f : top;
-    const float keep = exp2_fast(m - ref), w = exp2_fast(mine.x - ref);
+    const float keep = fast_exp2(m - ref), w = fast_exp2(mine.x - ref);
     float sum = mine.y * w;
 #pragma unroll
     for (int off = 4; off >= 1; off >>= 1) sum += __shfl_xor_sync(kFull, sum, off);
@@ -200,10 +209,10 @@ struct Tile {
   float qs[GR][NT][2];        // sum of q over a group, columns 8 nt + 2 t and the next
   float ch[NT][2];            // what brings a score to log2 units
   float m[NT][2], l[NT][2];   // reference, and this lane's share of the sum
+  float v_exp[NT][2];         // exponent that brings p * scale to fp16's range; inf: no key yet, and m is 0
   float low[GR][NT][2];       // this lane's share of sum p (low + 8 scale)
   float one[(GR + 1) / 2][NT][4];  // sum of the rounded p * scale, two groups to a tile
   float o[GR][4][NT][4];      // sum of those and the codes: n of a dim, and 16 n of the next
-  float v_down;               // power of two that V's scales are taken by
 };
 
 // From the sums over codes, 8 times the sum of what they were taken by, which is then counted
@@ -383,20 +392,12 @@ __device__ __forceinline__ void take_blocks(Tile<D, NT>& u, const char* place, i
       }
   }
 
-  // this lane's largest score of each column, and the largest V scale
-  float top[NT][2];
-  bool move = false;
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      top[nt][h] = fmaxf(x[0][nt][h], x[0][nt][h + 2]);
-#pragma unroll
-      for (int b = 1; b < KB; ++b) top[nt][h] = fmaxf(top[nt][h], fmaxf(x[b][nt][h], x[b][nt][h + 2]));
-      move |= top[nt][h] > u.m[nt][h] + kThreshold;
-    }
+  // Scores count from their column's reference from here. The largest of each column that this lane
+  // has; what p * scale may be is first bounded by it and the largest scale, and only where that
+  // bound calls for a move worked out key by key: a column moves for keys that it sees and no others.
   __half2 vp[KB][P][2][G];  // of keys g and g + 8
-  __half2 most = __half2half2(__ushort_as_half(0));
+  float top[NT][2];
+  __half2 most[KB][2];
 #pragma unroll
   for (int b = 0; b < KB; ++b)
 #pragma unroll
@@ -405,39 +406,80 @@ __device__ __forceinline__ void take_blocks(Tile<D, NT>& u, const char* place, i
       for (int h = 0; h < 2; ++h) {
         load_pairs<G>(place + (b * 2 + 1) * L::kRow + L::kCodes + pn * 64 * G + (g + 8 * h) * 4 * G, vp[b][pn][h]);
 #pragma unroll
-        for (int gi = 0; gi < G; ++gi) most = __hmax2(most, vp[b][pn][h][gi]);
+        for (int gi = 0; gi < G; ++gi)
+          most[b][h] = pn + gi == 0 ? vp[b][pn][h][gi] : __hmax2(most[b][h], vp[b][pn][h][gi]);
       }
-  float vmax = __low2float(most);
-  if (__any_sync(kFull, move || vmax * u.v_down > kScaleThreshold)) {
-    // move the references: the power of two of V's scales, and the scores' maxima
+  auto log2_scale = [](__half2 pair) { return log2_fast(fmaxf(__low2float(pair), power2(-30))); };  // a NaN counts as 0
 #pragma unroll
-    for (int k = 16; k >= 1; k >>= 1) vmax = fmaxf(vmax, __shfl_xor_sync(kFull, vmax, k));
-    float v_fix = 1.f;
-    if (vmax * u.v_down > kScaleThreshold) {
-      const float now = power2(-min(max(exponent(vmax), -24), 16));
-      v_fix = now / u.v_down;
-      u.v_down = now;
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) top[nt][h] = -INFINITY;
+  __half2 largest = most[0][0];
+#pragma unroll
+  for (int b = 0; b < KB; ++b)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (b + h > 0) largest = __hmax2(largest, most[b][h]);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 2 * h; c < 2 * h + 2; ++c) {
+          x[b][nt][c] -= u.m[nt][c & 1];
+          top[nt][c & 1] = fmaxf(top[nt][c & 1], x[b][nt][c]);
+        }
     }
+  const float above = log2_scale(largest) - (kScaleTop - 0.01f);
+  bool move = false;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) move |= top[nt][h] > kThreshold || top[nt][h] + above > -u.v_exp[nt][h];
+  if (__any_sync(kFull, move)) {
+    // move the references of the columns that need it
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        float mx = top[nt][h];
-        mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 4));
-        mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 8));
-        mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 16));
-        const float now = fmaxf(mx, u.m[nt][h]);
-        const float fix = exp2_fast(u.m[nt][h] - now);  // from kNoMax: 0
-        u.m[nt][h] = now;
+        float mx = top[nt][h], z = -INFINITY;  // log2 of the largest p * scale
+#pragma unroll
+        for (int b = 0; b < KB; ++b) {
+          z = fmaxf(z, x[b][nt][h] + log2_scale(most[b][0]));
+          z = fmaxf(z, x[b][nt][h + 2] + log2_scale(most[b][1]));
+        }
+#pragma unroll
+        for (int k = 4; k <= 16; k <<= 1) {
+          mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, k));
+          z = fmaxf(z, __shfl_xor_sync(kFull, z, k));
+        }
+        const bool first = u.v_exp[nt][h] == INFINITY;
+        float up = 0.f;
+        if (mx > kThreshold || (first && mx > -INFINITY)) {
+          const float now = u.m[nt][h] + mx;
+          up = now - u.m[nt][h];
+          u.m[nt][h] = now;
+        }
+        // what was summed up so far went down by 2^up, and its power of two up by as much
+        float e = first ? INFINITY : kScalePlace - floorf(kScalePlace - u.v_exp[nt][h] - up);
+        z -= up;
+        if (z > kScaleTop - e) e = kScalePlace - floorf(z);
+        if (!first || z > -INFINITY) e = fminf(fmaxf(e, -20.f), 100.f);
+        const float fix = first ? 0.f : fast_exp2(-up);  // nothing is summed up yet at first
+        const float z_fix = first ? 0.f : fix * (power_of(e) / power_of(u.v_exp[nt][h]));
+        u.v_exp[nt][h] = e;
         u.l[nt][h] *= fix;
+#pragma unroll
+        for (int b = 0; b < KB; ++b) {
+          x[b][nt][h] -= up;
+          x[b][nt][h + 2] -= up;
+        }
 #pragma unroll
         for (int gr = 0; gr < GR; ++gr) {
           u.low[gr][nt][h] *= fix;
-          u.one[gr / 2][nt][(gr & 1) * 2 + h] *= fix * v_fix;
+          u.one[gr / 2][nt][(gr & 1) * 2 + h] *= z_fix;
 #pragma unroll
           for (int mt = 0; mt < 4; ++mt) {
-            u.o[gr][mt][nt][h] *= fix * v_fix;
-            u.o[gr][mt][nt][h + 2] *= fix * v_fix;
+            u.o[gr][mt][nt][h] *= z_fix;
+            u.o[gr][mt][nt][h + 2] *= z_fix;
           }
         }
       }
@@ -447,12 +489,17 @@ __device__ __forceinline__ void take_blocks(Tile<D, NT>& u, const char* place, i
   // sum p low = sum p' (n - 8) + sum p (low + 8 scale) with p' = p scale rounded to fp16, so
   // that its rounding meets n - 8 and no more; sum p' is one more row of the product.
   // Keys that a column does not see have p = 0, and none of their parameters is used.
+  float v_down[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) v_down[nt][h] = power_of(u.v_exp[nt][h]);
 #pragma unroll
   for (int b = 0; b < KB; ++b) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-      for (int c = 0; c < 4; ++c) x[b][nt][c] = exp2_fast(x[b][nt][c] - u.m[nt][c & 1]);
+      for (int c = 0; c < 4; ++c) x[b][nt][c] = fast_exp2(x[b][nt][c]);
       u.l[nt][0] += x[b][nt][0] + x[b][nt][2];
       u.l[nt][1] += x[b][nt][1] + x[b][nt][3];
     }
@@ -470,13 +517,13 @@ __device__ __forceinline__ void take_blocks(Tile<D, NT>& u, const char* place, i
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const float scale = __low2float(vp[b][pn][h][gi]), low = __high2float(vp[b][pn][h][gi]);
-          const float sv = scale * u.v_down, mid = fmaf(8.f, scale, low);
+          const float mid = fmaf(8.f, scale, low);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int c = 2 * h; c < 2 * h + 2; ++c) {
               const bool hide = hidden(b, nt, c);
-              z[nt][c] = hide ? 0.f : x[b][nt][c] * sv;
+              z[nt][c] = hide ? 0.f : x[b][nt][c] * v_down[nt][c & 1] * scale;
               u.low[gr][nt][c & 1] = fmaf(x[b][nt][c], hide ? 0.f : mid, u.low[gr][nt][c & 1]);
             }
         }
@@ -663,8 +710,8 @@ __global__ void __launch_bounds__(NW * 32, CTAS) q4_attention_kernel(const Q4Par
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          u.m[nt][h] = kNoMax;
-          u.l[nt][h] = 0.f;
+          u.m[nt][h] = u.l[nt][h] = 0.f;
+          u.v_exp[nt][h] = INFINITY;
 #pragma unroll
           for (int gr = 0; gr < GR; ++gr) u.low[gr][nt][h] = 0.f;
         }
@@ -683,7 +730,6 @@ __global__ void __launch_bounds__(NW * 32, CTAS) q4_attention_kernel(const Q4Par
 #pragma unroll
         for (int h = 0; h < 2; ++h)
           end[nt][h] = p.causal ? min(row.k_len, first_sees + token_of(p, nt * 8 + 2 * t + h)) : row.k_len;
-      u.v_down = power2(60);  // the first scale moves it
 
       for (int b = blk0; b < blk1; b += 2, ++it) {
         const uint32_t s = it % STAGES;
@@ -717,13 +763,13 @@ __global__ void __launch_bounds__(NW * 32, CTAS) q4_attention_kernel(const Q4Par
       const bool whole = n == length;
       const bool last_run = pos + n == stop;
       float* po = reinterpret_cast<float*>(whole || last_run ? ring : ring + S::kRing);
-      const float v_up = power2(24) / u.v_down;
       __syncwarp();
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int col = nt * 8 + 2 * t + h;
+          const float v_up = u.v_exp[nt][h] == INFINITY ? 0.f : power_of(24.f - u.v_exp[nt][h]);
           float lt = u.l[nt][h];
 #pragma unroll
           for (int k = 4; k <= 16; k <<= 1) lt += __shfl_xor_sync(kFull, lt, k);
@@ -747,7 +793,7 @@ __global__ void __launch_bounds__(NW * 32, CTAS) q4_attention_kernel(const Q4Par
           }
           if (g == 0 && col < cols)
             reinterpret_cast<float2*>(po + kCols * D)[col] =
-                make_float2(u.m[nt][h] == kNoMax ? -INFINITY : u.m[nt][h], lt);
+                make_float2(lt == 0.f ? -INFINITY : u.m[nt][h], lt);
         }
       __syncwarp();
       if (whole) {
