@@ -374,7 +374,9 @@ SEB_API int seb_qk_norm_rope_append(const void* qkv, int64_t qkv_stride_token, i
  * is skipped. Rows of q and out are 16-byte aligned.
  * workspace: seb_paged_attention_q4_workspace_size(...) bytes, 16-byte aligned, of any
  * content. counter_slot: 0 .. SEB_Q4_COUNTER_SLOTS - 1, a set of the library's own
- * arrival counters. Calls that may overlap on the GPU need a workspace and a slot each. */
+ * arrival counters on the current device. Calls that may overlap on the GPU need a workspace
+ * and a slot each: with one of either in common their results are wrong, and what an overlap
+ * leaves in a slot's counters spoils later calls with that slot too. */
 #define SEB_Q4_COUNTER_SLOTS 128
 SEB_API int64_t seb_paged_attention_q4_workspace_size(int32_t num_rows, int32_t total_query, int32_t num_q_heads,
                                                       int32_t num_kv_heads, int32_t head_dim);

@@ -14,6 +14,7 @@ reported by ``check_device_errors``. bf16 and fp16, head_dim 64, 128 and 256.
 from __future__ import annotations
 
 import functools
+import threading
 
 import torch
 
@@ -37,22 +38,41 @@ def new_q4_pool(num_layers: int, num_blocks: int, num_kv_heads: int, head_dim: i
     return torch.zeros(num_layers, 2, num_blocks, num_kv_heads, row_bytes(head_dim), dtype=torch.uint8, device=device)
 
 
-# (device, stream) -> (workspace, counter slot). A workspace that a larger call outgrew
-# stays allocated: a captured CUDA graph may hold its address.
+# A stream's workspace and counter slot on a device. Slots are handed out under the lock, and one at a
+# time: two calls that overlap on the GPU with one slot would join sums that are not complete. A workspace
+# that a larger call outgrew stays allocated: a captured CUDA graph may hold its address.
+_lock = threading.Lock()
+_slots: dict[tuple[int, int], int] = {}
 _workspaces: dict[tuple[int, int], tuple[torch.Tensor, int]] = {}
 _retired: list[torch.Tensor] = []
+
+
+def _slot(device: int, stream: int) -> int:
+    with _lock:
+        slot = _slots.get((device, stream))
+        if slot is None:
+            taken = {s for (d, _), s in _slots.items() if d == device}
+            slot = next((s for s in range(Q4_COUNTER_SLOTS) if s not in taken), None)
+            if slot is None:
+                raise RuntimeError(f"paged_attention_q4: all {Q4_COUNTER_SLOTS} counter slots of device {device} belong to "
+                                   "streams; issue the calls on fewer streams")
+            _slots[device, stream] = slot
+    return slot
 
 
 def _workspace(device: int, stream: int, nbytes: int) -> tuple[torch.Tensor, int]:
     """The stream's own workspace and counters, so calls on different streams may overlap."""
     held = _workspaces.get((device, stream))
     if held is None or held[0].numel() < nbytes:
-        slot = len(_workspaces) % Q4_COUNTER_SLOTS if held is None else held[1]
-        if held is not None:
-            _retired.append(held[0])
+        slot = _slot(device, stream)
         with torch.inference_mode(False):
-            held = (torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", device)), slot)
-        _workspaces[device, stream] = held
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", device))
+        with _lock:
+            held = _workspaces.get((device, stream))
+            if held is None or held[0].numel() < nbytes:
+                if held is not None:
+                    _retired.append(held[0])
+                held = _workspaces[device, stream] = (ws, slot)
     return held
 
 
@@ -270,7 +290,8 @@ def paged_attention_q4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
     ``kv_append_q4``; block_table int32 [rows, max_blocks]; the other arrays int32 [rows].
     A query that sees no key gets 0 and -inf; tokens of no row keep what out held.
 
-    Every stream has its own workspace: calls on different streams may overlap. A CUDA
+    Every stream has its own workspace and counters: calls on different streams may overlap
+    (on 128 streams of a device; a call on one more raises RuntimeError). A CUDA
     graph holds the workspace of the stream it was captured on; graphs captured on one
     stream must not be replayed at the same time.
     """
