@@ -77,7 +77,9 @@ def _workspace(device: int, stream: int, nbytes: int) -> tuple[torch.Tensor, int
 
 
 @functools.lru_cache(maxsize=4096)
-def _attention_workspace_bytes(rows: int, total_query: int, num_q_heads: int, num_kv_heads: int, head_dim: int) -> int:
+def _attention_workspace_bytes(device: int, rows: int, total_query: int, num_q_heads: int, num_kv_heads: int,
+                               head_dim: int) -> int:
+    """By device: the library's answer depends on the device's SMs."""
     return int(lib().seb_paged_attention_q4_workspace_size(rows, total_query, num_q_heads, num_kv_heads, head_dim))
 
 
@@ -323,7 +325,8 @@ def paged_attention_q4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
     if not _aligned(out):
         out = result.clone(memory_format=torch.contiguous_format)
     stream = _raw_stream(device)
-    ws, slot = _workspace(device, stream, _attention_workspace_bytes(rows, total_q, num_q_heads, num_kv_heads, d))
+    ws, slot = _workspace(device, stream,
+                          _attention_workspace_bytes(device, rows, total_q, num_q_heads, num_kv_heads, d))
     qs, os = q.stride(), out.stride()
     st = lib().seb_paged_attention_q4(
         q.data_ptr(), qs[0], qs[1], k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0],

@@ -1,5 +1,6 @@
 """Workspaces and counter slots of paged_attention_q4: one of each for a stream (host logic, no GPU)."""
 import threading
+import types
 
 import pytest
 import torch
@@ -51,3 +52,14 @@ def test_a_larger_call_keeps_the_slot_and_the_old_memory(held):
     large = q4._workspace(0, 9, 64)
     assert large[1] == small[1] and large[0].numel() == 64 and q4._workspace(0, 9, 32)[0] is large[0]
     assert q4._retired[0] is small[0]
+
+
+def test_workspace_sizes_are_kept_by_device(monkeypatch):
+    """Devices may differ in SMs, by which the library sizes the workspace."""
+    sizes = iter((100, 900))
+    monkeypatch.setattr(q4, "lib", lambda: types.SimpleNamespace(seb_paged_attention_q4_workspace_size=lambda *a: next(sizes)))
+    q4._attention_workspace_bytes.cache_clear()
+    try:
+        assert [q4._attention_workspace_bytes(d, 3, 3, 4, 2, 64) for d in (0, 1, 0)] == [100, 900, 100]
+    finally:
+        q4._attention_workspace_bytes.cache_clear()
