@@ -14,7 +14,9 @@ reported by ``check_device_errors``. bf16 and fp16, head_dim 64, 128 and 256.
 from __future__ import annotations
 
 import functools
+import itertools
 import threading
+import weakref
 
 import torch
 
@@ -38,24 +40,55 @@ def new_q4_pool(num_layers: int, num_blocks: int, num_kv_heads: int, head_dim: i
     return torch.zeros(num_layers, 2, num_blocks, num_kv_heads, row_bytes(head_dim), dtype=torch.uint8, device=device)
 
 
-# A stream's workspace and counter slot on a device. Slots are handed out under the lock, and one at a
+# A stream's workspace and counter slot on a device (or a Workspace's, under a negative number). Slots are handed out under the lock, and one at a
 # time: two calls that overlap on the GPU with one slot would join sums that are not complete. A workspace
 # that a larger call outgrew stays allocated: a captured CUDA graph may hold its address.
 _lock = threading.Lock()
 _slots: dict[tuple[int, int], int] = {}
 _workspaces: dict[tuple[int, int], tuple[torch.Tensor, int]] = {}
 _retired: list[torch.Tensor] = []
+_own = threading.local()  # .key: the Workspace that this thread's calls use
+_own_keys = itertools.count(1)
+_gone: list[int] = []  # Workspaces that are no more
+_idle: dict[int, list[int]] = {}  # by device: slots that they left
+
+
+class Workspace:
+    """A workspace and counters of its own: calls that a thread issues ``with`` it use these and not their
+    stream's. For a CUDA graph, which holds those of its capture and may be replayed beside other calls and
+    other graphs of the same capture stream. Keep it as long as the graph."""
+
+    def __init__(self):
+        self._key = -next(_own_keys)
+        weakref.finalize(self, _gone.append, self._key)
+
+    def __enter__(self):
+        _own.outer = (getattr(_own, "key", None), getattr(_own, "outer", None))
+        _own.key = self._key
+        return self
+
+    def __exit__(self, *exc):
+        _own.key, _own.outer = _own.outer
 
 
 def _slot(device: int, stream: int) -> int:
     with _lock:
+        while _gone:
+            key = _gone.pop()
+            for at in [at for at in _slots if at[1] == key]:
+                _idle.setdefault(at[0], []).append(_slots.pop(at))
+                _workspaces.pop(at, None)
         slot = _slots.get((device, stream))
         if slot is None:
-            taken = {s for (d, _), s in _slots.items() if d == device}
+            idle = _idle.get(device, [])
+            taken = {s for (d, _), s in _slots.items() if d == device}.union(idle)
             slot = next((s for s in range(Q4_COUNTER_SLOTS) if s not in taken), None)
+            if slot is None and idle:
+                torch.cuda.synchronize(device)  # the last calls of the one that left it may still run
+                slot = idle.pop()
             if slot is None:
                 raise RuntimeError(f"paged_attention_q4: all {Q4_COUNTER_SLOTS} counter slots of device {device} belong to "
-                                   "streams; issue the calls on fewer streams")
+                                   "streams and Workspaces; issue the calls on fewer streams")
             _slots[device, stream] = slot
     return slot
 
@@ -295,7 +328,8 @@ def paged_attention_q4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
     Every stream has its own workspace and counters: calls on different streams may overlap
     (on 128 streams of a device; a call on one more raises RuntimeError). A CUDA
     graph holds the workspace of the stream it was captured on; graphs captured on one
-    stream must not be replayed at the same time.
+    stream must not be replayed at the same time, nor beside calls on that stream, unless
+    each is captured ``with`` a ``q4.Workspace`` of its own.
     """
     arrays = (q_starts, q_lens, k_lens, q_pos_offsets)
     device = _device("paged_attention_q4", q, k_cache, v_cache, block_table, *arrays)
@@ -325,7 +359,7 @@ def paged_attention_q4(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
     if not _aligned(out):
         out = result.clone(memory_format=torch.contiguous_format)
     stream = _raw_stream(device)
-    ws, slot = _workspace(device, stream,
+    ws, slot = _workspace(device, getattr(_own, "key", None) or stream,
                           _attention_workspace_bytes(device, rows, total_q, num_q_heads, num_kv_heads, d))
     qs, os = q.stride(), out.stride()
     st = lib().seb_paged_attention_q4(

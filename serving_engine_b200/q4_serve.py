@@ -23,7 +23,7 @@ import torch
 
 from . import ops
 from .llama_step import FusedLlamaStep
-from .q4 import new_q4_pool
+from .q4 import Workspace, new_q4_pool
 from .step_tables import StepTables
 
 BLOCK_SIZE = ops.BLOCK_SIZE
@@ -31,7 +31,8 @@ BLOCK_SIZE = ops.BLOCK_SIZE
 
 class Q4Batch:
     """``rows`` requests of up to ``max_len`` tokens each over a pool of ``num_blocks``
-    blocks (default: enough for all). ``model``: as FusedLlamaStep takes it, on a GPU."""
+    blocks (default: enough for all). ``model``: as FusedLlamaStep takes it, on a GPU.
+    Batches may run at the same time, each on a stream of its own."""
 
     def __init__(self, model, rows: int, max_len: int, num_blocks: int | None = None):
         cfg, device = model.config, next(model.parameters()).device
@@ -49,6 +50,7 @@ class Q4Batch:
         self._ones = torch.ones(rows, **i32)
         self._decode_tables = StepTables(rows, rows, device)
         self._graph = None
+        self._workspace = Workspace()  # the graph's: batches on different streams may decode at the same time
 
     def _advance(self, tables: StepTables) -> None:
         self.lens.copy_(tables.k_lens)
@@ -87,12 +89,13 @@ class Q4Batch:
             kept = [t.clone() for t in state]
             side = torch.cuda.Stream(self.device)
             side.wait_stream(torch.cuda.current_stream(self.device))
-            with torch.cuda.stream(side):
+            with torch.cuda.stream(side), self._workspace:
                 self._decode_step()
             torch.cuda.current_stream(self.device).wait_stream(side)
-            self._graph = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(self._graph):
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=side), self._workspace:
                 self._decode_step()
+            self._graph = graph
             for t, k in zip(state, kept):
                 t.copy_(k)
         out = torch.empty(steps, self.rows, dtype=torch.int64, device=self.device)

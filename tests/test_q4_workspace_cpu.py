@@ -1,4 +1,5 @@
 """Workspaces and counter slots of paged_attention_q4: one of each for a stream (host logic, no GPU)."""
+import gc
 import threading
 import types
 
@@ -63,3 +64,32 @@ def test_workspace_sizes_are_kept_by_device(monkeypatch):
         assert [q4._attention_workspace_bytes(d, 3, 3, 4, 2, 64) for d in (0, 1, 0)] == [100, 900, 100]
     finally:
         q4._attention_workspace_bytes.cache_clear()
+
+
+def test_a_workspace_of_its_own(held, monkeypatch):
+    """Two graphs captured on one stream, each with its own, hold different memory and counters; the slot
+    of one that is gone is handed out again only after the device is idle."""
+    synced = []
+    monkeypatch.setattr(q4.torch.cuda, "synchronize", synced.append)
+    monkeypatch.setattr(q4, "_gone", [])
+    monkeypatch.setattr(q4, "_idle", {})
+    own = getattr(q4._own, "key", None)
+    a, b = q4.Workspace(), q4.Workspace()
+    keys = []
+    for w in (a, b):
+        with w:
+            keys.append(q4._own.key)
+            with a:
+                assert q4._own.key == keys[0]
+            assert q4._own.key == keys[-1]
+    assert getattr(q4._own, "key", None) == own and keys[0] != keys[1] and max(keys) < 0
+    got = [q4._workspace(0, k, 64) for k in (5, *keys)]
+    assert len({s for _, s in got}) == 3 and len({w.data_ptr() for w, _ in got}) == 3
+    del a
+    gc.collect()
+    assert q4._gone == [keys[0]]
+    rest = [q4._workspace(0, 100 + s, 16)[1] for s in range(q4.Q4_COUNTER_SLOTS - 3)]
+    assert not synced and got[1][1] not in rest
+    assert q4._workspace(0, 1000, 16)[1] == got[1][1] and synced == [0]
+    with pytest.raises(RuntimeError, match="counter slots"):
+        q4._workspace(0, 1001, 16)
