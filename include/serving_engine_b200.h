@@ -368,7 +368,8 @@ SEB_API int seb_qk_norm_rope_append(const void* qkv, int64_t qkv_stride_token, i
  * q_starts[r] .. + q_lens[r], at positions q_pos_offsets[r] and on, and see the keys
  * j < k_lens[r] (causal: j <= position). q, out: bf16 or fp16; the sums are fp32. A
  * query that sees no key gets O = 0 and LSE = -inf; tokens of no row are left as they
- * are. Rows' token ranges must not overlap. A block id out of range sets
+ * are. A group of V that reads back as NaN makes its own 64 dims of O NaN for the queries
+ * that see its key, one of K all of their O and LSE. Rows' token ranges must not overlap. A block id out of range sets
  * SEB_ERRBIT_BLOCK_ID and its keys count as masked; a k_len beyond the table sets
  * SEB_ERRBIT_KLEN and ends there; a row outside total_query sets SEB_ERRBIT_META and
  * is skipped. Rows of q and out are 16-byte aligned.

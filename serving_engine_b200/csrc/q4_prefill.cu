@@ -71,7 +71,8 @@ struct Smem {
   static constexpr int oBar = oRaw + kRawStages * kRaw;
   static constexpr int oInfo = oBar + 384;                  // TileInfo [4]
   static constexpr int oPieces = oInfo + 4 * 16;            // Unit [kPieces], 96 bytes each
-  static constexpr int oPrefix = oPieces + kPieces * 96;    // uint32 [kThreads + 1]
+  static constexpr int oNan = oPieces + kPieces * 96;       // int [kPieces][2]
+  static constexpr int oPrefix = oNan + kPieces * 8;        // uint32 [kThreads + 1]
   static constexpr int oLongest = oPrefix + (kThreads + 1) * 4;            // uint32
   static constexpr int oMl = (oLongest + 4 + 7) / 8 * 8;    // float2 [2][kRows]
   static constexpr int kBytes = oMl + 2 * kRows * 8;
@@ -118,12 +119,15 @@ struct Unit {
 struct TileInfo {
   int limit;      // its keys below this exist
   unsigned none;  // bit b: block b has no data
-  int kind;       // kSplit, kDiag, or kEnd: no more tiles
-  int pad;
+  int kind;       // kSplit, kDiag, or kEnd: no more tiles; and kPlace times its piece's place
+  int key0;       // its first key
 };
 constexpr int kSplit = 1;  // K in two parts
-constexpr int kDiag = 2;   // some token does not see all of it: there a NaN must not meet a weight of zero
+// Some token does not see all of it. There a V that is NaN must not meet a weight of zero: it is taken as 0,
+// and a group's first key of this kind is kept for the piece; whoever sees that key gets NaN in the group.
+constexpr int kDiag = 2;
 constexpr int kEnd = 4;
+constexpr int kPlace = 8;
 
 // Units are whole where there are at least as many as CTAs (each takes every so manieth).
 // Fewer are laid end to end, kUnitPlaces places for a start and one for each key tile, and
@@ -298,6 +302,7 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
   TileInfo* info = reinterpret_cast<TileInfo*>(sbase + S::oInfo);
   uint32_t* prefix = reinterpret_cast<uint32_t*>(sbase + S::oPrefix);
   Unit* pieces = reinterpret_cast<Unit*>(sbase + S::oPieces);
+  int* nans = reinterpret_cast<int*>(sbase + S::oNan);
   static_assert(sizeof(Unit) <= 96, "room for pieces");
 
   // ---- the rows' units, and where there are few their places; errors in rows are reported by
@@ -422,12 +427,10 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
       if (!raw_full(ik)) break;
       const TileInfo ti = info[n & 3];
       if (ti.kind & kEnd) break;
-      const bool diag = ti.kind & kDiag;
-      if (diag && !raw_full(iv)) break;
+      if ((ti.kind & kDiag) && !raw_full(iv)) break;
       char* tile = k_place();
       if (!tile) break;
       const char* raw_k = sbase + S::oRaw + ik % kRawStages * S::kRaw + (th >> 6) * S::kRawRow;
-      const char* raw_v = sbase + S::oRaw + iv % kRawStages * S::kRaw + (th >> 6) * S::kRawRow;
       const int parts = ti.kind & kSplit ? 2 : 1;
       // K(key, 16 dims of each group): two 16-byte chunks a group, 128-byte swizzled rows of 64 dims
 #pragma unroll 1
@@ -444,11 +447,6 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
           } else {
             *reinterpret_cast<uint2*>(kw) = *reinterpret_cast<const uint2*>(words);
             kp[0] = *reinterpret_cast<const uint32_t*>(raw_k + pairs);
-          }
-          if (diag) {  // whoever sees a token whose V is NaN gets NaN, by way of its score
-#pragma unroll
-            for (int e = 0; e < G; ++e)
-              if (is_nan_pair(*reinterpret_cast<const uint32_t*>(raw_v + pairs + 4 * e))) kp[0] = 0x7fff7fffu;
           }
           const bool gone = 32 * i + kr >= ti.limit || ((ti.none >> (2 * i + (th >> 6))) & 1);
           __half2 most = as_half2(0);
@@ -542,8 +540,15 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
             vp[i] = *reinterpret_cast<const uint32_t*>(raw_v + L::kCodes + (8 * h + (i ^ (4 * h))) * 4 * G + gi * 4);
           if (ti.limit < kKeys || ti.none != 0 || diag) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              if (8 * vc + (i ^ (4 * h)) >= ti.limit || none || (diag && is_nan_pair(vp[i]))) vp[i] = 0;
+            for (int i = 0; i < 8; ++i) {
+              const int key = 8 * vc + (i ^ (4 * h));
+              if (key >= ti.limit || none) {
+                vp[i] = 0;
+              } else if (diag && is_nan_pair(vp[i])) {
+                vp[i] = 0;
+                atomicMin(nans + ti.kind / kPlace * 2 + gi, ti.key0 + key);
+              }
+            }
           }
           __half2 most = as_half2(0), sc[4], lo[4];
 #pragma unroll
@@ -608,6 +613,7 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
         }
         if (lane == 0) {
           pieces[s] = w;
+          nans[2 * s] = nans[2 * s + 1] = INT32_MAX;
           mbar_arrive(bar + 8 * (kBarPieceFull + s));
         }
       }
@@ -649,7 +655,9 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
               if (!is_v)
                 info[n & 3] = TileInfo{w.k_len - j * kKeys, ~have & 0xffu,
                                        (w.split ? kSplit : 0) |
-                                           ((j + 1) * kKeys > min(w.sees, w.k_len) ? kDiag : 0), 0};
+                                           ((j + 1) * kKeys > min(w.sees, w.k_len) ? kDiag : 0) |
+                                           ip % kPieces * kPlace,
+                                       j * kKeys};
               mbar_arrive_expect_tx(bar + 8 * (kBarRawFull + s), __popc(have) * L::kRow);
             }
             __syncwarp();
@@ -1024,6 +1032,10 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
           tc::tmem_wait_ld();
 #pragma unroll
           for (int i = 0; i < 32; ++i) o[i] = fmaf(x[i], f1, o[i] * f0);
+        }
+        if (nans[ip % kPieces * 2 + d / q4::kGroup] < vis) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = __int_as_float(0x7fffffff);
         }
       };
       T* op = reinterpret_cast<T*>(p.out) + token * p.o_st + (int64_t)head * p.o_sh;

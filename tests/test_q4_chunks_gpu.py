@@ -1,0 +1,51 @@
+"""Prompt chunks over a 4-bit pool (the tcgen05 kernel)."""
+import numpy as np
+import pytest
+import torch
+
+import serving_engine_b200 as b200
+from oracle import q4 as oracle
+from tests.test_q4_gpu import DEV, make_batch, metadata
+from tests.tolerance import dtype_key, half_ulp
+
+pytestmark = pytest.mark.gpu
+
+
+def run(b, causal=True):
+    return b200.paged_flash_attention(b["q"], b["pool"][0], b["pool"][1], metadata(b), b["hq"], b["hkv"], b["scale"],
+                                      is_causal=causal)
+
+
+def check_with_nan(b, o, lse):
+    """NaN where the definition has it and nowhere else; the bound of tests/test_q4_gpu.py, V's largest
+    value (below 6 here) in place of the largest that a query sees, for the rest."""
+    p = b["pool"].cpu().numpy()
+    ro, rl, _ = oracle.attention(b["q"].double().cpu().numpy(), p[0], p[1], b["table"], b["starts"], b["q_lens"],
+                                 b["k_lens"], b["pos"], b["scale"])
+    o, lse = o.double().cpu().numpy(), lse.double().cpu().numpy()
+    nan = np.isnan(ro)
+    assert np.array_equal(np.isnan(o), nan)
+    ro, o = np.nan_to_num(ro), np.nan_to_num(o)
+    assert (np.abs(o - ro) <= (2 * 2.0 ** -11 + 2.0 ** -13) * 6 + half_ulp(ro, dtype_key(b["q"].dtype)) + 1e-6).all()
+    assert (np.abs(lse - rl) <= 1e-4 + 1e-5 * np.abs(rl)).all()
+    return nan
+
+
+@pytest.mark.parametrize("d,group", [(64, 4), (128, 4), (128, 8)])
+@pytest.mark.parametrize("q_len,k_len,keys", [
+    (70, 75, [40]), (300, 300, [130, 290]), (150, 700, [3]), (150, 700, [560, 699]),
+    (12, 4000, [3995]), (12, 4000, [1, 3990]),  # one tile of queries, its keys taken in turn
+    (40, 6000, [5970]), (40, 6000, [2000])])    # cut by keys
+def test_nan_of_a_v_group(d, group, q_len, k_len, keys):
+    """A group of V that holds a NaN gives NaN in its own 64 dims, to the queries that see the key, and
+    leaves LSE and the other dims alone."""
+    b = make_batch([k_len], [q_len], 2 * group, 2, d, torch.bfloat16, seed=d + q_len)
+    slots = torch.tensor([int(b["table"][0, j // 16]) * 16 + j % 16 for j in keys], device=DEV)
+    k, v = b200.kv_gather_q4(b["pool"][0], b["pool"][1], slots, d, torch.float32)
+    for i in range(len(keys)):
+        v[i, i % 2, d - 1 if i % 2 else 5] = float("nan")  # head 0's first group, head 1's last
+    b200.kv_append_q4(k.bfloat16(), v.bfloat16(), b["pool"][0], b["pool"][1], slots)
+    o, lse = run(b)
+    nan = check_with_nan(b, o, lse)
+    assert nan.any() and not nan.all()
+    b200.check_device_errors()
