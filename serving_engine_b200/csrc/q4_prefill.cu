@@ -540,13 +540,22 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
             vp[i] = *reinterpret_cast<const uint32_t*>(raw_v + L::kCodes + (8 * h + (i ^ (4 * h))) * 4 * G + gi * 4);
           if (ti.limit < kKeys || ti.none != 0 || diag) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int key = 8 * vc + (i ^ (4 * h));
-              if (key >= ti.limit || none) {
-                vp[i] = 0;
-              } else if (diag && is_nan_pair(vp[i])) {
-                vp[i] = 0;
-                atomicMin(nans + ti.kind / kPlace * 2 + gi, ti.key0 + key);
+            for (int i = 0; i < 8; ++i)
+              if (8 * vc + (i ^ (4 * h)) >= ti.limit || none) vp[i] = 0;
+            bool nan = false;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) nan |= is_nan_pair(vp[i]);
+            if (diag && nan) {
+#pragma unroll 1
+              for (int i = 7; i >= 0; --i) {  // vp[0] in turn
+                if (is_nan_pair(vp[0])) {
+                  atomicMin(nans + ti.kind / kPlace * 2 + gi, ti.key0 + 8 * vc + ((7 - i) ^ (4 * h)));
+                  vp[0] = 0;
+                }
+                const uint32_t first = vp[0];
+#pragma unroll
+                for (int e = 0; e < 7; ++e) vp[e] = vp[e + 1];
+                vp[7] = first;
               }
             }
           }
