@@ -516,8 +516,10 @@ __device__ __forceinline__ void take_blocks(Tile<D, NT>& u, const char* place, i
         float z[NT][4];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const float scale = __low2float(vp[b][pn][h][gi]), low = __high2float(vp[b][pn][h][gi]);
-          const float mid = fmaf(8.f, scale, low);
+          // A group that is NaN is so by its share of the lows alone: in the products it would make the
+          // other group of the tile of sums NaN too.
+          const float2 pair = __half22float2(vp[b][pn][h][gi]);
+          const float scale = fmaxf(pair.x, 0.f), mid = fmaf(8.f, pair.x, pair.y);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll

@@ -31,6 +31,16 @@ def check_with_nan(b, o, lse):
     return nan
 
 
+def nan_in_v(b, keys):
+    """A NaN in one group of one head's V, of each of these keys of row 0."""
+    d = b["q"].shape[-1]
+    slots = torch.tensor([int(b["table"][0, j // 16]) * 16 + j % 16 for j in keys], device=DEV)
+    k, v = b200.kv_gather_q4(b["pool"][0], b["pool"][1], slots, d, torch.float32)
+    for i in range(len(keys)):
+        v[i, i % 2, d - 1 if i % 2 else 5] = float("nan")  # head 0's first group, head 1's last
+    b200.kv_append_q4(k.half(), v.half(), b["pool"][0], b["pool"][1], slots)
+
+
 @pytest.mark.parametrize("d,group", [(64, 4), (128, 4), (128, 8)])
 @pytest.mark.parametrize("q_len,k_len,keys", [
     (70, 75, [40]), (300, 300, [130, 290]), (150, 700, [3]), (150, 700, [560, 699]),
@@ -40,12 +50,24 @@ def test_nan_of_a_v_group(d, group, q_len, k_len, keys):
     """A group of V that holds a NaN gives NaN in its own 64 dims, to the queries that see the key, and
     leaves LSE and the other dims alone."""
     b = make_batch([k_len], [q_len], 2 * group, 2, d, torch.bfloat16, seed=d + q_len)
-    slots = torch.tensor([int(b["table"][0, j // 16]) * 16 + j % 16 for j in keys], device=DEV)
-    k, v = b200.kv_gather_q4(b["pool"][0], b["pool"][1], slots, d, torch.float32)
-    for i in range(len(keys)):
-        v[i, i % 2, d - 1 if i % 2 else 5] = float("nan")  # head 0's first group, head 1's last
-    b200.kv_append_q4(k.bfloat16(), v.bfloat16(), b["pool"][0], b["pool"][1], slots)
+    nan_in_v(b, keys)
     o, lse = run(b)
     nan = check_with_nan(b, o, lse)
     assert nan.any() and not nan.all()
+    b200.check_device_errors()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d,group", [(64, 4), (128, 4), (128, 16), (256, 4)])
+@pytest.mark.parametrize("q_len,k_len,keys", [(1, 75, [0]), (1, 75, [40, 74]), (3, 3000, [1500, 2998]), (5, 90, [88, 89])])
+def test_nan_of_a_v_group_in_rows_of_few_tokens(dtype, d, group, q_len, k_len, keys):
+    """As above, and the same of a token whether its row is a chunk or not."""
+    b = make_batch([k_len], [q_len], 2 * group, 2, d, dtype, seed=d + q_len)
+    nan_in_v(b, keys)
+    o, lse = run(b)
+    nan = check_with_nan(b, o, lse)
+    assert nan.any() and (d == 64 or not nan.all())  # with one group to a head it may be all
+    chunk = {**b, "q": b["q"][-1:].repeat(70, 1, 1), "q_lens": [70], "pos": [k_len - 70]}
+    many, many_lse = run(chunk)
+    assert torch.equal(torch.isnan(many[-1]), torch.isnan(o[-1])) and torch.isfinite(many_lse).all()
     b200.check_device_errors()
