@@ -88,7 +88,7 @@ enum {
   kBarPFull = kBarSFull + kTiles,     // + tile: P(t, j) stored
   kBarODone = kBarPFull + kTiles,     // + tile: the unit's last PV complete
   kBarRawFull = kBarODone + kTiles,   // + stage: rows have come
-  kBarRawEmpty = kBarRawFull + kRawStages,  // + stage: the 256 threads that decode are done with them
+  kBarRawEmpty = kBarRawFull + kRawStages,  // + stage: the 128 threads that decode K, or V, are done with them
   kBarMerge = kBarRawEmpty + kRawStages,  // both warpgroups have come to this point of a unit that they share
   kBarPieceFull,                            // + place: a piece, or the end, is described there
   kBarPieceEmpty = kBarPieceFull + kPieces,  // + place: the copying, the MMA and the 8 softmax warps are done with it
@@ -368,7 +368,7 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
     }
     for (int s = 0; s < kRawStages; ++s) {
       mbar_init(bar + 8 * (kBarRawFull + s), 1);
-      mbar_init(bar + 8 * (kBarRawEmpty + s), 256);
+      mbar_init(bar + 8 * (kBarRawEmpty + s), 128);
     }
     for (int s = 0; s < kPieces; ++s) {
       mbar_init(bar + 8 * (kBarPieceFull + s), 1);
@@ -423,11 +423,10 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
     const int k_at = at * 128 + (((2 * kt) ^ (at & 7)) << 4);
 #pragma unroll 1
     for (int n = 0;; ++n) {
-      const int ik = 2 * n, iv = 2 * n + 1;  // K's and V's places in the run of rows
+      const int ik = 2 * n;  // K's place in the run of rows; V's is the next. Whoever decodes rows gives them back.
       if (!raw_full(ik)) break;
       const TileInfo ti = info[n & 3];
       if (ti.kind & kEnd) break;
-      if ((ti.kind & kDiag) && !raw_full(iv)) break;
       char* tile = k_place();
       if (!tile) break;
       const char* raw_k = sbase + S::oRaw + ik % kRawStages * S::kRaw + (th >> 6) * S::kRawRow;
@@ -500,7 +499,6 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
       }
       if (!tile) break;
       mbar_arrive(bar + 8 * (kBarRawEmpty + ik % kRawStages));
-      mbar_arrive(bar + 8 * (kBarRawEmpty + iv % kRawStages));
     }
   } else if (warp >= 12 && warp < 16) {
     // ------------------------------------------------------------ V
@@ -512,11 +510,10 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
     const int v_at = (vc >> 3) * (D * 128) + vg * 1024 + ((vc & 7) << 4);
 #pragma unroll 1
     for (int n = 0;; ++n) {
-      const int s = n % kStages, ik = 2 * n, iv = 2 * n + 1;
-      if (!raw_full(ik)) break;
+      const int s = n % kStages, iv = 2 * n + 1;
+      if (!raw_full(iv)) break;
       const TileInfo ti = info[n & 3];
-      mbar_arrive(bar + 8 * (kBarRawEmpty + ik % kRawStages));
-      if ((ti.kind & kEnd) || !raw_full(iv)) break;
+      if (ti.kind & kEnd) break;
       const bool diag = ti.kind & kDiag;
       // V of 8 tokens, 8 dims of each group: one 16-byte chunk a dim, rows of 64 keys. The tokens are in the
       // places' order: of a block's second half the last four come first.
@@ -677,13 +674,16 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
           }
         }
       }
-      const int s = i % kRawStages;
-      if (!failed && (i < kRawStages || wait_or_flag(bar + 8 * (kBarRawEmpty + s), (i / kRawStages - 1) & 1, failed))) {
+      for (int last = i + 2; i < last && !failed; ++i) {  // the end, to K's warps and to V's
+        const int s = i % kRawStages;
+        if (i >= kRawStages && !wait_or_flag(bar + 8 * (kBarRawEmpty + s), (i / kRawStages - 1) & 1, failed)) break;
         if (lane == 0) {
           info[n & 3].kind = kEnd;
           mbar_arrive(bar + 8 * (kBarRawFull + s));
         }
-      } else {  // whoever would have waited for the copies has given up: leave none in flight
+        __syncwarp();
+      }
+      if (failed) {  // whoever would have waited for the copies has given up: leave none in flight
         for (int k = max(0, i - kRawStages); k < i; ++k)
           mbar_wait_bounded(bar + 8 * (kBarRawFull + k % kRawStages), (k / kRawStages) & 1, 1u << 16);
       }

@@ -5,7 +5,7 @@ import torch
 
 import serving_engine_b200 as b200
 from oracle import q4 as oracle
-from tests.test_q4_gpu import DEV, make_batch, metadata
+from tests.test_q4_gpu import DEV, check, make_batch, metadata
 from tests.tolerance import dtype_key, half_ulp
 
 pytestmark = pytest.mark.gpu
@@ -70,4 +70,22 @@ def test_nan_of_a_v_group_in_rows_of_few_tokens(dtype, d, group, q_len, k_len, k
     chunk = {**b, "q": b["q"][-1:].repeat(70, 1, 1), "q_lens": [70], "pos": [k_len - 70]}
     many, many_lse = run(chunk)
     assert torch.equal(torch.isnan(many[-1]), torch.isnan(o[-1])) and torch.isfinite(many_lse).all()
+    b200.check_device_errors()
+
+
+@pytest.mark.parametrize("d,hq,hkv", [(64, 8, 4), (128, 16, 4)])
+def test_the_same_bits_every_time(d, hq, hkv):
+    """Copies, decoding and products go on at the same time in warps of their own: what they hand on does
+    not depend on which is faster, beside other work or alone."""
+    b = make_batch([2500, 700, 1300, 90, 3000], [300, 64, 129, 90, 200], hq, hkv, d, torch.bfloat16, seed=1)
+    o, lse = run(b)
+    check(b, o, lse)
+    side = torch.cuda.Stream()
+    busy = torch.randn(1 << 24, device=DEV)
+    for i in range(60):
+        if i % 2:
+            with torch.cuda.stream(side):
+                busy.mul_(1.0001)
+        again = run(b)
+        assert torch.equal(o, again[0]) and torch.equal(lse, again[1])
     b200.check_device_errors()
