@@ -372,7 +372,9 @@ SEB_API int seb_qk_norm_rope_append(const void* qkv, int64_t qkv_stride_token, i
  * that see its key, one of K all of their O and LSE. Rows' token ranges must not overlap. A block id out of range sets
  * SEB_ERRBIT_BLOCK_ID and its keys count as masked; a k_len beyond the table sets
  * SEB_ERRBIT_KLEN and ends there; a row outside total_query sets SEB_ERRBIT_META and
- * is skipped. Rows of q and out are 16-byte aligned.
+ * is skipped. Rows of q and out are 16-byte aligned. SEB_EUNSUPPORTED where the rows that no
+ * chunk kernel takes (all at head_dim 256, else those of few tokens) could, with tables of
+ * max_blocks, come to 2^32 pairs of a tile of tokens and two blocks.
  * workspace: seb_paged_attention_q4_workspace_size(...) bytes, 16-byte aligned, of any
  * content. counter_slot: 0 .. SEB_Q4_COUNTER_SLOTS - 1, a set of the library's own
  * arrival counters on the current device. Calls that may overlap on the GPU need a workspace

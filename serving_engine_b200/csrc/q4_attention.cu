@@ -940,8 +940,11 @@ int launch(Q4Params& p, void* workspace, int64_t bytes, cudaStream_t s) {
   p.by_group = (65536 + p.group - 1) / p.group;
   const int rc = set_smem_limit_once<kern>(smem);
   if (rc != SEB_OK) return rc;
-  // no more CTAs than the longest rows that the table allows would fill
-  const int64_t tiles = ((int64_t)p.total_query + (int64_t)p.num_rows * (p.tile - 1)) / p.tile;
+  // no more CTAs than the longest rows that the table allows would fill; where there may be chunks, rows that
+  // are none have fewer tokens than one
+  int64_t tiles = ((int64_t)p.total_query + (int64_t)p.num_rows * (p.tile - 1)) / p.tile;
+  if (p.chunk_from > 0)
+    tiles = std::min<int64_t>(tiles, (int64_t)p.num_rows * (((p.chunk_from - 1) / p.group + p.tile - 1) / p.tile));
   const int64_t pairs = tiles * p.hkv * ((p.max_blocks + 1) / 2 + kUnitCost);
   if (pairs > 0xffff0000ll) {
     set_error("seb_paged_attention_q4: %lld tiles of %lld blocks are too much work for one call", (long long)tiles * p.hkv,
