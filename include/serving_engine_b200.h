@@ -369,10 +369,11 @@ SEB_API int seb_qk_norm_rope_append(const void* qkv, int64_t qkv_stride_token, i
  * j < k_lens[r] (causal: j <= position). q, out: bf16 or fp16; the sums are fp32. A
  * query that sees no key gets O = 0 and LSE = -inf; tokens of no row are left as they
  * are. A group of V that reads back as NaN makes its own 64 dims of O NaN for the queries
- * that see its key, one of K all of their O and LSE. Rows' token ranges must not overlap. A block id out of range sets
- * SEB_ERRBIT_BLOCK_ID and its keys count as masked; a k_len beyond the table sets
- * SEB_ERRBIT_KLEN and ends there; a row outside total_query sets SEB_ERRBIT_META and
- * is skipped. Rows of q and out are 16-byte aligned. SEB_EUNSUPPORTED where the rows that no
+ * that see its key, one of K all of their O and LSE. Rows' token ranges must not overlap
+ * (rows of few tokens whose work so passes 32 bits set SEB_ERRBIT_META and are skipped).
+ * A block id out of range sets SEB_ERRBIT_BLOCK_ID and its keys count as masked; a k_len
+ * beyond the table sets SEB_ERRBIT_KLEN and ends there; a row outside total_query sets
+ * SEB_ERRBIT_META and is skipped. Rows of q and out are 16-byte aligned. SEB_EUNSUPPORTED where the rows that no
  * chunk kernel takes (all at head_dim 256, else those of few tokens) could, with tables of
  * max_blocks, come to 2^32 pairs of a tile of tokens and two blocks.
  * workspace: seb_paged_attention_q4_workspace_size(...) bytes, 16-byte aligned, of any

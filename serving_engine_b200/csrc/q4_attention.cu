@@ -59,6 +59,10 @@ constexpr float kScaleTop = 15.f, kScalePlace = 8.f;
 constexpr int kMaxCtas = 512;
 __device__ int32_t g_q4_counters[SEB_Q4_COUNTER_SLOTS][kMaxCtas * 4];
 
+// What the units of a call may come to, in such places: less than 32 bits hold by what rounding each thread's
+// sum down to 2^12 hides (512 threads at most).
+constexpr uint32_t kMostWork = 0xffe00000u;
+
 // A unit's length in the run of all units: kUnitCost places that stand for no blocks, then its pairs.
 __device__ __forceinline__ uint32_t length_of(const Row& w) { return w.pairs + kUnitCost; }
 __device__ __forceinline__ uint32_t pairs_of(const Q4Params& p, const Row& w) { return w.tiles * p.hkv * length_of(w); }
@@ -81,8 +85,9 @@ struct Smem {
   static constexpr int kRing = STAGES * kStage > kPartBytes ? STAGES * kStage : kPartBytes;
   static constexpr int kWarp = (kRing + kPartBytes + 127) / 128 * 128;
   static constexpr int kParts = 0;                                     // Part[NW][2]
-  static constexpr int kPrefix = kParts + NW * 2 * (int)sizeof(Part);  // uint32 [NW * 32 + 1]
-  static constexpr int kBars = kPrefix + (NW * 32 + 2) * 4;
+  static constexpr int kPrefix = kParts + NW * 2 * (int)sizeof(Part);  // uint32 [NW * 32 + 2]
+  static constexpr int kMuch = kPrefix + (NW * 32 + 2) * 4;            // uint32 [NW]
+  static constexpr int kBars = kMuch + NW * 4;
   static constexpr int kWarps = (kBars + NW * STAGES * 8 + 127) / 128 * 128;
   static constexpr int kBytes = kWarps + NW * kWarp;
 };
@@ -583,14 +588,18 @@ __global__ void __launch_bounds__(NW * 32, CTAS) q4_attention_kernel(const Q4Par
   // ---- the units of all rows, and this warp's run of blocks
   const int chunk = (p.num_rows + NW * 32 - 1) / (NW * 32);  // rows that a thread sums up
   {
-    uint32_t sum = 0, bad = 0;
+    uint32_t bad = 0;
+    uint64_t all = 0;
 #pragma unroll 1
     for (int r = tid * chunk; r < min((tid + 1) * chunk, p.num_rows); ++r) {
       const Row row = row_of<false>(p, r, &bad);
-      sum += pairs_of(p, row);
+      all += pairs_of(p, row);
       if (r == 0) prefix[NW * 32 + 1] = length_of(row);
     }
     if (bad && blockIdx.x == 0) atomic_or_err(p.err, bad);
+    uint32_t sum = (uint32_t)all;
+    const uint32_t much = __reduce_add_sync(kFull, (uint32_t)min(all >> 12, (uint64_t)1 << 22));
+    if (lane == 0) reinterpret_cast<uint32_t*>(smem + S::kMuch)[warp] = much;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
       const uint32_t o = __shfl_up_sync(kFull, sum, off);
@@ -601,11 +610,16 @@ __global__ void __launch_bounds__(NW * 32, CTAS) q4_attention_kernel(const Q4Par
     if (lane < 2) parts[warp * 2 + lane].end = 0;
   }
   __syncthreads();
-  uint32_t total = 0, before = 0;
+  uint32_t total = 0, before = 0, much = 0;
 #pragma unroll
   for (int w = 0; w < NW; ++w) {
     if (w == warp) before = total;
     total += prefix[(w + 1) * 32];
+    much += reinterpret_cast<const uint32_t*>(smem + S::kMuch)[w];
+  }
+  if (much > kMostWork >> 12) {  // rows whose tokens overlap: the sums have passed 32 bits
+    if (blockIdx.x == 0 && tid == 0) atomic_or_err(p.err, SEB_ERRBIT_META);
+    return;
   }
   __syncthreads();
   prefix[tid + 1] += before;
@@ -654,7 +668,7 @@ __global__ void __launch_bounds__(NW * 32, CTAS) q4_attention_kernel(const Q4Par
         row = row_of<false>(p, ++r, &bad);
         len = pairs_of(p, row);
       }
-      if (off >= len) break;  // rows that overlap, beyond what can be counted
+      if (off >= len) break;
       const uint32_t length = length_of(row);
       const uint32_t unit = off / length;  // tiles of one kv head are neighbours: they read the same blocks
       const uint32_t place = off - unit * length, n = min(length - place, stop - pos);
@@ -946,7 +960,7 @@ int launch(Q4Params& p, void* workspace, int64_t bytes, cudaStream_t s) {
   if (p.chunk_from > 0)
     tiles = std::min<int64_t>(tiles, (int64_t)p.num_rows * (((p.chunk_from - 1) / p.group + p.tile - 1) / p.tile));
   const int64_t pairs = tiles * p.hkv * ((p.max_blocks + 1) / 2 + kUnitCost);
-  if (pairs > 0xffff0000ll) {
+  if (pairs > (int64_t)kMostWork) {
     set_error("seb_paged_attention_q4: %lld tiles of %lld blocks are too much work for one call", (long long)tiles * p.hkv,
               (long long)p.max_blocks);
     return SEB_EUNSUPPORTED;

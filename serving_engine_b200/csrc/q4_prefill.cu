@@ -319,6 +319,7 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
     for (int r = tid * chunk; r < min((tid + 1) * chunk, p.num_rows); ++r) {
       const Row row = row_of<true>(p, r, &bad);
       sum += length_of(p, row, cut);
+      if (!cut) sum = min(sum, 1u << 22);  // rows whose tokens overlap: 640 such sums still fit 32 bits
       if (cut && row.q_len > 0) atomicMax(longest, places_of(blocks_of(p, row, pairs_of(p, row) - 1)));
     }
 #pragma unroll
