@@ -410,7 +410,7 @@ SEB_API int seb_paged_attention_q4(const void* q, int64_t q_stride_token, int64_
  * SEB_ERRBIT_NOBLOCK is set; a k_len beyond the table sets SEB_ERRBIT_KLEN (slots -1,
  * no block taken); negative lengths (taken as 0), more tokens than total_query and a
  * free_state outside the ring (taken as empty) set SEB_ERRBIT_META.
- * num_rows <= 16384. */
+ * num_rows <= 16384. No output, block_table among them, overlaps another array. */
 SEB_API int seb_step_tables(const int32_t* q_lens, const int32_t* context_lens, int32_t num_rows,
                             int32_t total_query, int32_t* block_table, int64_t block_table_stride,
                             int64_t max_blocks, const int32_t* free_ids, int32_t free_capacity,

@@ -200,11 +200,35 @@ extern "C" int seb_step_tables(const int32_t* q_lens, const int32_t* context_len
                 "seb_step_tables: bad block table shape (max_blocks %lld, stride %lld)", (long long)max_blocks,
                 (long long)block_table_stride);
   SEB_CHECK_ARG(free_capacity > 0, "seb_step_tables: free_capacity must be positive");
-  SEB_CHECK_ARG(free_ids && free_state && free_next && free_state != free_next,
-                "seb_step_tables: free_ids, free_state and a separate free_next are required");
+  SEB_CHECK_ARG(free_ids && free_state && free_next, "seb_step_tables: free_ids, free_state and free_next are required");
   SEB_CHECK_ARG(num_rows == 0 || (q_lens && context_lens && block_table && q_starts && k_lens && q_pos_offsets),
                 "seb_step_tables: NULL row array");
   SEB_CHECK_ARG(total_query == 0 || (item_row && positions && slot_mapping), "seb_step_tables: NULL token array");
+  // Every CTA reads what the rows hold while others write already: no output may lie over an input, nor over
+  // another output.
+  const struct {
+    const void* at;
+    int64_t bytes;
+    const char* name;
+  } arrays[] = {{q_lens, 4ll * num_rows, "q_lens"},
+                {context_lens, 4ll * num_rows, "context_lens"},
+                {free_ids, 4ll * free_capacity, "free_ids"},
+                {free_state, 8, "free_state"},
+                {block_table, num_rows ? 4 * ((num_rows - 1) * block_table_stride + max_blocks) : 0, "block_table"},
+                {q_starts, 4ll * num_rows, "q_starts"},
+                {k_lens, 4ll * num_rows, "k_lens"},
+                {q_pos_offsets, 4ll * num_rows, "q_pos_offsets"},
+                {item_row, 4ll * total_query, "item_row"},
+                {positions, 8ll * total_query, "positions"},
+                {slot_mapping, 8ll * total_query, "slot_mapping"},
+                {free_next, 8, "free_next"}};
+  constexpr int kInputs = 4, kArrays = sizeof(arrays) / sizeof(arrays[0]);
+  for (int i = kInputs; i < kArrays; ++i)
+    for (int j = 0; j < i; ++j) {
+      const uintptr_t a = reinterpret_cast<uintptr_t>(arrays[i].at), b = reinterpret_cast<uintptr_t>(arrays[j].at);
+      SEB_CHECK_ARG(a + arrays[i].bytes <= b || b + arrays[j].bytes <= a || !arrays[i].bytes || !arrays[j].bytes,
+                    "seb_step_tables: %s overlaps %s", arrays[i].name, arrays[j].name);
+    }
   if (num_rows > kMaxRows) {
     set_error("seb_step_tables: %d rows above %d", num_rows, kMaxRows);
     return SEB_EUNSUPPORTED;

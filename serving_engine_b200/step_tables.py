@@ -50,8 +50,9 @@ class StepTables:
         [rows]); new blocks come from the ring free_ids (int32), of which free_state
         (int32 [2]: head, count) are free, and are written into block_table (int32 [rows,
         max_blocks], unit column stride). ``self.free_state`` is the state after the step:
-        copy it over free_state, or pass it to another StepTables' next build. Returns the
-        metadata dict of build_paged_batch_metadata. One launch.
+        copy it over free_state, or pass it to another StepTables' next build. The same goes
+        for context_lens and k_lens: this object's own buffers are no input of its build.
+        Returns the metadata dict of build_paged_batch_metadata. One launch.
 
         The host can follow without reading back: rows take ceil(k_len / 16) -
         ceil(context / 16) blocks each, in row order from the head of the ring.
