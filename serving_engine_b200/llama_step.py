@@ -63,6 +63,8 @@ class FusedLlamaStep:
                     raise ValueError("FusedLlamaStep: projections with bias are not supported")
                 if getattr(cfg, "hidden_act", "silu") != "silu":
                     raise ValueError(f"FusedLlamaStep: activation {cfg.hidden_act} is not supported (silu)")
+                for norm in (getattr(at, "q_norm", None), getattr(at, "k_norm", None)):
+                    self._check_head_norm(norm)
                 self.layers.append({
                     "wqkv": torch.cat([at.q_proj.weight, at.k_proj.weight, at.v_proj.weight]).contiguous(),
                     "wo": at.o_proj.weight,
@@ -74,6 +76,24 @@ class FusedLlamaStep:
                     "qn": getattr(getattr(at, "q_norm", None), "weight", None),
                     "kn": getattr(getattr(at, "k_norm", None), "weight", None),
                 })
+
+    def _check_head_norm(self, norm) -> None:
+        """Refuse a norm of query or key heads that is not x * rsqrt(mean(x^2) + eps) * weight with
+        the model's eps (one by 1 + weight, say): its value at two sizes of x tells."""
+        if norm is None or not callable(norm):
+            return
+        weight = norm.weight.float()
+        if weight.shape != (self.head_dim,):
+            raise ValueError(f"FusedLlamaStep: norm weights of query and key heads must be [{self.head_dim}], "
+                             f"got {list(weight.shape)}")
+        for size in (1.0, 2.0 * self.eps ** 0.5):
+            sign = 1.0 - 2.0 * (torch.arange(self.head_dim, device=weight.device) % 3 == 0)
+            x = (size * sign).to(self.dtype)
+            got, x = norm(x[None])[0].float(), x.float()
+            want = x * (x.square().mean() + self.eps).rsqrt() * weight
+            if not torch.allclose(got, want, rtol=2.0 ** -6, atol=2.0 ** -6 * float(weight.abs().max()) + 1e-6):
+                raise ValueError(f"FusedLlamaStep: {type(norm).__name__} of query or key heads is not an RMSNorm "
+                                 f"x * rsqrt(mean(x^2) + {self.eps}) * weight")
 
     def rotary(self, positions: torch.Tensor):
         """cos, sin [rows, head_dim] as HF's rotary embedding computes them (fp32,
