@@ -48,7 +48,8 @@ constexpr uint32_t kMinRun = 2;
 // What a unit's start and end cost a warp, in pairs of blocks. 256 rows of 32 to 4352 keys, heads of 64:
 // 0: 55.6 us, 1: 49.2, 2: 45.1, 3: 44.8, 4: 44.6, 6: 45.9; 64 rows of 1024 to 8192, heads of 128: 1 84.2, 2 83.6, 3 83.6.
 constexpr uint32_t kUnitCost = 2;
-constexpr float kThreshold = 8.f;  // scores may exceed the reference by 2^8 before it is moved
+constexpr float kNoMax = -FLT_MAX;  // no score yet: any score is above it by more than the threshold
+constexpr float kThreshold = 8.f;   // scores may exceed the reference by 2^8 before it is moved
 // p * V's scale stays below 2^15, and the largest of them is put at [2^8, 2^9) when its power of two is
 // taken: what is 2^-22 of that one is still not subnormal.
 constexpr float kScaleTop = 15.f, kScalePlace = 8.f;
@@ -214,7 +215,7 @@ struct Tile {
   float qs[GR][NT][2];        // sum of q over a group, columns 8 nt + 2 t and the next
   float ch[NT][2];            // what brings a score to log2 units
   float m[NT][2], l[NT][2];   // reference, and this lane's share of the sum
-  float v_exp[NT][2];         // exponent that brings p * scale to fp16's range; inf: no key yet, and m is 0
+  float v_exp[NT][2];         // exponent that brings p * scale to fp16's range; inf: no key yet
   float low[GR][NT][2];       // this lane's share of sum p (low + 8 scale)
   float one[(GR + 1) / 2][NT][4];  // sum of the rounded p * scale, two groups to a tile
   float o[GR][4][NT][4];      // sum of those and the codes: n of a dim, and 16 n of the next
@@ -397,9 +398,9 @@ __device__ __forceinline__ void take_blocks(Tile<D, NT>& u, const char* place, i
       }
   }
 
-  // Scores count from their column's reference from here. The largest of each column that this lane
-  // has; what p * scale may be is first bounded by it and the largest scale, and only where that
-  // bound calls for a move worked out key by key: a column moves for keys that it sees and no others.
+  // The largest score of each column that this lane has. What p * scale may be is first bounded by it and
+  // the largest scale, and worked out key by key only where that bound calls for a move: a column moves
+  // for keys that it sees and no others.
   __half2 vp[KB][P][2][G];  // of keys g and g + 8
   float top[NT][2];
   __half2 most[KB][2];
@@ -415,10 +416,6 @@ __device__ __forceinline__ void take_blocks(Tile<D, NT>& u, const char* place, i
           most[b][h] = pn + gi == 0 ? vp[b][pn][h][gi] : __hmax2(most[b][h], vp[b][pn][h][gi]);
       }
   auto log2_scale = [](__half2 pair) { return log2_fast(fmaxf(__low2float(pair), power2(-30))); };  // a NaN counts as 0
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-    for (int h = 0; h < 2; ++h) top[nt][h] = -INFINITY;
   __half2 largest = most[0][0];
 #pragma unroll
   for (int b = 0; b < KB; ++b)
@@ -428,55 +425,49 @@ __device__ __forceinline__ void take_blocks(Tile<D, NT>& u, const char* place, i
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int c = 2 * h; c < 2 * h + 2; ++c) {
-          x[b][nt][c] -= u.m[nt][c & 1];
-          top[nt][c & 1] = fmaxf(top[nt][c & 1], x[b][nt][c]);
-        }
+        for (int c = 2 * h; c < 2 * h + 2; ++c)
+          top[nt][c & 1] = b + h == 0 ? x[b][nt][c] : fmaxf(top[nt][c & 1], x[b][nt][c]);
     }
   const float above = log2_scale(largest) - (kScaleTop - 0.01f);
   bool move = false;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-    for (int h = 0; h < 2; ++h) move |= top[nt][h] > kThreshold || top[nt][h] + above > -u.v_exp[nt][h];
+    for (int h = 0; h < 2; ++h) {
+      const float over = top[nt][h] - u.m[nt][h];
+      move |= over > kThreshold || over + above > -u.v_exp[nt][h];
+    }
   if (__any_sync(kFull, move)) {
     // move the references of the columns that need it
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        float mx = top[nt][h], z = -INFINITY;  // log2 of the largest p * scale
+        float mx = top[nt][h];
 #pragma unroll
-        for (int b = 0; b < KB; ++b) {
-          z = fmaxf(z, x[b][nt][h] + log2_scale(most[b][0]));
-          z = fmaxf(z, x[b][nt][h + 2] + log2_scale(most[b][1]));
-        }
-#pragma unroll
-        for (int k = 4; k <= 16; k <<= 1) {
-          mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, k));
-          z = fmaxf(z, __shfl_xor_sync(kFull, z, k));
-        }
+        for (int k = 4; k <= 16; k <<= 1) mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, k));
         const bool first = u.v_exp[nt][h] == INFINITY;
         float up = 0.f;
-        if (mx > kThreshold || (first && mx > -INFINITY)) {
-          const float now = u.m[nt][h] + mx;
-          up = now - u.m[nt][h];
-          u.m[nt][h] = now;
+        if (mx - u.m[nt][h] > kThreshold) {
+          up = mx - u.m[nt][h];
+          u.m[nt][h] = mx;
         }
+        float z = -INFINITY;  // log2 of the largest p * scale
+#pragma unroll
+        for (int b = 0; b < KB; ++b) {
+          z = fmaxf(z, x[b][nt][h] - u.m[nt][h] + log2_scale(most[b][0]));
+          z = fmaxf(z, x[b][nt][h + 2] - u.m[nt][h] + log2_scale(most[b][1]));
+        }
+#pragma unroll
+        for (int k = 4; k <= 16; k <<= 1) z = fmaxf(z, __shfl_xor_sync(kFull, z, k));
         // what was summed up so far went down by 2^up, and its power of two up by as much
         float e = first ? INFINITY : kScalePlace - floorf(kScalePlace - u.v_exp[nt][h] - up);
-        z -= up;
         if (z > kScaleTop - e) e = kScalePlace - floorf(z);
         if (!first || z > -INFINITY) e = fminf(fmaxf(e, -20.f), 100.f);
         const float fix = first ? 0.f : fast_exp2(-up);  // nothing is summed up yet at first
         const float z_fix = first ? 0.f : fix * (power_of(e) / power_of(u.v_exp[nt][h]));
         u.v_exp[nt][h] = e;
         u.l[nt][h] *= fix;
-#pragma unroll
-        for (int b = 0; b < KB; ++b) {
-          x[b][nt][h] -= up;
-          x[b][nt][h + 2] -= up;
-        }
 #pragma unroll
         for (int gr = 0; gr < GR; ++gr) {
           u.low[gr][nt][h] *= fix;
@@ -504,7 +495,7 @@ __device__ __forceinline__ void take_blocks(Tile<D, NT>& u, const char* place, i
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-      for (int c = 0; c < 4; ++c) x[b][nt][c] = fast_exp2(x[b][nt][c]);
+      for (int c = 0; c < 4; ++c) x[b][nt][c] = fast_exp2(x[b][nt][c] - u.m[nt][c & 1]);
       u.l[nt][0] += x[b][nt][0] + x[b][nt][2];
       u.l[nt][1] += x[b][nt][1] + x[b][nt][3];
     }
@@ -726,7 +717,8 @@ __global__ void __launch_bounds__(NW * 32, CTAS) q4_attention_kernel(const Q4Par
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          u.m[nt][h] = u.l[nt][h] = 0.f;
+          u.m[nt][h] = kNoMax;
+          u.l[nt][h] = 0.f;
           u.v_exp[nt][h] = INFINITY;
 #pragma unroll
           for (int gr = 0; gr < GR; ++gr) u.low[gr][nt][h] = 0.f;
