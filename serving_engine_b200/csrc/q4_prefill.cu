@@ -87,8 +87,10 @@ enum {
   kBarSFull = kBarVEmpty + kStages,   // + tile: S(t, j) complete, and every MMA before it
   kBarPFull = kBarSFull + kTiles,     // + tile: P(t, j) stored
   kBarODone = kBarPFull + kTiles,     // + tile: the unit's last PV complete
-  kBarRawFull = kBarODone + kTiles,   // + stage: rows have come
-  kBarRawEmpty = kBarRawFull + kRawStages,  // + stage: the 128 threads that decode K, or V, are done with them
+  // + n % kRawStages for K's rows of tile n, and kRawStages on for V's: rows have come. A place holds K's and V's in
+  // turn; whoever waits for one kind alone needs a barrier whose every phase is of that kind.
+  kBarRawFull = kBarODone + kTiles,
+  kBarRawEmpty = kBarRawFull + 2 * kRawStages,  // + place: the 128 threads that decode K, or V, are done with them
   kBarMerge = kBarRawEmpty + kRawStages,  // both warpgroups have come to this point of a unit that they share
   kBarPieceFull,                            // + place: a piece, or the end, is described there
   kBarPieceEmpty = kBarPieceFull + kPieces,  // + place: the copying, the MMA and the 8 softmax warps are done with it
@@ -369,6 +371,7 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
     }
     for (int s = 0; s < kRawStages; ++s) {
       mbar_init(bar + 8 * (kBarRawFull + s), 1);
+      mbar_init(bar + 8 * (kBarRawFull + kRawStages + s), 1);
       mbar_init(bar + 8 * (kBarRawEmpty + s), 128);
     }
     for (int s = 0; s < kPieces; ++s) {
@@ -399,9 +402,10 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
     __syncwarp();
     if (lane == 0) mbar_arrive(bar + 8 * (kBarPieceEmpty + i % kPieces));
   };
-  auto raw_full = [&](int i) {
-    return wait_or_flag(bar + 8 * (kBarRawFull + i % kRawStages), (i / kRawStages) & 1, failed);
-  };
+  // Of place i of the run K(0), V(0), K(1), ...
+  auto raw_full_bar = [&](int i) { return bar + 8 * (kBarRawFull + (i & 1) * kRawStages + (i >> 1) % kRawStages); };
+  auto raw_full_parity = [&](int i) { return ((i >> 1) / kRawStages) & 1; };
+  auto raw_full = [&](int i) { return wait_or_flag(raw_full_bar(i), raw_full_parity(i), failed); };
   if (warp >= 8 && warp < 12) {
     // ------------------------------------------------------------ K
     registers_down<kRegsK>();
@@ -665,13 +669,13 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
                                            ((j + 1) * kKeys > min(w.sees, w.k_len) ? kDiag : 0) |
                                            ip % kPieces * kPlace,
                                        j * kKeys};
-              mbar_arrive_expect_tx(bar + 8 * (kBarRawFull + s), __popc(have) * L::kRow);
+              mbar_arrive_expect_tx(raw_full_bar(i), __popc(have) * L::kRow);
             }
             __syncwarp();
             if (lane < 8 && id >= 0)
               bulk_g2s(base + S::oRaw + s * S::kRaw + lane * S::kRawRow,
                        (is_v ? p.v_cache : p.k_cache) + ((int64_t)id * p.hkv + w.kvh) * L::kRow, L::kRow,
-                       bar + 8 * (kBarRawFull + s));
+                       raw_full_bar(i));
           }
         }
       }
@@ -680,13 +684,13 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
         if (i >= kRawStages && !wait_or_flag(bar + 8 * (kBarRawEmpty + s), (i / kRawStages - 1) & 1, failed)) break;
         if (lane == 0) {
           info[n & 3].kind = kEnd;
-          mbar_arrive(bar + 8 * (kBarRawFull + s));
+          mbar_arrive(raw_full_bar(i));
         }
         __syncwarp();
       }
       if (failed) {  // whoever would have waited for the copies has given up: leave none in flight
         for (int k = max(0, i - kRawStages); k < i; ++k)
-          mbar_wait_bounded(bar + 8 * (kBarRawFull + k % kRawStages), (k / kRawStages) & 1, 1u << 16);
+          mbar_wait_bounded(raw_full_bar(k), raw_full_parity(k), 1u << 16);
       }
       goto done;
     }
