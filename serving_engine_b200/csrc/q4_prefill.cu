@@ -865,10 +865,11 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
       mbar_arrive(bar + 8 * (kBarQFull + qt));
       return copysignf(fminf(fabsf(p.scale_log2) * power2(ex), FLT_MAX), p.scale_log2);
     };
-    // The CTA's first piece from the ip-th on that has work for this warpgroup; rows that see nothing are written here.
-    auto next_unit = [&](int& ip) -> const Unit* {
+    // The CTA's first piece from the ip-th on, and before the until-th, that has work for this warpgroup; rows
+    // that see nothing are written here.
+    auto next_unit = [&](int& ip, int until) -> const Unit* {
 #pragma unroll 1
-      for (;; ++ip) {
+      for (; ip < until; ++ip) {
         const Unit* at = piece(ip);
         if (!at || qt < at->slots) return at;
         const Unit& w = *at;
@@ -882,12 +883,19 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
         }
         piece_done(ip);
       }
+      return nullptr;
     };
     int ip = 0, ip_next = 0;
-    const Unit* at = next_unit(ip_next);
-    float c_next = at ? store_query(*at) : 0.f;
+    const Unit* at = nullptr;
+    float c_next = 0.f;
+    bool later = true;  // the next unit is still to be looked for
 #pragma unroll 1
-    while (at) {
+    for (;;) {
+      if (later) {
+        at = next_unit(ip_next, INT32_MAX);
+        if (at) c_next = store_query(*at);
+      }
+      if (!at) break;
       const Unit& w = *at;
       ip = ip_next;
       const float c = c_next;
@@ -1006,8 +1014,10 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
         if (lane == 0) mbar_arrive(bar + 8 * (kBarPFull + qt));
       }
       // ---- the next unit's query, so that its first scores come while this one's O is written
+      // A piece that takes this one's place is described only once this one is given back: not waited for here.
       ++ip_next;
-      at = __any_sync(kFull, failed) ? nullptr : next_unit(ip_next);
+      at = __any_sync(kFull, failed) ? nullptr : next_unit(ip_next, ip + kPieces);
+      later = ip_next == ip + kPieces;
       if (at) c_next = store_query(*at);
       // ---- O is final
       wait_or_flag(bar + 8 * (kBarODone + qt), nd & 1, failed);

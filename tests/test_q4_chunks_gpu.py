@@ -89,3 +89,35 @@ def test_the_same_bits_every_time(d, hq, hkv):
         again = run(b)
         assert torch.equal(o, again[0]) and torch.equal(lse, again[1])
     b200.check_device_errors()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("first", [(64, 200), (12, 400)])      # two tiles of queries; one, its keys taken in turn
+@pytest.mark.parametrize("idle", [(12, 40), (64, 0), (20, 0)])  # a tile for one warpgroup; queries that see no key
+def test_units_without_work_for_a_warpgroup(d, first, idle):
+    """Many units in a row that one warpgroup of a CTA, or both, have nothing to do for, between units that they
+    share: more than there are places to describe units ahead."""
+    hkv, group = 4, 4
+    rows = [first] * 80 + [idle] * 330 + [first] * 45 + [idle] * 200
+    q_lens, k_lens = [q for q, _ in rows], [k for _, k in rows]
+    b = make_batch(k_lens, q_lens, hkv * group, hkv, d, torch.float16, seed=d)
+    b["pos"] = [k - q if k else 0 for q, k in rows]
+    out, lse = run(b)
+    b200.check_device_errors()
+    slots = (torch.tensor(b["table"], device=DEV).long()[:, :, None] * 16 + torch.arange(16, device=DEV)).view(len(rows), -1)
+    for shape in {first, idle}:
+        which = [r for r, x in enumerate(rows) if x == shape]
+        nq, nk = shape
+        tokens = (torch.tensor([b["starts"][r] for r in which], device=DEV)[:, None] + torch.arange(nq, device=DEV)).view(-1)
+        o, l = out[tokens].view(len(which), nq, -1, d), lse[tokens].view(len(which), nq, -1)
+        if nk == 0:
+            assert (o == 0).all() and torch.isneginf(l).all()
+            continue
+        k, v = b200.kv_gather_q4(b["pool"][0], b["pool"][1], slots[which, :nk].reshape(-1), d, torch.float32)
+        k, v = (x.view(len(which), nk, hkv, d).double().repeat_interleave(group, 2) for x in (k, v))
+        s = torch.einsum("rqhd,rkhd->rhqk", b["q"][tokens].view(len(which), nq, -1, d).double(), k) * b["scale"]
+        s = s.masked_fill(torch.ones(nq, nk, dtype=torch.bool, device=DEV).triu(nk - nq + 1), -torch.inf)
+        ref = torch.einsum("rhqk,rkhd->rqhd", s.softmax(-1), v)
+        # the bound of tests/test_q4_gpu.py, V below 6
+        assert ((o.double() - ref).abs() <= (2 * 2.0 ** -11 + 2.0 ** -13) * 6 + 2.0 ** -11 * ref.abs() + 1e-6).all()
+        assert ((l.double() - s.logsumexp(-1).transpose(1, 2)).abs() <= 1e-4).all()
