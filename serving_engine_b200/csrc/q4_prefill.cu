@@ -23,7 +23,7 @@
 // Rounding to 16 bits: a query to fp16 after a power of two of its own that puts its largest
 // element at 2^14 (exact, see q4_attention.cu; the power is part of the row's scale); K and
 // V values once to fp16 (unit 2^-11; clamped to +-65504), which is what a 16-bit pool would
-// hold; P to fp16, below 2^8. Scores, O and all sums are fp32. One rounding of K costs a
+// hold; P to fp16, below 2^15. Scores, O and all sums are fp32. One rounding of K costs a
 // score about 2e-4 at unit scores, and LSE that over the root of the keys seen; units whose
 // first token sees few keys take K as the sum of two fp16 numbers, one product for each.
 //
@@ -52,7 +52,9 @@ constexpr int kThreads = 640;  // 5 warpgroups; the last has the MMA warp, the c
 constexpr int kPieces = 4;     // places for what the planning warp says of pieces
 constexpr int kTmemCols = 512;
 constexpr int kColO = 256;     // S of tile t at 128 t (P over its first 64 columns), O at 256 + t * D
-constexpr float kLazy = 8.f;   // scores may exceed the reference by 2^8 before it is moved
+// The reference is put 2^7 below the largest score, and moved when one exceeds it by 2^15: P stays below fp16's
+// 65504, and weights down to 2^-21 of the largest are not subnormal.
+constexpr float kBelow = 7.f, kLazy = 15.f;
 // Keys seen by a unit's first token from which on K is rounded once. 16 chunks of 512 over 2560 keys: LSE is
 // off by 1.4e-6 of itself (2.4e-4 at most) in 448 us; with K in two parts for all by 5.7e-8 (1.8e-6 at most) in
 // 762 us, and O, in bf16, by as much as before. Below 512 keys one rounding could leave LSE off by 1e-4 and more.
@@ -960,9 +962,9 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
         const bool move = top > m_ref + kLazy;
         float factor = 1.f;
         if (move) {
-          factor = fast_exp2(m_ref - top);
+          factor = fast_exp2(m_ref - (top - kBelow));
           l *= factor;
-          m_ref = top;
+          m_ref = top - kBelow;
         }
         const float neg = m_ref == -INFINITY ? 0.f : -m_ref;
         // scores so large that a product's rounding matters: rounded as in the reference

@@ -8,7 +8,7 @@ import serving_engine_b200 as b200
 from oracle import q4 as oracle
 from serving_engine_b200.paged_attention import metadata_from_lists
 from tests.test_q4_gpu import DEV, make_batch, metadata
-from tests.tolerance import half_ulp
+from tests.tolerance import dtype_key, half_ulp
 
 pytestmark = pytest.mark.gpu
 
@@ -108,3 +108,37 @@ def test_queries_of_any_size(q_len, size):
     tol = (2 * 2.0 ** -11 + 2.0 ** -13) * top[..., None] + half_ulp(ro, "bf16") + 1e-6
     assert (np.abs(o.double().cpu().numpy() - ro) <= tol).all()
     assert (np.abs(lse.double().cpu().numpy() - rl) <= 1e-4 + 1e-5 * np.abs(rl)).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("q_len", [1, 2, 70])
+@pytest.mark.parametrize("gap", [10.0, 13.3, 14.7])
+def test_a_first_key_that_takes_most(dtype, d, q_len, gap):
+    """A first key with a score `gap` above all others and a V of next to nothing, as models learn it: O is what
+    the others give, and right to its own size though each of them weighs 10^-6 of the first."""
+    n, group = 20000, 4
+    blocks = -(-n // 16)
+    g = torch.Generator(device=DEV).manual_seed(d)
+    pool = b200.new_q4_pool(1, blocks, 1, d)[0]
+    k = torch.randn(n, 1, d, generator=g, device=DEV) * 0.1
+    k[0] = gap
+    v = 1 + 0.5 * torch.randn(n, 1, d, generator=g, device=DEV)
+    v[0] *= 1e-3
+    for start in range(0, n, 8192):
+        part = slice(start, min(start + 8192, n))
+        b200.kv_append_q4(k[part].to(dtype), v[part].to(dtype), pool[0], pool[1],
+                          torch.arange(part.start, part.stop, device=DEV))
+    q = (1 + 0.01 * torch.randn(q_len, group, d, generator=g, device=DEV)).to(dtype)
+    md = metadata_from_lists([q_len], [n], [0], [n - q_len], [list(range(blocks))], DEV)
+    o, lse = b200.paged_flash_attention(q, pool[0], pool[1], md, group, 1, 1.0 / d)
+    b200.check_device_errors()
+    kk, vv = (x.double().repeat_interleave(group, 1)
+              for x in b200.kv_gather_q4(pool[0], pool[1], torch.arange(n, device=DEV), d, torch.float32))
+    ref, ref_lse, size, root = reference(q, kk, vv, 1.0 / d, n - q_len, True)
+    half = torch.from_numpy(half_ulp(ref.cpu().numpy(), dtype_key(dtype))).to(DEV)
+    # roundings of each key's term on its own, as above; of sums, 2^-23 of them for each 16 keys, always down
+    bound = half + 8 * 2.6e-4 * root + n / 16 * 2.0 ** -24 * size + 2.0 ** -25
+    err = (o.double() - ref).abs()
+    assert (err <= bound).all(), float((err / bound).max())
+    assert ((lse.double() - ref_lse).abs() <= 1e-4 + 1e-5 * ref_lse.abs()).all()
