@@ -17,14 +17,12 @@
 //
 // Rounding to 16 bits: q becomes fp16 after a power of two per head that puts its
 // largest element at 2^14 (exact for bf16 and fp16 down to 2^-28 of that element);
-// p_j sV_jG becomes fp16 (unit 2^-11) after a power of two that keeps it below 2^15: each column has its
+// p_j sV_jG becomes fp16 (unit 2^-11), p_j counting from a reference that keeps it below 2^15: each column's
 // own, from the largest p_j sV_jG of the keys that it sees, so that no other key, and none of no weight,
-// costs those that count their bits (one power for a warp, from V's scales alone, took 1 to 2 % less time,
-// 84.2 us instead of 85.1 at 64 decode rows, but a stale slot could cost a few per cent of O). And
-// where O is fp16 the sum of two such numbers, a product for each: with one, O was off by 2.9e-4
-// and 3.7e-4 (256 rows, heads of 64; 2 of 120,000 keys) where its own rounding is 2.1e-4, with two by 2.1e-4
-// and 2.6e-4, for 48 us instead of 45 and 85 instead of 73. In bf16 its own rounding (1.7e-3) hides
-// either. Scores, maxima, sums and O are fp32.
+// costs those that count their bits. Where O is fp16 it is the sum of two such numbers, a product for each:
+// with one, O was off by 2.9e-4 and 3.7e-4 (256 rows, heads of 64; 2 of 120,000 keys) where its own rounding
+// is 2.1e-4, with two by 2.1e-4 and 2.6e-4, for 48 us instead of 45 and 85 instead of 73. In bf16 its own
+// rounding (1.7e-3) hides either. Scores, maxima, sums and O are fp32.
 //
 // Work: a unit is (row, tile of tokens, kv head) and its blocks, taken in pairs; the units
 // of all rows laid end to end are cut in equal runs of pairs, one per resident warp,
@@ -48,10 +46,9 @@ constexpr uint32_t kMinRun = 2;
 // What a unit's start and end cost a warp, in pairs of blocks. 256 rows of 32 to 4352 keys, heads of 64:
 // 0: 55.6 us, 1: 49.2, 2: 45.1, 3: 44.8, 4: 44.6, 6: 45.9; 64 rows of 1024 to 8192, heads of 128: 1 84.2, 2 83.6, 3 83.6.
 constexpr uint32_t kUnitCost = 2;
-constexpr float kNoMax = -FLT_MAX;  // no score yet: any score is above it by more than the threshold
-constexpr float kThreshold = 8.f;   // scores may exceed the reference by 2^8 before it is moved
-// p * V's scale stays below 2^15, and the largest of them is put at [2^8, 2^9) when its power of two is
-// taken: what is 2^-22 of that one is still not subnormal.
+// The reference of a column's exponents is where the largest p * scale is 2^8, and moved when one passes 2^15: what
+// is 2^-22 of that one is still not subnormal in fp16. (p itself stays below 2^45, in fp32.)
+constexpr float kNoMax = -FLT_MAX;  // no key yet: any score passes it
 constexpr float kScaleTop = 15.f, kScalePlace = 8.f;
 
 // Arrivals at the units that span CTAs, one for each four columns, at the CTA that a unit
@@ -97,10 +94,6 @@ __device__ __forceinline__ float log2_fast(float x) {
   float y;
   asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
-}
-// 2^e of a whole e in [-126, 127]: the sum holds 127 + e in its lowest bits. 0 for an infinity.
-__device__ __forceinline__ float power_of(float e) {
-  return __uint_as_float(__float_as_uint(e + (12582912.f + 127.f)) << 23);
 }
 // The token, of its tile, of a column.
 __device__ __forceinline__ int token_of(const Q4Params& p, int col) { return (int)(col * p.by_group >> 16); }
@@ -215,7 +208,6 @@ struct Tile {
   float qs[GR][NT][2];        // sum of q over a group, columns 8 nt + 2 t and the next
   float ch[NT][2];            // what brings a score to log2 units
   float m[NT][2], l[NT][2];   // reference, and this lane's share of the sum
-  float v_exp[NT][2];         // exponent that brings p * scale to fp16's range; inf: no key yet
   float low[GR][NT][2];       // this lane's share of sum p (low + 8 scale)
   float one[(GR + 1) / 2][NT][4];  // sum of the rounded p * scale, two groups to a tile
   float o[GR][4][NT][4];      // sum of those and the codes: n of a dim, and 16 n of the next
@@ -434,8 +426,7 @@ __device__ __forceinline__ void take_blocks(Tile<D, NT>& u, const char* place, i
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const float over = top[nt][h] - u.m[nt][h];
-      move |= over > kThreshold || over + above > -u.v_exp[nt][h];
+      move |= top[nt][h] - u.m[nt][h] + above > 0.f;
     }
   if (__any_sync(kFull, move)) {
     // move the references of the columns that need it
@@ -446,36 +437,30 @@ __device__ __forceinline__ void take_blocks(Tile<D, NT>& u, const char* place, i
         float mx = top[nt][h];
 #pragma unroll
         for (int k = 4; k <= 16; k <<= 1) mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, k));
-        const bool first = u.v_exp[nt][h] == INFINITY;
-        float up = 0.f;
-        if (mx - u.m[nt][h] > kThreshold) {
-          up = mx - u.m[nt][h];
-          u.m[nt][h] = mx;
-        }
-        float z = -INFINITY;  // log2 of the largest p * scale
+        float z = -INFINITY;  // log2 of the largest p * scale, as if the largest score were the reference
 #pragma unroll
         for (int b = 0; b < KB; ++b) {
-          z = fmaxf(z, x[b][nt][h] - u.m[nt][h] + log2_scale(most[b][0]));
-          z = fmaxf(z, x[b][nt][h + 2] - u.m[nt][h] + log2_scale(most[b][1]));
+          z = fmaxf(z, x[b][nt][h] - mx + log2_scale(most[b][0]));
+          z = fmaxf(z, x[b][nt][h + 2] - mx + log2_scale(most[b][1]));
         }
 #pragma unroll
         for (int k = 4; k <= 16; k <<= 1) z = fmaxf(z, __shfl_xor_sync(kFull, z, k));
-        // what was summed up so far went down by 2^up, and its power of two up by as much
-        float e = first ? INFINITY : kScalePlace - floorf(kScalePlace - u.v_exp[nt][h] - up);
-        if (z > kScaleTop - e) e = kScalePlace - floorf(z);
-        if (!first || z > -INFINITY) e = fminf(fmaxf(e, -20.f), 100.f);
-        const float fix = first ? 0.f : fast_exp2(-up);  // nothing is summed up yet at first
-        const float z_fix = first ? 0.f : fix * (power_of(e) / power_of(u.v_exp[nt][h]));
-        u.v_exp[nt][h] = e;
+        float fix = 1.f;
+        if (mx - u.m[nt][h] + z > kScaleTop) {
+          // at most the largest score, rounded up: scores may be so large that the sum is not exact
+          const float now = __fadd_ru(mx, fminf(z - kScalePlace, 0.f));
+          fix = fast_exp2(u.m[nt][h] - now);  // from kNoMax: 0
+          u.m[nt][h] = now;
+        }
         u.l[nt][h] *= fix;
 #pragma unroll
         for (int gr = 0; gr < GR; ++gr) {
           u.low[gr][nt][h] *= fix;
-          u.one[gr / 2][nt][(gr & 1) * 2 + h] *= z_fix;
+          u.one[gr / 2][nt][(gr & 1) * 2 + h] *= fix;
 #pragma unroll
           for (int mt = 0; mt < 4; ++mt) {
-            u.o[gr][mt][nt][h] *= z_fix;
-            u.o[gr][mt][nt][h + 2] *= z_fix;
+            u.o[gr][mt][nt][h] *= fix;
+            u.o[gr][mt][nt][h + 2] *= fix;
           }
         }
       }
@@ -485,11 +470,6 @@ __device__ __forceinline__ void take_blocks(Tile<D, NT>& u, const char* place, i
   // sum p low = sum p' (n - 8) + sum p (low + 8 scale) with p' = p scale rounded to fp16, so
   // that its rounding meets n - 8 and no more; sum p' is one more row of the product.
   // Keys that a column does not see have p = 0, and none of their parameters is used.
-  float v_down[NT][2];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-    for (int h = 0; h < 2; ++h) v_down[nt][h] = power_of(u.v_exp[nt][h]);
 #pragma unroll
   for (int b = 0; b < KB; ++b) {
 #pragma unroll
@@ -521,7 +501,7 @@ __device__ __forceinline__ void take_blocks(Tile<D, NT>& u, const char* place, i
 #pragma unroll
             for (int c = 2 * h; c < 2 * h + 2; ++c) {
               const bool hide = hidden(b, nt, c);
-              z[nt][c] = hide ? 0.f : x[b][nt][c] * v_down[nt][c & 1] * scale;
+              z[nt][c] = hide ? 0.f : x[b][nt][c] * scale;
               u.low[gr][nt][c & 1] = fmaf(x[b][nt][c], hide ? 0.f : mid, u.low[gr][nt][c & 1]);
             }
         }
@@ -719,7 +699,6 @@ __global__ void __launch_bounds__(NW * 32, CTAS) q4_attention_kernel(const Q4Par
         for (int h = 0; h < 2; ++h) {
           u.m[nt][h] = kNoMax;
           u.l[nt][h] = 0.f;
-          u.v_exp[nt][h] = INFINITY;
 #pragma unroll
           for (int gr = 0; gr < GR; ++gr) u.low[gr][nt][h] = 0.f;
         }
@@ -777,7 +756,7 @@ __global__ void __launch_bounds__(NW * 32, CTAS) q4_attention_kernel(const Q4Par
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int col = nt * 8 + 2 * t + h;
-          const float v_up = u.v_exp[nt][h] == INFINITY ? 0.f : power_of(24.f - u.v_exp[nt][h]);
+          constexpr float v_up = 16777216.f;  // 2^24, as the codes carry it
           float lt = u.l[nt][h];
 #pragma unroll
           for (int k = 4; k <= 16; k <<= 1) lt += __shfl_xor_sync(kFull, lt, k);
