@@ -286,10 +286,13 @@ __device__ __forceinline__ bool elect_one() {
       : "=r"(yes));
   return yes != 0;
 }
-// Of the 96 that a thread has at the launch. No role may spill: 16 bytes of it took the case
-// above from 453 to 483 us.
-constexpr int kRegsSoftmax = 120, kRegsK = 80, kRegsV = 80, kRegsMma = 80;
-static_assert(2 * kRegsSoftmax + kRegsK + kRegsV + kRegsMma <= 5 * 96, "the roles' registers are those of the launch");
+// Of the 96 that a thread has at the launch. No role spills: 16 bytes of it took 16 chunks of 512 tokens, heads
+// of 128, from 453 to 483 us; heads of 64 with the other's split, 8 bytes, 383 instead of 372.
+template <int D>
+struct Regs {
+  static constexpr int kSoftmax = D == 64 ? 128 : 120, kK = D == 64 ? 72 : 80, kV = 80, kMma = D == 64 ? 72 : 80;
+  static_assert(2 * kSoftmax + kK + kV + kMma <= 5 * 96, "the roles' registers are those of the launch");
+};
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params p) {
   using S = Smem<D>;
@@ -410,7 +413,7 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
   auto raw_full = [&](int i) { return wait_or_flag(raw_full_bar(i), raw_full_parity(i), failed); };
   if (warp >= 8 && warp < 12) {
     // ------------------------------------------------------------ K
-    registers_down<kRegsK>();
+    registers_down<Regs<D>::kK>();
     const int th = tid - 256;
     const int kt = th & 3, kr = th >> 2;  // for i < 4 token 32 i + kr of the tile, chunk kt of its dims
     int gk = 0;  // places of the K ring filled
@@ -509,7 +512,7 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
     }
   } else if (warp >= 12 && warp < 16) {
     // ------------------------------------------------------------ V
-    registers_down<kRegsV>();
+    registers_down<Regs<D>::kV>();
     const int th = tid - 384;
     // half block vc (of 16) and dims 8 vg ... of each group
     const int vc = (th & 7) + 8 * (th >> 6), vg = ((th >> 3) & 3) + 4 * ((th >> 5) & 1);
@@ -592,7 +595,7 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
       }
     }
   } else if (warp >= 16) {
-    registers_down<kRegsMma>();
+    registers_down<Regs<D>::kMma>();
     if (warp > 18) goto done;
     if (warp == 18) {
       // --------------------------------------------------------------- plan
@@ -825,7 +828,7 @@ __global__ void __launch_bounds__(kThreads, 1) q4_prefill_kernel(const Q4Params 
     mbar_wait_bounded(bar + 8 * kBarFinal, 0, 1u << 20);
   } else {
     // ------------------------------------------------------------ softmax
-    registers_up<kRegsSoftmax>();
+    registers_up<Regs<D>::kSoftmax>();
     const int qt = warp >> 2;
     const int m = (warp & 3) * 32 + lane;
     const uint32_t taddr = tmem + ((uint32_t)((warp & 3) * 32) << 16);
