@@ -334,7 +334,8 @@ SEB_API int seb_allreduce_add_rmsnorm(void* const* partial, void* const* x, void
  * ------------------------------------------------------------------------ */
 
 /* seb_kv_append for a 4-bit pool: quantises k_new and v_new (bf16 or fp16) into the
- * tokens' slots. Values beyond +-65504 are clamped; a group that holds an infinity or
+ * tokens' slots. A group's low is clamped to +-65504 and its scale to 65504, so that values
+ * beyond 65504 may read back as up to low + 15 * scale; a group that holds an infinity or
  * a NaN reads back as NaN. Slot -1 is a token of no row (seb_step_tables) and is
  * skipped; other slots out of range set SEB_ERRBIT_SLOT and are skipped. */
 SEB_API int seb_kv_append_q4(const void* k_new, int64_t k_stride_token, int64_t k_stride_head,
@@ -369,12 +370,14 @@ SEB_API int seb_qk_norm_rope_append(const void* qkv, int64_t qkv_stride_token, i
  * j < k_lens[r] (causal: j <= position). q, out: bf16 or fp16; the sums are fp32. A
  * query that sees no key gets O = 0 and LSE = -inf; tokens of no row are left as they
  * are. A group of V that reads back as NaN makes its own 64 dims of O NaN for the queries
- * that see its key, one of K all of their O and LSE. Rows' token ranges must not overlap
- * (rows of few tokens whose work so passes 32 bits set SEB_ERRBIT_META and are skipped).
- * A block id out of range sets SEB_ERRBIT_BLOCK_ID and its keys count as masked; a k_len
- * beyond the table sets SEB_ERRBIT_KLEN and ends there; a row outside total_query sets
- * SEB_ERRBIT_META and is skipped. Rows of q and out are 16-byte aligned. SEB_EUNSUPPORTED where the rows that no
- * chunk kernel takes (all at head_dim 256, else those of few tokens) could, with tables of
+ * that see its key, one of K all of their O and LSE. Rows of 48 / group tokens and more
+ * are chunks at head_dim 64 and 128, where total_query > num_rows: they take decoded K and V
+ * rounded to fp16 and clamped to +-65504.
+ * Rows' token ranges must not overlap (rows of few tokens whose work so passes 32 bits set
+ * SEB_ERRBIT_META and are skipped). A block id out of range sets SEB_ERRBIT_BLOCK_ID and its
+ * keys count as masked; a k_len beyond the table sets SEB_ERRBIT_KLEN and ends there; a row
+ * outside total_query sets SEB_ERRBIT_META and is skipped. Rows of q and out are 16-byte
+ * aligned. SEB_EUNSUPPORTED where the rows that are no chunks could, with tables of
  * max_blocks, come to 2^32 pairs of a tile of tokens and two blocks.
  * workspace: seb_paged_attention_q4_workspace_size(...) bytes, 16-byte aligned, of any
  * content. counter_slot: 0 .. SEB_Q4_COUNTER_SLOTS - 1, a set of the library's own

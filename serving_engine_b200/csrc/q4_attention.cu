@@ -876,7 +876,8 @@ __global__ void __launch_bounds__(NW * 32, CTAS) q4_attention_kernel(const Q4Par
 // blocks 83.7, 73.7, 13.0; 2 x 5, two blocks 98.1, 85.3, 8.8; 1 x 12, two blocks 83.4, 71.5, 14.3.
 // Heads of 64: 2 x 8 44.6 (256 rows), 2 x 7 48.7, 2 x 6 47.8; two tiles of columns of 64 (48 rows of 2
 // tokens, 3000 keys): 2 x 6, two blocks 48.7, one 49.4; 2 x 8 51.2. Two tiles of 128: 2 x 4 196 (48 rows of
-// drafts, with their chunks), 2 x 5 214.
+// drafts, with their chunks), 2 x 5 214. Heads of 256, 2 x 4 with one ring stage: 172 us (the 64 rows, bf16);
+// their two tiles of columns (groups above 8) spill some 700 bytes.
 template <int D, int NT>
 struct Shape {
   static constexpr int kSize = D / 64 * NT;  // a measure of the tile's accumulators

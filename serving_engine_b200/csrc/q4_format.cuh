@@ -79,7 +79,7 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 
 // A group's parameters from its extremes. scale and low are rounded to fp16 and the
 // codes are taken against the rounded values, so that rounding costs the group no
-// more than its ends; what lies outside +-65504 is clamped there. A group that holds
+// more than its ends; low is clamped to +-65504 and scale to 65504. A group that holds
 // an infinity or a NaN reads back as NaN in every value.
 struct Params {
   uint32_t bits;  // scale, then low

@@ -31,7 +31,7 @@
 // exponential at 16 a clock and SM, a rounding and two passes through TMEM; beside them the MMAs
 // take 1.6 us of the 3.0 us that an SM spends on 128 keys of two query tiles (head_dim 128),
 // and a unit's start and end, when the MMAs run dry, another 7. 16 rows of 512 tokens that see
-// 2560 keys, 32/8 heads of 128, bf16: 458 us, 675 TFLOP/s; 1 row of 512 that sees 32,768: 724 TFLOP/s.
+// 2560 keys, 32/8 heads of 128, bf16: 462 us, 669 TFLOP/s; 1 row of 512 that sees 32,768: 715 TFLOP/s.
 #include "q4_attention.cuh"
 #include "seb_softmax.cuh"
 #include "seb_tcgen05.cuh"
@@ -137,9 +137,10 @@ constexpr int kPlace = 8;
 // Fewer are laid end to end, kUnitPlaces places for a start and one for each key tile, and
 // cut in equal runs, one for each CTA; what is left of a unit that was cut is joined by
 // the last of its CTAs to come, in order of the parts' places. Measured, whole and cut (bf16,
-// 32/8 heads of 128): 1 row of 512 tokens that sees 32,768 keys 720 and 367 us, 1 of 64 and 131,072
-// keys 2776 and 221; but 4 rows of 512 and 4096 keys (256 units) 206 and 227. A start, with a
-// part's join, costs as much as 10 key tiles (48 rows of drafts: 3 places 205 us, 6 202, 10 196).
+// 32/8 heads of 128), with an earlier softmax: 1 row of 512 tokens that sees 32,768 keys 720 and 367 us
+// (382 now), 1 of 64 and 131,072 keys 2776 and 221 (225 now); but 4 rows of 512 and 4096 keys (256 units)
+// 206 and 227. A start, with a part's join, costs as much as 10 key tiles (48 rows of drafts: 3 places
+// 205 us, 6 202, 10 196).
 constexpr uint32_t kUnitPlaces = 10;
 // Shortest run worth a CTA. One row of 64 tokens that sees 2000 / 4000 / 8000 keys, us: 4: 40.8 / 48.4 / 66.3;
 // 8: 49.9 / 53.1 / 60.5; 12: 61.4 / 63.8 / 66.3; 20: 65.5 / 85.7 / 84.3. Where such a run would be as long as the

@@ -33,7 +33,7 @@ def rewrite_v(b, size):
         b200.kv_append_q4(k.half(), v.half(), b["pool"][0], b["pool"][1], slots)
 
 
-def weighted_bound(b, ro, causal=True, k_off=0.0):
+def weighted_bound(b, ro, causal=True):
     """What roundings may cost O: p * scale (or p) to 2^-11 of itself, weighing a code (up to 15 scale) and its
     group's offset, so 2 * 2^-11 of the sum of p |v|, |v| the largest of a key's group; 2^-13 of it for scores
     and sums in fp32; what p * scale loses to fp16's subnormals, 2^-20 of the largest p |v| (of any group) for
